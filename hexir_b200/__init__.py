@@ -11,10 +11,14 @@ this package is a thin Python face over it.
 
 from ._ffi import HexirError, lib  # noqa: F401
 from .api import (Buffer, Device, Module, Program, Rng, cuda_activation,  # noqa: F401
-                  cuda_add, cuda_matmul, cuda_matmul_acc, cuda_matmul_add, cuda_relu,
+                  cuda_add, cuda_layer_norm, cuda_layer_norm_grad, cuda_linear,
+                  cuda_linear_input_grad, cuda_linear_output_grad,
+                  cuda_linear_weight_grad,
+                  cuda_matmul, cuda_matmul_acc, cuda_matmul_add, cuda_relu,
                   cuda_synchronize, device_count, fault_calls,
-                  fault_configure,
+                  fault_configure, grad_workspace_bytes,
                   execute, kernel_image, last_kernel_ms, launch_count,
+                  linear_plan,
                   matmul_plan, parse, read_executables, read_launch,
                   read_program,
                   read_sections, shard_gather_pieces, shard_rows,

@@ -45,6 +45,20 @@ ACTIVATIONS = {"leaky_relu": 7, "elu": 8, "sigmoid": 9, "tanh": 10,
                "softmax": 11, "gelu": 12, "swish": 13, "mish": 14}
 
 
+# include/hexir_b200/layers.h
+DTYPES = {"f64": 0, "f32": 1, "bf16": 2, "f16": 3}
+LINEAR_ACTIVATIONS = {"none": 0, "relu": 3,
+                      **{k: v for k, v in ACTIVATIONS.items() if k != "softmax"}}
+LINEAR_FORCE_PAIR = 0x100
+LINEAR_FORCE_SINGLE = 0x200
+LINEAR_FORCE_SKINNY = 0x400
+LINEAR_FORCE_GUARDED = 0x800
+
+
+def LINEAR_SPLIT(s: int) -> int:
+    return (s & 0xFF) << 16
+
+
 def MATMUL_SPLIT_K(s: int) -> int:
     return (s & 0xFF) << 16
 
@@ -62,6 +76,35 @@ class Rng(C.Structure):
 _vp, _sz, _u32, _u64, _i32, _int = (C.c_void_p, C.c_size_t, C.c_uint32,
                                     C.c_uint64, C.c_int32, C.c_int)
 _dp = C.POINTER(C.c_double)
+
+
+def _struct(name: str, *groups):
+    """A ctypes structure: (type, "field field ...") groups in order."""
+    return type(name, (C.Structure,), {"_fields_": [
+        (field, kind) for kind, fields in groups for field in fields.split()]})
+
+
+# include/hexir_b200/layers.h
+LinearCall = _struct(
+    "LinearCall", (_u32, "dtype activation m n k flags"),
+    (_vp, "x w bias residual preact y"), (_u64, "ldx ldw ldr ldp ldy"))
+LinearOutputGradCall = _struct(
+    "LinearOutputGradCall", (_u32, "dtype activation m n"),
+    (_vp, "dy preact dz dbias workspace"),
+    (_u64, "workspace_bytes lddy ldp lddz"))
+LinearInputGradCall = _struct(
+    "LinearInputGradCall", (_u32, "dtype activation m n k flags"),
+    (_vp, "dz w preact residual dx"), (_u64, "lddz ldw ldp ldr lddx"))
+LinearWeightGradCall = _struct(
+    "LinearWeightGradCall", (_u32, "dtype reserved m n k flags"),
+    (_vp, "x dz dw"), (_u64, "ldx lddz lddw"))
+LayerNormCall = _struct(
+    "LayerNormCall", (_u32, "dtype cols"), (_u64, "rows"), (C.c_double, "eps"),
+    (_vp, "x gamma beta y mean rstd"), (_u64, "ldx ldy"))
+LayerNormGradCall = _struct(
+    "LayerNormGradCall", (_u32, "dtype cols"), (_u64, "rows"),
+    (_vp, "dy x mean rstd gamma residual dx dgamma dbeta workspace"),
+    (_u64, "workspace_bytes lddy ldx ldr lddx"))
 
 # (name, restype, argtypes)
 _SIGNATURES = [
@@ -133,6 +176,21 @@ _SIGNATURES = [
     ("hexir_cuda_sm_count", _int, [_int]),
     ("hexir_cuda_kernel_image", _int, [C.POINTER(_vp), C.POINTER(_sz)]),
     ("hexir_cuda_last_error", C.c_char_p, []),
+    # hexir_b200/layers.h
+    ("hexir_cuda_linear", _int, [_int, C.POINTER(LinearCall), _vp]),
+    ("hexir_cuda_linear_output_grad", _int,
+     [_int, C.POINTER(LinearOutputGradCall), _vp]),
+    ("hexir_cuda_linear_input_grad", _int,
+     [_int, C.POINTER(LinearInputGradCall), _vp]),
+    ("hexir_cuda_linear_weight_grad", _int,
+     [_int, C.POINTER(LinearWeightGradCall), _vp]),
+    ("hexir_cuda_linear_plan", _int,
+     [_int, _u32, _u32, _u32, _u32, _int, _u32, C.POINTER(_u32),
+      C.POINTER(_u32), C.POINTER(_u32)]),
+    ("hexir_cuda_grad_workspace", _u64, [_u32, _u32]),
+    ("hexir_cuda_layer_norm", _int, [_int, C.POINTER(LayerNormCall), _vp]),
+    ("hexir_cuda_layer_norm_grad", _int,
+     [_int, C.POINTER(LayerNormGradCall), _vp]),
     # hexir_b200/comm.h
     ("hexir_shard_rows", _int, [_u64, _u32, _u32, C.POINTER(_u64),
                                 C.POINTER(_u64)]),

@@ -458,6 +458,130 @@ def cuda_activation(ordinal: int, op, x: int, y: int, rows: int, cols: int,
           "hexir_cuda_activation_f64")
 
 
+# ----------------------------------------------------------------- layers
+#
+# A feed-forward block's layers (include/hexir_b200/layers.h).  Pointers are
+# device addresses, 0 = absent; ld* are row strides in elements, 0 = dense;
+# dtype is a name of _ffi.DTYPES, activation one of _ffi.LINEAR_ACTIVATIONS.
+
+
+def _dtype(dtype) -> int:
+    if dtype not in _ffi.DTYPES:
+        raise ValueError(f"unknown dtype {dtype!r}: one of {sorted(_ffi.DTYPES)}")
+    return _ffi.DTYPES[dtype]
+
+
+def _activation(act) -> int:
+    if act not in _ffi.LINEAR_ACTIVATIONS:
+        raise ValueError(f"unknown activation {act!r}: one of "
+                         f"{sorted(_ffi.LINEAR_ACTIVATIONS)}")
+    return _ffi.LINEAR_ACTIVATIONS[act]
+
+
+def cuda_linear(ordinal: int, x: int, w: int, y: int, m: int, n: int, k: int,
+                dtype: str = "bf16", activation: str = "none", *, bias: int = 0,
+                residual: int = 0, preact: int = 0, ldx: int = 0, ldw: int = 0,
+                ldy: int = 0, ldr: int = 0, ldp: int = 0, flags: int = 0,
+                stream: int = 0) -> None:
+    """y = activation(x . w + bias) + residual for x [m][k], w [k][n], bf16 or
+    f16; preact (optional) receives x . w + bias (hexir_cuda_linear)."""
+    call = _ffi.LinearCall(_dtype(dtype), _activation(activation), m, n, k, flags,
+                           x, w, bias, residual, preact, y, ldx, ldw, ldr, ldp, ldy)
+    check(lib().hexir_cuda_linear(ordinal, C.byref(call), stream or None),
+          "hexir_cuda_linear")
+
+
+def cuda_linear_output_grad(ordinal: int, dy: int, m: int, n: int,
+                            dtype: str = "bf16", activation: str = "none", *,
+                            preact: int = 0, dz: int = 0, dbias: int = 0,
+                            workspace: int = 0, workspace_bytes: int = 0,
+                            lddy: int = 0, ldp: int = 0, lddz: int = 0,
+                            stream: int = 0) -> None:
+    """dz = dy * activation'(preact) and dbias = the column sums of dz
+    (hexir_cuda_linear_output_grad); dbias needs a workspace of
+    grad_workspace_bytes(n, dtype)."""
+    call = _ffi.LinearOutputGradCall(_dtype(dtype), _activation(activation), m, n,
+                                     dy, preact, dz, dbias, workspace,
+                                     workspace_bytes, lddy, ldp, lddz)
+    check(lib().hexir_cuda_linear_output_grad(ordinal, C.byref(call),
+                                              stream or None),
+          "hexir_cuda_linear_output_grad")
+
+
+def cuda_linear_input_grad(ordinal: int, dz: int, w: int, dx: int, m: int, n: int,
+                           k: int, dtype: str = "bf16", activation: str = "none",
+                           *, preact: int = 0, residual: int = 0, lddz: int = 0,
+                           ldw: int = 0, lddx: int = 0, ldp: int = 0, ldr: int = 0,
+                           flags: int = 0, stream: int = 0) -> None:
+    """dx = (dz . w^T) * activation'(preact) + residual, with the activation
+    and preactivations of the layer whose output this layer's input was
+    (hexir_cuda_linear_input_grad)."""
+    call = _ffi.LinearInputGradCall(_dtype(dtype), _activation(activation), m, n, k,
+                                    flags, dz, w, preact, residual, dx, lddz, ldw,
+                                    ldp, ldr, lddx)
+    check(lib().hexir_cuda_linear_input_grad(ordinal, C.byref(call), stream or None),
+          "hexir_cuda_linear_input_grad")
+
+
+def cuda_linear_weight_grad(ordinal: int, x: int, dz: int, dw: int, m: int, n: int,
+                            k: int, dtype: str = "bf16", *, ldx: int = 0,
+                            lddz: int = 0, lddw: int = 0, flags: int = 0,
+                            stream: int = 0) -> None:
+    """dw = x^T . dz, [k][n] (hexir_cuda_linear_weight_grad)."""
+    call = _ffi.LinearWeightGradCall(_dtype(dtype), 0, m, n, k, flags, x, dz, dw,
+                                     ldx, lddz, lddw)
+    check(lib().hexir_cuda_linear_weight_grad(ordinal, C.byref(call),
+                                              stream or None),
+          "hexir_cuda_linear_weight_grad")
+
+
+def linear_plan(op: str, m: int, n: int, k: int, aligned: bool = True,
+                flags: int = 0, ordinal: int = 0) -> tuple:
+    """(variant, tile_n, split) a product would run with: op is "forward",
+    "input_grad" or "weight_grad"; variant 1 = CTA pairs, 2 = single CTAs,
+    3 = skinny, 4 = guarded loads (hexir_cuda_linear_plan)."""
+    ops = ("forward", "input_grad", "weight_grad")
+    out = [C.c_uint32() for _ in range(3)]
+    check(lib().hexir_cuda_linear_plan(ordinal, ops.index(op), m, n, k,
+                                       int(aligned), flags, *map(C.byref, out)),
+          "hexir_cuda_linear_plan")
+    return tuple(v.value for v in out)
+
+
+def grad_workspace_bytes(cols: int, dtype: str = "bf16") -> int:
+    """Workspace of the two calls that sum over rows
+    (hexir_cuda_grad_workspace)."""
+    return lib().hexir_cuda_grad_workspace(cols, _dtype(dtype))
+
+
+def cuda_layer_norm(ordinal: int, x: int, y: int, rows: int, cols: int,
+                    dtype: str = "f64", *, gamma: int = 0, beta: int = 0,
+                    mean: int = 0, rstd: int = 0, eps: float = 1e-5, ldx: int = 0,
+                    ldy: int = 0, stream: int = 0) -> None:
+    """y = (x - mean) * rstd * gamma + beta along each row; mean and rstd
+    (optional outputs, [rows]) are f32, f64 for f64 (hexir_cuda_layer_norm)."""
+    call = _ffi.LayerNormCall(_dtype(dtype), cols, rows, eps, x, gamma, beta, y,
+                              mean, rstd, ldx, ldy)
+    check(lib().hexir_cuda_layer_norm(ordinal, C.byref(call), stream or None),
+          "hexir_cuda_layer_norm")
+
+
+def cuda_layer_norm_grad(ordinal: int, dy: int, x: int, mean: int, rstd: int,
+                         dx: int, rows: int, cols: int, dtype: str = "f64", *,
+                         gamma: int = 0, dgamma: int = 0, dbeta: int = 0,
+                         residual: int = 0, workspace: int = 0,
+                         workspace_bytes: int = 0, lddy: int = 0, ldx: int = 0,
+                         lddx: int = 0, ldr: int = 0, stream: int = 0) -> None:
+    """Layer norm's gradient: dx (+ residual), dgamma and dbeta
+    (hexir_cuda_layer_norm_grad); dgamma and dbeta need a workspace of
+    grad_workspace_bytes(cols, dtype)."""
+    call = _ffi.LayerNormGradCall(_dtype(dtype), cols, rows, dy, x, mean, rstd,
+                                  gamma, residual, dx, dgamma, dbeta, workspace,
+                                  workspace_bytes, lddy, ldx, ldr, lddx)
+    check(lib().hexir_cuda_layer_norm_grad(ordinal, C.byref(call), stream or None),
+          "hexir_cuda_layer_norm_grad")
+
+
 def cuda_synchronize(ordinal: int, stream: int = 0) -> None:
     check(lib().hexir_cuda_synchronize(ordinal, stream or None),
           "hexir_cuda_synchronize")

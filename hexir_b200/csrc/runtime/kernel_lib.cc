@@ -27,9 +27,6 @@ std::map<int, std::unique_ptr<DeviceState>> g_devices;
 std::atomic<uint64_t> g_launches{0};
 thread_local std::string g_last_error;
 
-// Every pipeline wait in the kernels gives up after this much wall time.
-constexpr uint64_t kWaitTimeoutNs = 4000000000ull;
-
 bool aligned16(const void *p) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
 }
@@ -38,12 +35,16 @@ uint32_t ceil_div(uint64_t a, uint64_t b) {
   return static_cast<uint32_t>((a + b - 1) / b);
 }
 
+}  // namespace
+
 hexir_status_t fail(std::string *error, std::string message,
-                    hexir_status_t status = HEXIR_ERROR_DEVICE) {
+                    hexir_status_t status) {
   if (error)
     *error = std::move(message);
   return status;
 }
+
+namespace {
 
 // Workspace for split-K partials: grown on demand, never shrunk.  Growing
 // frees the old block only after the context is idle.
@@ -67,6 +68,8 @@ hexir_status_t ensure_workspace(DeviceState *dev, size_t bytes,
   return HEXIR_OK;
 }
 
+}  // namespace
+
 hexir_status_t launch(CUfunction fn, unsigned gx, unsigned gy, unsigned bx,
                       unsigned smem, CUstream stream, void **params,
                       const char *what, std::string *error) {
@@ -80,8 +83,7 @@ hexir_status_t launch(CUfunction fn, unsigned gx, unsigned gy, unsigned bx,
   return HEXIR_OK;
 }
 
-// A launch that depends on the kernel queued before it on `stream` only
-// through memory: with programmatic stream serialization its CTAs may be
+// launch_after: with programmatic stream serialization its CTAs may be
 // placed while that kernel's last CTAs run, and the kernel itself waits
 // (griddepcontrol.wait) for that kernel's completion before reading.  Hides
 // the launch gap between a GEMM and its split-K reduction or stream-K
@@ -115,6 +117,8 @@ hexir_status_t launch_after(CUfunction fn, unsigned gx, unsigned gy,
   count_launch();
   return HEXIR_OK;
 }
+
+namespace {
 
 // The launch configuration of `gx` CTAs in clusters of `cluster` along x.
 struct ClusterLaunch {
@@ -156,6 +160,8 @@ unsigned max_active_clusters(CUfunction fn, unsigned cluster, unsigned bx,
              : 0u;
 }
 
+}  // namespace
+
 // A launch with a cluster shape of `cluster` CTAs along x.
 hexir_status_t launch_cluster(CUfunction fn, unsigned gx, unsigned cluster,
                               unsigned bx, unsigned smem, CUstream stream,
@@ -173,6 +179,8 @@ hexir_status_t launch_cluster(CUfunction fn, unsigned gx, unsigned cluster,
   count_launch();
   return HEXIR_OK;
 }
+
+namespace {
 
 unsigned stream_grid(const DeviceState *dev, uint64_t pairs) {
   // Four 16-byte vectors per thread per pass, 256 threads per CTA; at most
@@ -899,18 +907,22 @@ hexir_status_t check_device(DeviceState *dev, CUstream stream,
   if (r != CUDA_SUCCESS)
     return fail(error, cuda_message("kernel execution", r));
   std::lock_guard<std::mutex> lock(dev->mu);
+  std::vector<CUdeviceptr> words;
+  for (auto &entry : dev->libs)
+    words.push_back(entry.second->error_word);
+  if (dev->layers)
+    words.push_back(layers_error_word(dev->layers));
   unsigned int bits = 0;
-  for (auto &entry : dev->libs) {
-    KernelLib *lib = entry.second.get();
+  for (CUdeviceptr at : words) {
     unsigned int word = 0;
-    r = d.MemcpyDtoHAsync(&word, lib->error_word, sizeof(word), stream);
+    r = d.MemcpyDtoHAsync(&word, at, sizeof(word), stream);
     if (r == CUDA_SUCCESS)
       r = d.StreamSynchronize(stream);
     if (r != CUDA_SUCCESS)
       return fail(error, cuda_message("reading the device error word", r));
     if (word) {
       bits |= word;
-      d.MemsetD8Async(lib->error_word, 0, sizeof(word), stream);
+      d.MemsetD8Async(at, 0, sizeof(word), stream);
       d.StreamSynchronize(stream);
     }
   }

@@ -50,6 +50,13 @@ struct KernelLib {
   CUdeviceptr error_word = 0;
 };
 
+// The layer kernels' module on one device (layers.cc).
+struct LayersLib;
+CUdeviceptr layers_error_word(const LayersLib *lib);
+
+// Every pipeline wait in the kernels gives up after this much wall time.
+constexpr uint64_t kWaitTimeoutNs = 4000000000ull;
+
 struct DeviceState {
   int ordinal = -1;
   CUdevice device = 0;
@@ -60,6 +67,7 @@ struct DeviceState {
   std::mutex mu;
   std::map<uint64_t, std::unique_ptr<KernelLib>> libs;  // by image hash
   KernelLib *embedded = nullptr;
+  LayersLib *layers = nullptr;  // loaded by the first layer call, under mu
 
   // split-K partial sums; reuse across streams is ordered by `ws_ready`.
   CUdeviceptr workspace = 0;
@@ -139,6 +147,25 @@ hexir_status_t check_device(DeviceState *dev, CUstream stream,
 // 1024 k at 8192 rows and columns over PCIe) ends before the previous
 // pieces' compute (~3.9 ms per 1024 k) does.
 std::vector<uint32_t> weight_stream_bounds(uint32_t k1);
+
+// Set *error and return `status`.
+hexir_status_t fail(std::string *error, std::string message,
+                    hexir_status_t status = HEXIR_ERROR_DEVICE);
+
+// Launch helpers (fault injection, launch count, error message): a plain
+// launch; one that depends on the kernel queued before it on `stream` only
+// through memory and may be placed while that kernel's last CTAs run; and one
+// with a cluster shape of `cluster` CTAs along x.
+hexir_status_t launch(CUfunction fn, unsigned gx, unsigned gy, unsigned bx,
+                      unsigned smem, CUstream stream, void **params,
+                      const char *what, std::string *error);
+hexir_status_t launch_after(CUfunction fn, unsigned gx, unsigned gy,
+                            unsigned bx, CUstream stream, void **params,
+                            const char *what, std::string *error);
+hexir_status_t launch_cluster(CUfunction fn, unsigned gx, unsigned cluster,
+                              unsigned bx, unsigned smem, CUstream stream,
+                              void **params, const char *what,
+                              std::string *error);
 
 void count_launch();
 void set_last_error(const std::string &message);

@@ -1,0 +1,865 @@
+// layers.cc -- the layer calls (include/hexir_b200/layers.h): argument
+// checks, kernel choice and launches of the kernels in kernels/layers.cu.
+
+#include "hexir_b200/layers.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <initializer_list>
+#include <limits>
+
+#include "../kernels/launch_abi.h"
+#include "../kernels/layers_abi.h"
+#include "cuda_driver.h"
+#include "kernel_lib.h"
+
+extern "C" {
+extern const unsigned char hexir_layers_cubin_begin[];
+}
+
+namespace hexir {
+
+namespace {
+
+constexpr int kNormShapes = 7;
+// Threads per row (32: a warp, 8 rows per block) and elements per thread.
+constexpr struct {
+  uint32_t threads, elements;
+} kNorm[kNormShapes] = {{32, 8},   {32, 16},  {32, 32},  {256, 8},
+                        {256, 16}, {512, 16}, {1024, 16}};
+
+const char *const kDtypeName[4] = {"f64", "f32", "bf16", "f16"};
+constexpr uint32_t kDtypeSize[4] = {8, 4, 2, 2};
+
+}  // namespace
+
+struct LayersLib {
+  CUmodule module = nullptr;
+  CUdeviceptr error_word = 0;
+  // By HEXIR_PRODUCT_*; skinny is the forward's only.
+  CUfunction pair[3] = {}, single[3] = {}, guarded[3] = {}, skinny = nullptr;
+  // By dtype.
+  CUfunction norm[4][kNormShapes] = {}, norm_wide[4] = {};
+  CUfunction norm_grad[4][kNormShapes] = {}, norm_grad_wide[4] = {},
+             norm_grad_columns[4] = {}, norm_grad_join[4] = {};
+  CUfunction output_grad[4] = {}, output_grad_join[4] = {};
+};
+
+CUdeviceptr layers_error_word(const LayersLib *lib) { return lib->error_word; }
+
+namespace {
+
+// The most dynamic shared memory any of the product kernels is launched with.
+constexpr uint32_t kSmemLimit = 227u * 1024u - 1024u;
+
+LayersLib *layers_library(DeviceState *dev, std::string *error) {
+  std::lock_guard<std::mutex> lock(dev->mu);
+  if (dev->layers)
+    return dev->layers;
+  const Driver &d = driver();
+  ContextGuard guard(dev->context);
+  auto lib = std::make_unique<LayersLib>();
+  CUresult r = d.ModuleLoadData(&lib->module, hexir_layers_cubin_begin);
+  if (r != CUDA_SUCCESS) {
+    fail(error, cuda_message("cuModuleLoadData", r) +
+                    " (the layer kernels are built for sm_100a)");
+    return nullptr;
+  }
+  std::string missing;
+  auto get = [&](CUfunction *slot, const std::string &name) {
+    if (d.ModuleGetFunction(slot, lib->module, name.c_str()) != CUDA_SUCCESS &&
+        missing.empty())
+      missing = name;
+  };
+  const char *const products[3] = {"hexir_linear_16", "hexir_linear_16_input_grad",
+                                   "hexir_linear_16_weight_grad"};
+  for (int i = 0; i < 3; ++i) {
+    const std::string base = products[i];
+    get(&lib->pair[i], base + "_pair");
+    get(&lib->single[i], base + "_single");
+    get(&lib->guarded[i], base + "_guarded");
+  }
+  get(&lib->skinny, "hexir_linear_16_skinny");
+  for (int t = 0; t < 4; ++t) {
+    const std::string norm = std::string("hexir_layer_norm_") + kDtypeName[t];
+    const std::string grad = std::string("hexir_layer_norm_grad_") + kDtypeName[t];
+    for (int s = 0; s < kNormShapes; ++s) {
+      const std::string shape = "_" + std::to_string(kNorm[s].threads) + "x" +
+                                std::to_string(kNorm[s].elements);
+      get(&lib->norm[t][s], norm + shape);
+      get(&lib->norm_grad[t][s], grad + shape);
+    }
+    get(&lib->norm_wide[t], norm + "_wide");
+    get(&lib->norm_grad_wide[t], grad + "_wide");
+    get(&lib->norm_grad_columns[t], grad + "_columns");
+    get(&lib->norm_grad_join[t], grad + "_join");
+    if (t >= static_cast<int>(HEXIR_DTYPE_BF16)) {
+      const std::string out = std::string("hexir_linear_output_grad_") + kDtypeName[t];
+      get(&lib->output_grad[t], out);
+      get(&lib->output_grad_join[t], out + "_join");
+    }
+  }
+  if (!missing.empty()) {
+    d.ModuleUnload(lib->module);
+    fail(error, "the layer kernels lack " + missing);
+    return nullptr;
+  }
+  size_t bytes = 0;
+  r = d.ModuleGetGlobal(&lib->error_word, &bytes, lib->module,
+                        "hexir_device_error_word");
+  for (int i = 0; i < 3 && r == CUDA_SUCCESS; ++i)
+    for (CUfunction fn : {lib->pair[i], lib->single[i], lib->guarded[i]})
+      if (r == CUDA_SUCCESS)
+        r = d.FuncSetAttribute(fn, CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES,
+                               kSmemLimit);
+  if (r == CUDA_SUCCESS)
+    r = d.FuncSetAttribute(lib->skinny,
+                           CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES,
+                           kSmemLimit);
+  if (r != CUDA_SUCCESS) {
+    d.ModuleUnload(lib->module);
+    fail(error, cuda_message("layer kernels setup", r));
+    return nullptr;
+  }
+  dev->layers = lib.release();
+  return dev->layers;
+}
+
+struct Call {
+  DeviceState *dev = nullptr;
+  LayersLib *lib = nullptr;
+  std::string error;
+  bool open(int ordinal) {
+    dev = device_state(ordinal, &error);
+    lib = dev ? layers_library(dev, &error) : nullptr;
+    return lib != nullptr;
+  }
+  hexir_status_t finish(hexir_status_t status) {
+    if (status != HEXIR_OK)
+      set_last_error(error.empty() ? hexir_status_string(status) : error);
+    return status;
+  }
+  hexir_status_t refuse(std::string message,
+                        hexir_status_t status = HEXIR_ERROR_INVALID_ARGUMENT) {
+    error = std::move(message);
+    return finish(status);
+  }
+};
+
+uint32_t ceil_div(uint64_t a, uint64_t b) {
+  return static_cast<uint32_t>((a + b - 1) / b);
+}
+
+bool off(const void *p, uint32_t bytes) {
+  return reinterpret_cast<uintptr_t>(p) % bytes != 0;
+}
+
+// Rows that start on 16-byte boundaries: what TMA and 16-byte accesses need.
+bool rows16(const void *p, uint64_t ld, uint32_t size) {
+  return !off(p, 16) && ld * size % 16 == 0;
+}
+
+// One tensor argument: its row stride made explicit, and checked.
+struct Tensor {
+  const char *name;
+  const void *p;
+  uint64_t *ld;
+  uint64_t rows, cols;
+};
+
+// Empty if fine.  Element alignment matters: a kernel's access off it faults.
+std::string check_tensors(const char *op, uint32_t size,
+                          std::initializer_list<Tensor> tensors) {
+  for (const Tensor &t : tensors) {
+    if (*t.ld == 0)
+      *t.ld = t.cols;
+    if (t.p && off(t.p, size))
+      return std::string(op) + ": " + t.name + " is not aligned to its elements";
+    if (*t.ld < t.cols)
+      return std::string(op) + ": the row stride of " + t.name +
+             " is smaller than its row";
+    // Byte offsets stay within 63 bits.
+    if (t.rows && *t.ld > (std::numeric_limits<uint64_t>::max() >> 4) / t.rows)
+      return std::string(op) + ": " + t.name + " is too large";
+    if (t.rows <= 1)  // one row has no stride: leave it aligned
+      *t.ld = (t.cols + 15) / 16 * 16;
+  }
+  return std::string();
+}
+
+bool linear_activation(uint32_t a) {
+  return a == HEXIR_ACTIVATION_NONE || a == HEXIR_ACTIVATION_RELU ||
+         (a >= HEXIR_ACTIVATION_LEAKY_RELU && a <= HEXIR_ACTIVATION_MISH &&
+          a != HEXIR_ACTIVATION_SOFTMAX);
+}
+
+// What the linear calls share.
+std::string check_linear(const char *op, uint32_t dtype, uint32_t activation,
+                         uint32_t flags, hexir_status_t *status) {
+  *status = HEXIR_ERROR_INVALID_ARGUMENT;
+  if (dtype == HEXIR_DTYPE_F64 || dtype == HEXIR_DTYPE_F32) {
+    *status = HEXIR_ERROR_UNIMPLEMENTED;
+    return std::string(op) + ": bf16 or f16 only (f64: hexir_cuda_matmul_add_f64)";
+  }
+  if (dtype > HEXIR_DTYPE_F16)
+    return std::string(op) + ": unknown dtype " + std::to_string(dtype);
+  if (!linear_activation(activation))
+    return std::string(op) + ": no such elementwise activation " +
+           std::to_string(activation);
+  const uint32_t forces = flags & 0xF00u;
+  if ((flags & ~0xFF0F00u) || (forces & (forces - 1)))
+    return std::string(op) + ": unknown flags";
+  const uint32_t split = flags >> 16;
+  if (split && split != 1 && split != 2 && split != 4 && split != 8)
+    return std::string(op) + ": the split is 1, 2, 4 or 8";
+  return std::string();
+}
+
+// ------------------------------------------------------------ the products
+
+enum ProductVariant { kPair = 1, kSingle = 2, kSkinny = 3, kGuardedLoads = 4 };
+
+struct ProductPlan {
+  uint32_t variant = 0;
+  uint32_t tile_n = 0, split = 1, stages = 0;
+  uint32_t tiles_m = 0, tiles_n = 0;
+  uint32_t tmem_cols = 0, smem = 0;
+  std::string refusal;  // a forced kernel that cannot run this
+};
+
+uint32_t stage_bytes(uint32_t tile_n) {
+  return HEXIR_PRODUCT_BM * 128u + tile_n * 128u;
+}
+
+ProductPlan plan_product(uint32_t op, uint32_t m, uint32_t n, uint32_t k,
+                         bool aligned, uint32_t flags, uint32_t sms) {
+  // out [rows][cols], summed over depth.
+  const uint32_t rows = op == HEXIR_PRODUCT_WEIGHT_GRAD ? k : m;
+  const uint32_t cols = op == HEXIR_PRODUCT_INPUT_GRAD ? k : n;
+  const uint32_t depth = op == HEXIR_PRODUCT_FORWARD      ? k
+                         : op == HEXIR_PRODUCT_INPUT_GRAD ? n
+                                                          : m;
+  const uint32_t k_tiles = ceil_div(depth, HEXIR_PRODUCT_BK);
+  const uint32_t forced_split = flags >> 16;
+  ProductPlan p;
+  const bool tma = aligned && depth > 0;
+  const bool skinny = tma && op == HEXIR_PRODUCT_FORWARD && m <= 64;
+  if (flags & HEXIR_LINEAR_FORCE_GUARDED) {
+    p.variant = kGuardedLoads;
+  } else if (flags & HEXIR_LINEAR_FORCE_SKINNY) {
+    p.variant = kSkinny;
+    if (!skinny)
+      p.refusal = "the skinny kernel needs aligned rows, the forward and m <= 64";
+  } else if (flags & (HEXIR_LINEAR_FORCE_PAIR | HEXIR_LINEAR_FORCE_SINGLE)) {
+    p.variant = flags & HEXIR_LINEAR_FORCE_PAIR ? kPair : kSingle;
+    if (!tma)
+      p.refusal = "the TMA kernels need aligned rows and a sum that is not empty";
+  } else if (!tma) {
+    p.variant = kGuardedLoads;
+  } else if (skinny) {
+    p.variant = kSkinny;
+  }
+  if (!p.refusal.empty())
+    return p;
+
+  const uint32_t max_split = std::max<uint32_t>(
+      1, k_tiles >= 32 ? 8 : (k_tiles >= 16 ? 4 : (k_tiles >= 8 ? 2 : 1)));
+  if (p.variant == kSkinny) {
+    p.tile_n = (std::max<uint32_t>(m, 1) + 15) / 16 * 16;
+    p.tiles_m = ceil_div(n, HEXIR_PRODUCT_BM);
+    p.tiles_n = 1;
+    // The weight stream is the cost: CTAs for every SM, two per SM.
+    while (p.split < max_split && p.tiles_m * p.split * 2 <= 2 * sms)
+      p.split *= 2;
+    p.stages = std::min<uint32_t>(HEXIR_SINGLE_MAX_STAGES,
+                                  100u * 1024u / stage_bytes(p.tile_n));
+    p.tmem_cols = p.tile_n <= 32 ? 32 : 64;
+  } else {
+    if (p.variant == 0 || p.variant == kPair) {
+      // Modelled cycles: waves of tiles, each its k-tiles plus a fill and an
+      // epilogue.
+      double best = 0;
+      uint32_t best_variant = 0, best_n = 0, best_split = 1;
+      for (uint32_t tile_n : {256u, 128u}) {
+        const uint64_t tiles = static_cast<uint64_t>(ceil_div(rows, 256)) *
+                               ceil_div(cols, tile_n);
+        const uint64_t waves = (tiles + sms / 2 - 1) / std::max<uint32_t>(sms / 2, 1);
+        const double t = waves * (k_tiles * 2.15 * tile_n + 600.0) + 3500.0;
+        if (best_variant == 0 || t < best) {
+          best = t;
+          best_variant = kPair;
+          best_n = tile_n;
+        }
+      }
+      if (p.variant == 0) {
+        for (uint32_t tile_n : {128u, 64u})
+          for (uint32_t split = 1; split <= max_split; split *= 2) {
+            const uint64_t ctas = static_cast<uint64_t>(ceil_div(rows, 128)) *
+                                  ceil_div(cols, tile_n) * split;
+            const uint64_t waves = (ctas + sms - 1) / sms;
+            const double t =
+                waves * (ceil_div(k_tiles, split) * (tile_n == 128 ? 300.0 : 220.0) +
+                         800.0) + 3000.0 + (split > 1 ? 1500.0 : 0.0);
+            if (t < best) {
+              best = t;
+              best_variant = kSingle;
+              best_n = tile_n;
+              best_split = split;
+            }
+          }
+      }
+      p.variant = best_variant;
+      p.tile_n = best_n;
+      p.split = best_split;
+    } else {
+      p.tile_n = 128;
+      const uint64_t tiles = static_cast<uint64_t>(ceil_div(rows, 128)) *
+                             ceil_div(cols, 128);
+      while (p.split < max_split && tiles * p.split * 2 <= sms)
+        p.split *= 2;
+    }
+    if (p.variant == kPair) {
+      p.tiles_m = ceil_div(rows, 2 * HEXIR_PRODUCT_BM);
+      p.tiles_n = ceil_div(cols, p.tile_n);
+      p.smem = HEXIR_PAIR_SMEM_BYTES;
+      p.split = 1;
+      if (forced_split > 1)
+        p.refusal = "CTA pairs do not split the sum";
+      return p;
+    }
+    p.tiles_m = ceil_div(rows, HEXIR_PRODUCT_BM);
+    p.tiles_n = ceil_div(cols, p.tile_n);
+    // One CTA per SM with a deep ring, or two whose main loops and epilogues
+    // overlap.
+    const uint64_t ctas = static_cast<uint64_t>(p.tiles_m) * p.tiles_n * p.split;
+    p.stages = (ctas <= sms ? 196u : 100u) * 1024u / stage_bytes(p.tile_n);
+    p.stages = std::min<uint32_t>(p.stages, HEXIR_SINGLE_MAX_STAGES);
+    p.tmem_cols = p.tile_n;
+  }
+  if (forced_split)
+    p.split = forced_split;
+  // Shared memory: at least what keeps the TMEM columns of the CTAs that fit
+  // an SM within its 512 (a CTA that waits for columns while it holds a place
+  // in a cluster could wait on a cluster that waits for it): 227 KiB / 512
+  // columns = 454 bytes per column.
+  const uint32_t ring = p.stages * stage_bytes(p.tile_n);
+  p.smem = std::max<uint32_t>(ring, p.tmem_cols * 512u) + 1024u;
+  return p;
+}
+
+struct Operand {
+  const void *p;
+  uint64_t ld;
+  bool mn;             // MN-major: rows along the summed index
+  uint32_t side, box;  // extent of the tile's side, and of a box along it
+};
+
+CUresult encode(CUtensorMap *map, const Operand &o, uint32_t depth, bool f16) {
+  const cuuint64_t dims[2] = {o.mn ? o.side : depth, o.mn ? depth : o.side};
+  const cuuint64_t strides[1] = {o.ld * 2};
+  const cuuint32_t box[2] = {64, o.mn ? 64u : o.box};
+  const cuuint32_t unit[2] = {1, 1};
+  return driver().TensorMapEncodeTiled(
+      map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+      2, const_cast<void *>(o.p), dims, strides, box, unit,
+      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+// out[rows][cols] = a . b over depth with op's epilogue (args: everything but
+// the tiling).  a and b as the product has them: x and w, dz and w, x and dz.
+hexir_status_t launch_product(Call &call, uint32_t op, uint32_t m, uint32_t n,
+                              uint32_t k, uint32_t flags,
+                              hexir_product_args_t &args, CUstream stream) {
+  if (args.rows == 0 || args.cols == 0)
+    return HEXIR_OK;
+  const bool a_mn = op == HEXIR_PRODUCT_WEIGHT_GRAD;
+  const bool b_mn = op != HEXIR_PRODUCT_INPUT_GRAD;
+  const bool aligned = rows16(args.a, args.lda, 2) && rows16(args.b, args.ldb, 2) &&
+                       args.lda < 1ull << 39 && args.ldb < 1ull << 39;
+  const uint32_t sms = static_cast<uint32_t>(std::max(call.dev->sm_count, 2));
+  const ProductPlan p = plan_product(op, m, n, k, aligned, flags, sms);
+  if (!p.refusal.empty())
+    return fail(&call.error, "linear: " + p.refusal, HEXIR_ERROR_INVALID_ARGUMENT);
+  const uint64_t tiles = static_cast<uint64_t>(p.tiles_m) * p.tiles_n;
+  if (tiles * p.split > 0x7FFFFFFFull)
+    return fail(&call.error, "linear: too many tiles", HEXIR_ERROR_INVALID_ARGUMENT);
+
+  args.tiles_m = p.tiles_m;
+  args.tiles_n = p.tiles_n;
+  args.group_m = std::min<uint32_t>(8, p.tiles_m);
+  args.tile_n = p.tile_n;
+  args.k_tiles = ceil_div(args.depth, HEXIR_PRODUCT_BK);
+  args.split = p.split;
+  args.stages = p.stages;
+  args.tmem_cols = p.tmem_cols;
+  args.timeout_ns = kWaitTimeoutNs;
+  args.vec = rows16(args.out, args.ldo, 2) &&
+             (!args.preact_out || rows16(args.preact_out, args.ldp, 2)) &&
+             (!args.bias || !off(args.bias, 16)) &&
+             (!args.residual || rows16(args.residual, args.ldr, 2)) &&
+             (!args.slope_at || rows16(args.slope_at, args.lds, 2));
+
+  const unsigned grid = static_cast<unsigned>(tiles * p.split);
+  if (p.variant == kGuardedLoads) {
+    void *params[] = {&args};
+    const char *what = "launch hexir_linear_16 guarded";
+    return p.split > 1
+               ? launch_cluster(call.lib->guarded[op], grid, p.split,
+                                HEXIR_SINGLE_THREADS, p.smem, stream, params,
+                                what, &call.error)
+               : launch(call.lib->guarded[op], grid, 1, HEXIR_SINGLE_THREADS,
+                        p.smem, stream, params, what, &call.error);
+  }
+  Operand a = {args.a, args.lda, a_mn, args.rows, HEXIR_PRODUCT_BM};
+  Operand b = {args.b, args.ldb, b_mn, args.cols,
+               p.variant == kPair ? p.tile_n / 2 : p.tile_n};
+  if (p.variant == kSkinny) {
+    // The transposed product: the weight's columns are the tile's rows.
+    const Operand x = {args.a, args.lda, false, args.rows, p.tile_n};
+    a = {args.b, args.ldb, true, args.cols, HEXIR_PRODUCT_BM};
+    b = x;
+  }
+  CUtensorMap map_a, map_b;
+  CUresult r = encode(&map_a, a, args.depth, args.is_f16 != 0);
+  if (r == CUDA_SUCCESS)
+    r = encode(&map_b, b, args.depth, args.is_f16 != 0);
+  if (r != CUDA_SUCCESS)
+    return fail(&call.error, cuda_message("cuTensorMapEncodeTiled", r));
+  void *params[] = {&map_a, &map_b, &args};
+  if (p.variant == kPair) {
+    const uint64_t pairs = std::min<uint64_t>(tiles, sms / 2);
+    return launch(call.lib->pair[op], static_cast<unsigned>(2 * pairs), 1,
+                  HEXIR_PAIR_THREADS, p.smem, stream, params,
+                  "launch hexir_linear_16 pair", &call.error);
+  }
+  CUfunction fn = p.variant == kSkinny ? call.lib->skinny : call.lib->single[op];
+  const char *what = p.variant == kSkinny ? "launch hexir_linear_16 skinny"
+                                          : "launch hexir_linear_16 single";
+  return p.split > 1 ? launch_cluster(fn, grid, p.split, HEXIR_SINGLE_THREADS,
+                                      p.smem, stream, params, what, &call.error)
+                     : launch(fn, grid, 1, HEXIR_SINGLE_THREADS, p.smem, stream,
+                              params, what, &call.error);
+}
+
+// TMA coordinates are signed 32-bit numbers.
+bool extents_ok(uint32_t m, uint32_t n, uint32_t k) {
+  constexpr uint32_t kMost = 0x7FFFFF00u;
+  return m <= kMost && n <= kMost && k <= kMost;
+}
+
+// ----------------------------------------------------------- the norms
+
+int norm_shape(uint32_t cols) {
+  for (int s = 0; s < kNormShapes; ++s)
+    if (cols <= kNorm[s].threads * kNorm[s].elements)
+      return s;
+  return -1;
+}
+
+constexpr uint32_t kSumsPerColumn = 640;  // hexir_cuda_grad_workspace
+
+}  // namespace
+
+}  // namespace hexir
+
+using namespace hexir;
+
+extern "C" uint64_t hexir_cuda_grad_workspace(uint32_t cols, uint32_t dtype) {
+  return static_cast<uint64_t>(kSumsPerColumn) * cols *
+         (dtype == HEXIR_DTYPE_F64 ? 8 : 4);
+}
+
+extern "C" hexir_status_t hexir_cuda_linear_plan(
+    int ordinal, uint32_t op, uint32_t m, uint32_t n, uint32_t k, int aligned,
+    uint32_t flags, uint32_t *variant, uint32_t *tile_n, uint32_t *split) {
+  Call call;
+  hexir_status_t status;
+  std::string bad = check_linear("linear_plan", HEXIR_DTYPE_BF16, 0, flags, &status);
+  if (op > HEXIR_PRODUCT_WEIGHT_GRAD || !bad.empty())
+    return call.refuse(bad.empty() ? "linear_plan: op is 0, 1 or 2" : bad);
+  // Without a GPU: B200's 148 SMs.
+  std::string error;
+  DeviceState *dev = device_state(ordinal, &error);
+  const ProductPlan p = plan_product(op, m, n, k, aligned != 0, flags,
+                                     dev ? std::max(dev->sm_count, 2) : 148);
+  if (!p.refusal.empty())
+    return call.refuse("linear_plan: " + p.refusal);
+  if (variant)
+    *variant = p.variant;
+  if (tile_n)
+    *tile_n = p.tile_n;
+  if (split)
+    *split = p.split;
+  return HEXIR_OK;
+}
+
+extern "C" hexir_status_t hexir_cuda_linear(int ordinal,
+                                            const hexir_linear_call_t *given,
+                                            void *stream) {
+  Call call;
+  if (!given)
+    return call.refuse("linear: null call");
+  hexir_linear_call_t c = *given;
+  hexir_status_t status;
+  std::string bad = check_linear("linear", c.dtype, c.activation, c.flags, &status);
+  if (!bad.empty())
+    return call.refuse(bad, status);
+  const bool some = c.m && c.n;
+  if (some && (!c.y || (c.k && (!c.x || !c.w))))
+    return call.refuse("linear: null pointer");
+  if (!extents_ok(c.m, c.n, c.k))
+    return call.refuse("linear: m, n or k is too large");
+  uint64_t dense = 0;
+  bad = check_tensors("linear", 2,
+                      {{"x", c.x, &c.ldx, c.m, c.k},
+                       {"w", c.w, &c.ldw, c.k, c.n},
+                       {"bias", c.bias, &dense, 1, c.n},
+                       {"residual", c.residual, &c.ldr, c.m, c.n},
+                       {"preact", c.preact, &c.ldp, c.m, c.n},
+                       {"y", c.y, &c.ldy, c.m, c.n}});
+  if (!bad.empty())
+    return call.refuse(bad);
+  if (!call.open(ordinal))
+    return call.finish(HEXIR_ERROR_DEVICE);
+  hexir_product_args_t args;
+  std::memset(&args, 0, sizeof(args));
+  args.a = c.x;
+  args.lda = c.ldx;
+  args.b = c.w;
+  args.ldb = c.ldw;
+  args.out = c.y;
+  args.ldo = c.ldy;
+  args.preact_out = c.preact;
+  args.ldp = c.ldp;
+  args.bias = c.bias;
+  args.residual = c.residual;
+  args.ldr = c.ldr;
+  args.rows = c.m;
+  args.cols = c.n;
+  args.depth = c.k;
+  args.activation = c.activation;
+  args.is_f16 = c.dtype == HEXIR_DTYPE_F16;
+  ContextGuard guard(call.dev->context);
+  return call.finish(launch_product(call, HEXIR_PRODUCT_FORWARD, c.m, c.n, c.k,
+                                    c.flags, args, static_cast<CUstream>(stream)));
+}
+
+extern "C" hexir_status_t hexir_cuda_linear_input_grad(
+    int ordinal, const hexir_linear_input_grad_call_t *given, void *stream) {
+  Call call;
+  if (!given)
+    return call.refuse("linear_input_grad: null call");
+  hexir_linear_input_grad_call_t c = *given;
+  hexir_status_t status;
+  std::string bad =
+      check_linear("linear_input_grad", c.dtype, c.activation, c.flags, &status);
+  if (!bad.empty())
+    return call.refuse(bad, status);
+  const bool some = c.m && c.k;
+  if (some && (!c.dx || (c.n && (!c.dz || !c.w)) || (c.activation && !c.preact)))
+    return call.refuse("linear_input_grad: null pointer");
+  if (!extents_ok(c.m, c.n, c.k))
+    return call.refuse("linear_input_grad: m, n or k is too large");
+  bad = check_tensors("linear_input_grad", 2,
+                      {{"dz", c.dz, &c.lddz, c.m, c.n},
+                       {"w", c.w, &c.ldw, c.k, c.n},
+                       {"preact", c.preact, &c.ldp, c.m, c.k},
+                       {"residual", c.residual, &c.ldr, c.m, c.k},
+                       {"dx", c.dx, &c.lddx, c.m, c.k}});
+  if (!bad.empty())
+    return call.refuse(bad);
+  if (!call.open(ordinal))
+    return call.finish(HEXIR_ERROR_DEVICE);
+  hexir_product_args_t args;
+  std::memset(&args, 0, sizeof(args));
+  args.a = c.dz;
+  args.lda = c.lddz;
+  args.b = c.w;
+  args.ldb = c.ldw;
+  args.out = c.dx;
+  args.ldo = c.lddx;
+  args.slope_at = c.activation ? c.preact : nullptr;
+  args.lds = c.ldp;
+  args.residual = c.residual;
+  args.ldr = c.ldr;
+  args.rows = c.m;
+  args.cols = c.k;
+  args.depth = c.n;
+  args.activation = c.activation;
+  args.is_f16 = c.dtype == HEXIR_DTYPE_F16;
+  ContextGuard guard(call.dev->context);
+  return call.finish(launch_product(call, HEXIR_PRODUCT_INPUT_GRAD, c.m, c.n, c.k,
+                                    c.flags, args, static_cast<CUstream>(stream)));
+}
+
+extern "C" hexir_status_t hexir_cuda_linear_weight_grad(
+    int ordinal, const hexir_linear_weight_grad_call_t *given, void *stream) {
+  Call call;
+  if (!given)
+    return call.refuse("linear_weight_grad: null call");
+  hexir_linear_weight_grad_call_t c = *given;
+  hexir_status_t status;
+  std::string bad = check_linear("linear_weight_grad", c.dtype, 0, c.flags, &status);
+  if (!bad.empty())
+    return call.refuse(bad, status);
+  if (c.reserved)
+    return call.refuse("linear_weight_grad: reserved is not 0");
+  const bool some = c.k && c.n;
+  if (some && (!c.dw || (c.m && (!c.x || !c.dz))))
+    return call.refuse("linear_weight_grad: null pointer");
+  if (!extents_ok(c.m, c.n, c.k))
+    return call.refuse("linear_weight_grad: m, n or k is too large");
+  bad = check_tensors("linear_weight_grad", 2,
+                      {{"x", c.x, &c.ldx, c.m, c.k},
+                       {"dz", c.dz, &c.lddz, c.m, c.n},
+                       {"dw", c.dw, &c.lddw, c.k, c.n}});
+  if (!bad.empty())
+    return call.refuse(bad);
+  if (!call.open(ordinal))
+    return call.finish(HEXIR_ERROR_DEVICE);
+  hexir_product_args_t args;
+  std::memset(&args, 0, sizeof(args));
+  args.a = c.x;
+  args.lda = c.ldx;
+  args.b = c.dz;
+  args.ldb = c.lddz;
+  args.out = c.dw;
+  args.ldo = c.lddw;
+  args.rows = c.k;
+  args.cols = c.n;
+  args.depth = c.m;
+  args.is_f16 = c.dtype == HEXIR_DTYPE_F16;
+  ContextGuard guard(call.dev->context);
+  return call.finish(launch_product(call, HEXIR_PRODUCT_WEIGHT_GRAD, c.m, c.n, c.k,
+                                    c.flags, args, static_cast<CUstream>(stream)));
+}
+
+extern "C" hexir_status_t hexir_cuda_linear_output_grad(
+    int ordinal, const hexir_linear_output_grad_call_t *given, void *stream) {
+  Call call;
+  if (!given)
+    return call.refuse("linear_output_grad: null call");
+  hexir_linear_output_grad_call_t c = *given;
+  hexir_status_t status;
+  std::string bad = check_linear("linear_output_grad", c.dtype, c.activation, 0, &status);
+  if (!bad.empty())
+    return call.refuse(bad, status);
+  const bool some = c.m && c.n;
+  if (some && (!c.dy || (c.activation && (!c.preact || !c.dz))))
+    return call.refuse("linear_output_grad: null pointer");
+  bad = check_tensors("linear_output_grad", 2,
+                      {{"dy", c.dy, &c.lddy, c.m, c.n},
+                       {"preact", c.preact, &c.ldp, c.m, c.n},
+                       {"dz", c.dz, &c.lddz, c.m, c.n}});
+  if (!bad.empty())
+    return call.refuse(bad);
+  if (c.dbias && off(c.dbias, 2))
+    return call.refuse("linear_output_grad: dbias is not aligned to its elements");
+  if (c.dbias && c.n &&
+      (!c.workspace || off(c.workspace, 16) ||
+       c.workspace_bytes < hexir_cuda_grad_workspace(c.n, c.dtype)))
+    return call.refuse("linear_output_grad: dbias needs a 16-byte aligned "
+                       "workspace of hexir_cuda_grad_workspace(n, dtype) bytes");
+  if (!call.open(ordinal))
+    return call.finish(HEXIR_ERROR_DEVICE);
+  if (!c.n || (!c.dz && !c.dbias))
+    return HEXIR_OK;
+  ContextGuard guard(call.dev->context);
+  CUstream s = static_cast<CUstream>(stream);
+  hexir_output_grad_args_t args;
+  std::memset(&args, 0, sizeof(args));
+  args.dy = c.dy;
+  args.lddy = c.lddy;
+  args.preact = c.preact;
+  args.ldp = c.ldp;
+  args.dz = c.dz == c.dy && !c.activation ? nullptr : c.dz;
+  args.lddz = c.lddz;
+  args.dbias = c.dbias;
+  args.partials = c.dbias ? static_cast<float *>(c.workspace) : nullptr;
+  args.m = c.m;
+  args.n = c.n;
+  args.activation = c.activation;
+  args.vec = rows16(c.dy, c.lddy, 2) &&
+             (!c.activation || rows16(c.preact, c.ldp, 2)) &&
+             (!args.dz || rows16(c.dz, c.lddz, 2));
+  const uint32_t gx = ceil_div(c.n, 256);
+  hexir_status_t st = HEXIR_OK;
+  if (c.m) {
+    const uint64_t sms = static_cast<uint64_t>(std::max(call.dev->sm_count, 1));
+    const uint64_t want = std::max<uint64_t>(1, sms * 8 / gx);
+    args.parts = static_cast<uint32_t>(std::min<uint64_t>(
+        {want, static_cast<uint64_t>(ceil_div(c.m, 32)), uint64_t(kSumsPerColumn)}));
+    args.rows_per_part = ceil_div(c.m, args.parts);
+    args.parts = ceil_div(c.m, args.rows_per_part);
+    void *params[] = {&args};
+    st = launch(call.lib->output_grad[c.dtype], gx, args.parts, 256, 0, s, params,
+                "launch hexir_linear_output_grad", &call.error);
+  }
+  if (st == HEXIR_OK && c.dbias) {
+    void *params[] = {&args};
+    st = launch_after(call.lib->output_grad_join[c.dtype], ceil_div(c.n, 32), 1,
+                      256, s, params, "launch hexir_linear_output_grad_join",
+                      &call.error);
+  }
+  return call.finish(st);
+}
+
+extern "C" hexir_status_t hexir_cuda_layer_norm(int ordinal,
+                                                const hexir_layer_norm_call_t *given,
+                                                void *stream) {
+  Call call;
+  if (!given)
+    return call.refuse("layer_norm: null call");
+  hexir_layer_norm_call_t c = *given;
+  if (c.dtype > HEXIR_DTYPE_F16)
+    return call.refuse("layer_norm: unknown dtype " + std::to_string(c.dtype));
+  if (!c.cols)
+    return call.refuse("layer_norm: a row needs at least one column");
+  if (!(c.eps >= 0.0) || std::isinf(c.eps))
+    return call.refuse("layer_norm: eps is not a finite number >= 0");
+  if (c.rows && (!c.x || !c.y))
+    return call.refuse("layer_norm: null pointer");
+  const uint32_t size = kDtypeSize[c.dtype];
+  const uint32_t real = c.dtype == HEXIR_DTYPE_F64 ? 8 : 4;
+  uint64_t dense = 0;
+  std::string bad = check_tensors("layer_norm", size,
+                                  {{"x", c.x, &c.ldx, c.rows, c.cols},
+                                   {"y", c.y, &c.ldy, c.rows, c.cols},
+                                   {"gamma", c.gamma, &dense, 1, c.cols},
+                                   {"beta", c.beta, &dense, 1, c.cols}});
+  if (bad.empty())
+    bad = check_tensors("layer_norm", real,
+                        {{"mean", c.mean, &dense, 1, 1}, {"rstd", c.rstd, &dense, 1, 1}});
+  if (!bad.empty())
+    return call.refuse(bad);
+  if (!call.open(ordinal))
+    return call.finish(HEXIR_ERROR_DEVICE);
+  if (!c.rows)
+    return HEXIR_OK;
+  hexir_layer_norm_args_t args;
+  std::memset(&args, 0, sizeof(args));
+  args.x = c.x;
+  args.ldx = c.ldx;
+  args.y = c.y;
+  args.ldy = c.ldy;
+  args.gamma = c.gamma;
+  args.beta = c.beta;
+  args.mean = c.mean;
+  args.rstd = c.rstd;
+  args.rows = c.rows;
+  args.cols = c.cols;
+  args.eps = c.eps;
+  args.vec = rows16(c.x, c.ldx, size) && rows16(c.y, c.ldy, size) &&
+             !off(c.gamma, 16) && !off(c.beta, 16);
+  void *params[] = {&args};
+  ContextGuard guard(call.dev->context);
+  CUstream s = static_cast<CUstream>(stream);
+  const int shape = norm_shape(c.cols);
+  const uint64_t cap = 1u << 24;  // the rest by stride
+  if (shape < 0)
+    return call.finish(launch(call.lib->norm_wide[c.dtype],
+                              static_cast<unsigned>(std::min(c.rows, cap)), 1, 512, 0,
+                              s, params, "launch hexir_layer_norm wide", &call.error));
+  const bool warp = kNorm[shape].threads == 32;
+  const uint64_t blocks = warp ? (c.rows + 7) / 8 : c.rows;
+  return call.finish(launch(call.lib->norm[c.dtype][shape],
+                            static_cast<unsigned>(std::min(blocks, cap)), 1,
+                            warp ? 256 : kNorm[shape].threads, 0, s, params,
+                            "launch hexir_layer_norm", &call.error));
+}
+
+extern "C" hexir_status_t hexir_cuda_layer_norm_grad(
+    int ordinal, const hexir_layer_norm_grad_call_t *given, void *stream) {
+  Call call;
+  if (!given)
+    return call.refuse("layer_norm_grad: null call");
+  hexir_layer_norm_grad_call_t c = *given;
+  if (c.dtype > HEXIR_DTYPE_F16)
+    return call.refuse("layer_norm_grad: unknown dtype " + std::to_string(c.dtype));
+  if (!c.cols)
+    return call.refuse("layer_norm_grad: a row needs at least one column");
+  if (c.rows && (!c.dy || !c.x || !c.mean || !c.rstd))
+    return call.refuse("layer_norm_grad: null pointer");
+  const uint32_t size = kDtypeSize[c.dtype];
+  const uint32_t real = c.dtype == HEXIR_DTYPE_F64 ? 8 : 4;
+  uint64_t dense = 0;
+  std::string bad = check_tensors("layer_norm_grad", size,
+                                  {{"dy", c.dy, &c.lddy, c.rows, c.cols},
+                                   {"x", c.x, &c.ldx, c.rows, c.cols},
+                                   {"residual", c.residual, &c.ldr, c.rows, c.cols},
+                                   {"dx", c.dx, &c.lddx, c.rows, c.cols},
+                                   {"gamma", c.gamma, &dense, 1, c.cols},
+                                   {"dgamma", c.dgamma, &dense, 1, c.cols},
+                                   {"dbeta", c.dbeta, &dense, 1, c.cols}});
+  if (bad.empty())
+    bad = check_tensors("layer_norm_grad", real,
+                        {{"mean", c.mean, &dense, 1, 1}, {"rstd", c.rstd, &dense, 1, 1}});
+  if (!bad.empty())
+    return call.refuse(bad);
+  const bool sums = c.dgamma || c.dbeta;
+  if (sums && (!c.workspace || off(c.workspace, 16) ||
+               c.workspace_bytes < hexir_cuda_grad_workspace(c.cols, c.dtype)))
+    return call.refuse("layer_norm_grad: dgamma and dbeta need a 16-byte aligned "
+                       "workspace of hexir_cuda_grad_workspace(cols, dtype) bytes");
+  if (!call.open(ordinal))
+    return call.finish(HEXIR_ERROR_DEVICE);
+  if (!sums && (!c.dx || !c.rows))
+    return HEXIR_OK;
+  hexir_layer_norm_grad_args_t args;
+  std::memset(&args, 0, sizeof(args));
+  args.dy = c.dy;
+  args.lddy = c.lddy;
+  args.x = c.x;
+  args.ldx = c.ldx;
+  args.mean = c.mean;
+  args.rstd = c.rstd;
+  args.gamma = c.gamma;
+  args.residual = c.residual;
+  args.ldr = c.ldr;
+  args.dx = c.dx;
+  args.lddx = c.lddx;
+  args.dgamma = c.dgamma;
+  args.dbeta = c.dbeta;
+  args.partials = sums ? c.workspace : nullptr;
+  args.rows = c.rows;
+  args.cols = c.cols;
+  args.vec = rows16(c.x, c.ldx, size) && rows16(c.dy, c.lddy, size) &&
+             !off(c.gamma, 16) && (!c.dx || rows16(c.dx, c.lddx, size)) &&
+             (!c.residual || rows16(c.residual, c.ldr, size));
+  ContextGuard guard(call.dev->context);
+  CUstream s = static_cast<CUstream>(stream);
+  const uint64_t sms = static_cast<uint64_t>(std::max(call.dev->sm_count, 1));
+  const int shape = norm_shape(c.cols);
+  hexir_status_t st = HEXIR_OK;
+  void *params[] = {&args};
+  if (c.rows && shape >= 0) {
+    const bool warp = kNorm[shape].threads == 32;
+    const uint64_t blocks = warp ? (c.rows + 7) / 8 : c.rows;
+    const uint64_t resident = sms * (kNorm[shape].threads <= 256 ? 2 : 1);
+    args.parts = static_cast<uint32_t>(
+        std::min<uint64_t>({blocks, resident, uint64_t(kSumsPerColumn / 2)}));
+    st = launch(call.lib->norm_grad[c.dtype][shape], args.parts, 1,
+                warp ? 256 : kNorm[shape].threads, 0, s, params,
+                "launch hexir_layer_norm_grad", &call.error);
+  } else if (c.rows) {
+    // The column sums first: dx may be dy.
+    if (sums) {
+      args.parts = static_cast<uint32_t>(
+          std::min<uint64_t>(kSumsPerColumn / 2, (c.rows + 63) / 64));
+      st = launch(call.lib->norm_grad_columns[c.dtype], ceil_div(c.cols, 32),
+                  args.parts, 256, 0, s, params,
+                  "launch hexir_layer_norm_grad columns", &call.error);
+    }
+    if (st == HEXIR_OK && c.dx)
+      st = launch(call.lib->norm_grad_wide[c.dtype],
+                  static_cast<unsigned>(std::min<uint64_t>(c.rows, 1u << 24)), 1, 512,
+                  0, s, params, "launch hexir_layer_norm_grad wide", &call.error);
+  }
+  if (st == HEXIR_OK && sums)
+    st = launch_after(call.lib->norm_grad_join[c.dtype], ceil_div(c.cols, 32), 2,
+                      256, s, params, "launch hexir_layer_norm_grad_join",
+                      &call.error);
+  return call.finish(st);
+}

@@ -1,0 +1,156 @@
+"""The layer calls' argument checks and kernel plans (include/hexir_b200/
+layers.h) without a GPU: every refusal comes before a device is opened."""
+
+import ctypes as C
+
+import pytest
+
+import hexir_b200 as hx
+from hexir_b200 import _ffi
+
+P = 4096  # an aligned address that no refused call reads
+
+
+def status(call, *args, **kw):
+    with pytest.raises(_ffi.HexirError) as err:
+        call(*args, **kw)
+    return err.value.status
+
+
+def linear(m=4, n=8, k=16, dtype="bf16", act="none", x=P, w=P, y=P, **kw):
+    return status(hx.cuda_linear, 0, x, w, y, m, n, k, dtype, act, **kw)
+
+
+BAD = _ffi.ERROR_INVALID_ARGUMENT
+
+
+def test_linear_refusals():
+    assert linear(dtype="f64") == _ffi.ERROR_UNIMPLEMENTED
+    assert linear(dtype="f32") == _ffi.ERROR_UNIMPLEMENTED
+    for ptr in ("x", "w", "y"):
+        assert linear(**{ptr: 0}) == BAD
+        assert linear(**{ptr: P + 1}) == BAD          # not on its elements
+    for ptr in ("bias", "residual", "preact"):
+        assert linear(**{ptr: P + 1}) == BAD
+    assert linear(ldx=15) == BAD                        # a stride below its row
+    assert linear(ldw=7) == BAD
+    assert linear(ldy=7) == BAD
+    assert linear(residual=P, ldr=7) == BAD
+    assert linear(preact=P, ldp=7) == BAD
+    assert linear(m=1 << 20, ldx=1 << 62) == BAD        # offsets past 63 bits
+    assert linear(flags=0x1) == BAD
+    assert linear(flags=_ffi.LINEAR_FORCE_PAIR | _ffi.LINEAR_FORCE_SINGLE) == BAD
+    assert linear(flags=_ffi.LINEAR_SPLIT(3)) == BAD
+    assert linear(flags=1 << 24) == BAD
+    assert linear(m=0xFFFFFFFF) == BAD
+    with pytest.raises(ValueError):
+        hx.cuda_linear(0, P, P, P, 4, 8, 16, "bf16", "softmax")
+    with pytest.raises(ValueError):
+        hx.cuda_linear(0, P, P, P, 4, 8, 16, "int8")
+
+
+def raw(fn, call):
+    return getattr(hx.lib(), fn)(0, C.byref(call) if call is not None else None, None)
+
+
+def test_raw_calls_refuse_null_and_unknown_codes():
+    for fn in ("hexir_cuda_linear", "hexir_cuda_linear_output_grad",
+               "hexir_cuda_linear_input_grad", "hexir_cuda_linear_weight_grad",
+               "hexir_cuda_layer_norm", "hexir_cuda_layer_norm_grad"):
+        assert raw(fn, None) == BAD
+    for activation in (1, 2, 4, 11, 15, 99):            # 11: softmax, a row op
+        call = _ffi.LinearCall(2, activation, 4, 8, 16, 0, P, P, 0, 0, 0, P)
+        assert raw("hexir_cuda_linear", call) == BAD
+    assert raw("hexir_cuda_linear", _ffi.LinearCall(4, 0, 4, 8, 16, 0, P, P, 0, 0, 0,
+                                                    P)) == BAD
+    call = _ffi.LinearWeightGradCall(2, 1, 4, 8, 16, 0, P, P, P)
+    assert raw("hexir_cuda_linear_weight_grad", call) == BAD   # reserved
+    call = _ffi.LayerNormCall(7, 8, 1, 1e-5, P, 0, 0, P)
+    assert raw("hexir_cuda_layer_norm", call) == BAD
+
+
+def test_grad_refusals():
+    def dx(act="none", **kw):
+        args = {"dz": P, "w": P, "dx": P, **{a: kw.pop(a) for a in ("dz", "w", "dx")
+                                             if a in kw}}
+        return status(hx.cuda_linear_input_grad, 0, args["dz"], args["w"], args["dx"],
+                      4, 8, 16, "bf16", act, **kw)
+    assert dx(dz=0) == dx(w=0) == dx(dx=0) == BAD
+    assert dx(act="gelu") == BAD                        # no preactivations
+    assert dx(lddz=7) == dx(ldw=7) == dx(lddx=15) == BAD
+    assert dx(dz=P + 1) == BAD
+    assert status(hx.cuda_linear_weight_grad, 0, 0, P, P, 4, 8, 16) == BAD
+    assert status(hx.cuda_linear_weight_grad, 0, P, P, P, 4, 8, 16, lddw=7) == BAD
+    assert status(hx.cuda_linear_weight_grad, 0, P, P, P, 4, 8, 16, "f32") == \
+        _ffi.ERROR_UNIMPLEMENTED
+
+    def out(act="none", dy=P, **kw):
+        return status(hx.cuda_linear_output_grad, 0, dy, 4, 8, "bf16", act, **kw)
+    assert out(dy=0, dz=P) == BAD
+    assert out(act="gelu", dz=P) == BAD                 # no preactivations
+    assert out(act="gelu", preact=P) == BAD             # nowhere for dz
+    need = hx.grad_workspace_bytes(8, "bf16")
+    assert out(dbias=P) == BAD                          # no workspace
+    assert out(dbias=P, workspace=P, workspace_bytes=need - 1) == BAD
+    assert out(dbias=P, workspace=P + 8, workspace_bytes=need) == BAD
+    assert out(dbias=P + 1, workspace=P, workspace_bytes=need) == BAD
+
+
+def test_layer_norm_refusals():
+    def norm(x=P, y=P, rows=4, cols=8, dtype="f32", **kw):
+        return status(hx.cuda_layer_norm, 0, x, y, rows, cols, dtype, **kw)
+    assert norm(x=0) == norm(y=0) == norm(cols=0) == BAD
+    assert norm(x=P + 2) == norm(gamma=P + 2) == norm(beta=P + 2) == BAD
+    assert norm(mean=P + 2) == norm(rstd=P + 2) == BAD
+    assert norm(ldx=7) == norm(ldy=7) == BAD
+    for eps in (-1e-5, float("nan"), float("inf")):
+        assert norm(eps=eps) == BAD
+
+    def grad(dy=P, x=P, mean=P, rstd=P, dx=P, rows=4, cols=8, dtype="f64", **kw):
+        return status(hx.cuda_layer_norm_grad, 0, dy, x, mean, rstd, dx, rows, cols,
+                      dtype, **kw)
+    assert grad(dy=0) == grad(x=0) == grad(mean=0) == grad(rstd=0) == BAD
+    assert grad(cols=0) == grad(lddy=7) == grad(lddx=7) == BAD
+    assert grad(residual=P, ldr=7) == grad(residual=P + 4) == BAD
+    need = hx.grad_workspace_bytes(8, "f64")
+    assert need == 640 * 8 * 8
+    assert grad(dgamma=P) == BAD
+    assert grad(dbeta=P, workspace=P, workspace_bytes=need - 1) == BAD
+    assert grad(dbeta=P, workspace=P + 8, workspace_bytes=need) == BAD
+
+
+@pytest.mark.skipif(hx.device_count() > 0, reason="checks the no-GPU behaviour")
+def test_good_arguments_need_a_gpu():
+    dev = _ffi.ERROR_DEVICE
+    assert linear() == dev
+    assert linear(m=0) == dev
+    assert status(hx.cuda_layer_norm, 0, P, P, 4, 8) == dev
+    assert status(hx.cuda_linear_weight_grad, 0, P, P, P, 4, 8, 16) == dev
+
+
+def test_plans():
+    PAIR, SINGLE, SKINNY, GUARDED = 1, 2, 3, 4
+    assert hx.linear_plan("forward", 8192, 8192, 8192)[:2] == (PAIR, 256)
+    assert hx.linear_plan("weight_grad", 8192, 8192, 8192)[:2] == (PAIR, 256)
+    for m in (1, 16, 64):
+        assert hx.linear_plan("forward", m, 8192, 8192)[0] == SKINNY
+    assert hx.linear_plan("forward", 65, 8192, 8192)[0] != SKINNY
+    assert hx.linear_plan("input_grad", 1, 8192, 8192)[0] != SKINNY
+    # Few tiles and a long sum: the sum is split.
+    assert hx.linear_plan("forward", 256, 512, 8192)[2] > 1
+    assert hx.linear_plan("forward", 1, 8192, 8192)[2] > 1
+    # No rows to load, or rows off 16 bytes.
+    assert hx.linear_plan("forward", 256, 512, 0)[0] == GUARDED
+    assert hx.linear_plan("forward", 256, 512, 512, aligned=False)[0] == GUARDED
+    for op in ("forward", "input_grad", "weight_grad"):
+        for flags, variant in ((_ffi.LINEAR_FORCE_PAIR, PAIR),
+                               (_ffi.LINEAR_FORCE_SINGLE, SINGLE),
+                               (_ffi.LINEAR_FORCE_GUARDED, GUARDED)):
+            assert hx.linear_plan(op, 200, 264, 520, flags=flags)[0] == variant
+    with pytest.raises(_ffi.HexirError):
+        hx.linear_plan("forward", 65, 8, 8, flags=_ffi.LINEAR_FORCE_SKINNY)
+    with pytest.raises(_ffi.HexirError):
+        hx.linear_plan("input_grad", 5, 8, 8, flags=_ffi.LINEAR_FORCE_SKINNY)
+    with pytest.raises(_ffi.HexirError):
+        hx.linear_plan("forward", 5, 8, 8, aligned=False,
+                       flags=_ffi.LINEAR_FORCE_PAIR)
