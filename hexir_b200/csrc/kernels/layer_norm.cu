@@ -55,67 +55,278 @@ __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
+// 16 bytes of a row.  widen_pack / narrow_pack convert whole words, two 16-bit
+// elements at a time: element by element, the conversions were what bounded
+// the 16-bit kernels (0.55 of copy bandwidth at 16384 x 4096, f32 0.92).
 template <typename T>
-struct alignas(16) Pack {
+struct Pack {
   static constexpr int kN = 16 / sizeof(T);
-  T v[kN];
+  uint4 w;
 };
 
-// Which columns a thread of `TH` holds: with 16-byte aligned rows, packs
-// tid, tid + TH, ...; otherwise single elements tid, tid + TH, ..., so that a
-// warp's loads stay consecutive either way.
-template <typename T, int TH>
-__device__ __forceinline__ uint32_t column(int pack, int j, uint32_t tid,
-                                           bool vec) {
-  constexpr int kN = Pack<T>::kN;
-  return vec ? (pack * TH + tid) * kN + j : (pack * kN + j) * TH + tid;
+// Two values that are computed side by side: sm_100 adds and multiplies two
+// f32 with one instruction.
+template <typename R>
+struct Two {
+  R x, y;
+};
+__device__ __forceinline__ uint64_t both(const Two<float> &a) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+  return r;
+}
+__device__ __forceinline__ Two<float> apart(uint64_t r) {
+  Two<float> a;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(r));
+  return a;
+}
+__device__ __forceinline__ Two<float> add(const Two<float> &a, const Two<float> &b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(both(a)), "l"(both(b)));
+  return apart(r);
+}
+__device__ __forceinline__ Two<float> mul(const Two<float> &a, const Two<float> &b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(both(a)), "l"(both(b)));
+  return apart(r);
+}
+__device__ __forceinline__ Two<float> fma(const Two<float> &a, const Two<float> &b,
+                                          const Two<float> &c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(r)
+      : "l"(both(a)), "l"(both(b)), "l"(both(c)));
+  return apart(r);
+}
+__device__ __forceinline__ Two<double> add(const Two<double> &a,
+                                           const Two<double> &b) {
+  return {a.x + b.x, a.y + b.y};
+}
+__device__ __forceinline__ Two<double> mul(const Two<double> &a,
+                                           const Two<double> &b) {
+  return {a.x * b.x, a.y * b.y};
+}
+__device__ __forceinline__ Two<double> fma(const Two<double> &a,
+                                           const Two<double> &b,
+                                           const Two<double> &c) {
+  return {::fma(a.x, b.x, c.x), ::fma(a.y, b.y, c.y)};
+}
+template <typename R>
+__device__ __forceinline__ R half_of(const Two<R> &a, int j) {
+  return j % 2 ? a.y : a.x;
+}
+template <typename R>
+__device__ __forceinline__ Two<R> twice(R v) {
+  return {v, v};
 }
 
-// NE elements of a row in packs; columns past the end give `fill`.
-template <typename T, int TH, int NE>
-__device__ __forceinline__ void load_row(const T *row, uint32_t cols,
-                                         uint32_t tid, bool vec, T fill,
-                                         Pack<T> (&v)[NE / Pack<T>::kN]) {
-  constexpr int kN = Pack<T>::kN;
+__device__ __forceinline__ void widen_pack(const Pack<double> &p,
+                                           Two<double> (&f)[1]) {
+  f[0] = {__hiloint2double(static_cast<int>(p.w.y), static_cast<int>(p.w.x)),
+          __hiloint2double(static_cast<int>(p.w.w), static_cast<int>(p.w.z))};
+}
+__device__ __forceinline__ void widen_pack(const Pack<float> &p,
+                                           Two<float> (&f)[2]) {
+  f[0] = {__uint_as_float(p.w.x), __uint_as_float(p.w.y)};
+  f[1] = {__uint_as_float(p.w.z), __uint_as_float(p.w.w)};
+}
+__device__ __forceinline__ void widen_pack(const Pack<__nv_bfloat16> &p,
+                                           Two<float> (&f)[4]) {
+  const uint32_t w[4] = {p.w.x, p.w.y, p.w.z, p.w.w};
 #pragma unroll
-  for (int i = 0; i < NE / kN; ++i) {
-    const uint32_t c0 = column<T, TH>(i, 0, tid, true);
-    if (vec && c0 + kN <= cols) {
-      v[i] = *reinterpret_cast<const Pack<T> *>(row + c0);
-    } else {
+  for (int i = 0; i < 4; ++i)
+    f[i] = {__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u)};
+}
+__device__ __forceinline__ void widen_pack(const Pack<__half> &p,
+                                           Two<float> (&f)[4]) {
+  const uint32_t w[4] = {p.w.x, p.w.y, p.w.z, p.w.w};
 #pragma unroll
-      for (int j = 0; j < kN; ++j) {
-        const uint32_t c = column<T, TH>(i, j, tid, vec);
-        v[i].v[j] = c < cols ? row[c] : fill;
-      }
-    }
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+    f[i] = {v.x, v.y};
   }
 }
+__device__ __forceinline__ void narrow_pack(const Two<double> (&f)[1],
+                                            Pack<double> &p) {
+  p.w = make_uint4(__double2loint(f[0].x), __double2hiint(f[0].x),
+                   __double2loint(f[0].y), __double2hiint(f[0].y));
+}
+__device__ __forceinline__ void narrow_pack(const Two<float> (&f)[2],
+                                            Pack<float> &p) {
+  p.w = make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y),
+                   __float_as_uint(f[1].x), __float_as_uint(f[1].y));
+}
+__device__ __forceinline__ uint32_t bits2(const __nv_bfloat162 &h) {
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t bits2(const __half2 &h) {
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ void narrow_pack(const Two<float> (&f)[4],
+                                            Pack<__nv_bfloat16> &p) {
+  p.w = make_uint4(bits2(__floats2bfloat162_rn(f[0].x, f[0].y)),
+                   bits2(__floats2bfloat162_rn(f[1].x, f[1].y)),
+                   bits2(__floats2bfloat162_rn(f[2].x, f[2].y)),
+                   bits2(__floats2bfloat162_rn(f[3].x, f[3].y)));
+}
+__device__ __forceinline__ void narrow_pack(const Two<float> (&f)[4],
+                                            Pack<__half> &p) {
+  p.w = make_uint4(bits2(__floats2half2_rn(f[0].x, f[0].y)),
+                   bits2(__floats2half2_rn(f[1].x, f[1].y)),
+                   bits2(__floats2half2_rn(f[2].x, f[2].y)),
+                   bits2(__floats2half2_rn(f[3].x, f[3].y)));
+}
 
-template <typename T, int TH, int NE>
-__device__ __forceinline__ void store_row(T *row, uint32_t cols, uint32_t tid,
-                                          bool vec,
-                                          const Pack<T> (&v)[NE / Pack<T>::kN]) {
+// Element j of a pack, for the packs at a row's ends.
+template <typename T>
+__device__ __forceinline__ T pack_get(const Pack<T> &p, int j) {
+  T v[Pack<T>::kN];
+  *reinterpret_cast<uint4 *>(v) = p.w;
+  return v[j];
+}
+
+// How a row lies over its threads.
+//   kWhole    16-byte packs tid, tid + TH, ... of a row that starts and ends on
+//             16-byte boundaries;
+//   kShifted  the same packs of memory, but the row starts `phase` elements
+//             after a boundary: its first pack is filled from element `phase`
+//             on (16-bit types; every tensor of the call has the same phase,
+//             and a block's rows are a multiple of 8 apart so that they
+//             share it);
+//   kAny      single elements tid, tid + TH, ..., so that a warp's accesses
+//             stay consecutive.
+enum Layout { kWhole, kShifted, kAny };
+
+// The packs at the ends of a shifted row, an element at a time.  Out of line:
+// inlined, their predicated loads were more than half of the instructions
+// every pack cost (410 a warp and row of 16 elements a thread).
+template <typename T>
+__device__ __noinline__ uint4 gather_pack(const T *row, uint32_t column,
+                                          uint32_t cols) {
   constexpr int kN = Pack<T>::kN;
+  T e[kN];
 #pragma unroll
-  for (int i = 0; i < NE / kN; ++i) {
-    const uint32_t c0 = column<T, TH>(i, 0, tid, true);
-    if (vec && c0 + kN <= cols) {
-      *reinterpret_cast<Pack<T> *>(row + c0) = v[i];
-    } else {
+  for (int j = 0; j < kN; ++j)
+    e[j] = column + j < cols ? row[column + j] : narrow<T>(real_t<T>(0));
+  return *reinterpret_cast<const uint4 *>(e);
+}
+template <typename T>
+__device__ __noinline__ void scatter_pack(T *row, uint32_t column, uint32_t cols,
+                                          uint4 v) {
+  constexpr int kN = Pack<T>::kN;
+  T e[kN];
+  *reinterpret_cast<uint4 *>(e) = v;
+#pragma unroll
+  for (int j = 0; j < kN; ++j)
+    if (column + j < cols)
+      row[column + j] = e[j];
+}
+
+template <typename T, int TH, int NE, int LAYOUT>
+struct Row {
+  static constexpr int kN = Pack<T>::kN;
+  static constexpr int kPacks = NE / kN;
+  uint32_t tid, cols, phase;
+
+  __device__ __forceinline__ Row(uint32_t tid_, uint32_t cols_, const void *row)
+      : tid(tid_), cols(cols_),
+        phase(LAYOUT == kShifted
+                  ? static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) % 16 /
+                                          sizeof(T))
+                  : 0) {}
+  // Column of element j of pack i; wraps below 0 for the elements before the
+  // row, so `column < cols` holds for the row's elements alone.
+  __device__ __forceinline__ uint32_t column(int i, int j) const {
+    return LAYOUT != kAny ? (i * TH + tid) * kN + j - phase
+                          : (i * kN + j) * TH + tid;
+  }
+  // Whether pack i has elements of the row; whether it has others too.
+  __device__ __forceinline__ bool some(int i) const {
+    return LAYOUT == kWhole     ? column(i, 0) < cols
+           : LAYOUT == kShifted ? (i * TH + tid) * kN < cols + phase
+                                : (i * kN) * TH + tid < cols;
+  }
+  __device__ __forceinline__ bool cut(int i) const {
+    if (LAYOUT != kShifted)
+      return false;
+    const uint32_t c = column(i, 0);
+    return c >= cols || cols - c < kN;
+  }
+  // The elements of the row as stored, zeros elsewhere.  STREAM: read once,
+  // not kept in L1.
+  template <bool STREAM>
+  __device__ __forceinline__ void load(const T *row, Pack<T> (&v)[kPacks]) const {
+#pragma unroll
+    for (int i = 0; i < kPacks; ++i)
+      v[i] = load_pack<STREAM>(row, i);
+  }
+  template <bool STREAM>
+  __device__ __forceinline__ Pack<T> load_pack(const T *row, int i) const {
+    Pack<T> v;
+    v.w = make_uint4(0, 0, 0, 0);
+    if (LAYOUT == kAny) {
+      T e[kN];
 #pragma unroll
       for (int j = 0; j < kN; ++j) {
-        const uint32_t c = column<T, TH>(i, j, tid, vec);
+        const uint32_t c = column(i, j);
+        e[j] = c < cols ? row[c] : narrow<T>(real_t<T>(0));
+      }
+      v.w = *reinterpret_cast<const uint4 *>(e);
+    } else if (some(i)) {
+      if (cut(i)) {
+        v.w = gather_pack(row, column(i, 0), cols);
+      } else {
+        const uint4 *at = reinterpret_cast<const uint4 *>(row + column(i, 0));
+        v.w = STREAM ? __ldcs(at) : *at;
+      }
+    }
+    return v;
+  }
+  __device__ __forceinline__ void store(T *row, int i, const Pack<T> &v) const {
+    if (LAYOUT == kAny) {
+#pragma unroll
+      for (int j = 0; j < kN; ++j) {
+        const uint32_t c = column(i, j);
         if (c < cols)
-          row[c] = v[i].v[j];
+          row[c] = pack_get(v, j);
       }
+    } else if (some(i)) {
+      if (cut(i))
+        scatter_pack(row, column(i, 0), cols, v.w);
+      else
+        __stcs(reinterpret_cast<uint4 *>(row + column(i, 0)), v.w);
     }
   }
+  // Pack i of gamma or beta, which start at column 0: as the row's packs
+  // lie.
+  __device__ __forceinline__ Pack<T> parameter(const T *p, int i) const {
+    if (LAYOUT != kShifted)
+      return load_pack<false>(p, i);
+    Pack<T> v;
+    v.w = gather_pack(p, column(i, 0), cols);
+    return v;
+  }
+};
+
+// Sum over the TH threads of a row, in an order that depends on TH alone.
+// `slot` holds TH / 32 values (2 * TH / 32 for row_sum2); calls alternate
+// between two slots, so one barrier per call is enough.
+template <int TH, typename R>
+__device__ __forceinline__ void row_sum(R &a, R *slot) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
+  if (TH == 32)
+    return;
+  if (threadIdx.x % 32 == 0)
+    slot[threadIdx.x / 32] = a;
+  __syncthreads();
+  a = slot[0];
+#pragma unroll
+  for (int w = 1; w < TH / 32; ++w)
+    a += slot[w];
 }
 
-// Sums of two values over the TH threads of a row, in an order that depends
-// on TH alone.  `slot` holds 2 * TH / 32 values; calls alternate between two
-// slots, so one barrier per call is enough.
 template <int TH, typename R>
 __device__ __forceinline__ void row_sum2(R &a, R &b, R *slot) {
 #pragma unroll
@@ -125,84 +336,144 @@ __device__ __forceinline__ void row_sum2(R &a, R &b, R *slot) {
   }
   if (TH == 32)
     return;
-  constexpr int kWarps = TH / 32;
-  const uint32_t warp = threadIdx.x / 32;
   if (threadIdx.x % 32 == 0) {
-    slot[2 * warp] = a;
-    slot[2 * warp + 1] = b;
+    slot[2 * (threadIdx.x / 32)] = a;
+    slot[2 * (threadIdx.x / 32) + 1] = b;
   }
   __syncthreads();
   a = slot[0];
   b = slot[1];
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) {
+  for (int w = 1; w < TH / 32; ++w) {
     a += slot[2 * w];
     b += slot[2 * w + 1];
   }
 }
 
-__device__ __forceinline__ float inv_sqrt(float v) { return 1.0f / sqrtf(v); }
-__device__ __forceinline__ double inv_sqrt(double v) { return 1.0 / sqrt(v); }
+__device__ __forceinline__ float inv_sqrt(float v) { return rsqrtf(v); }
+__device__ __forceinline__ double inv_sqrt(double v) { return rsqrt(v); }
 
 // Rows of up to TH * NE columns; TH == 32: a warp per row, 8 rows per block.
-template <typename T, int TH, int NE>
+// Blocks are persistent and load their next row before they work on the
+// present one, so that HBM is read while the row's sums and barriers run; the
+// row stays packed in registers, which lets several blocks share an SM.
+template <typename T, int TH, int NE, int LAYOUT>
 __device__ __forceinline__ void norm_rows(const hexir_layer_norm_args_t &p) {
   typedef real_t<T> R;
-  constexpr int kN = Pack<T>::kN;
+  typedef Row<T, TH, NE, LAYOUT> Lay;
+  constexpr int kN = Lay::kN, kPacks = Lay::kPacks;
   constexpr uint32_t kRows = TH == 32 ? 8 : 1;
-  __shared__ R slots[2][TH == 32 ? 1 : 2 * TH / 32];
+  __shared__ R slots[2][TH == 32 ? 1 : TH / 32];
+  extern __shared__ uint4 copies[];  // gamma and beta as this block's rows lie
   const uint32_t tid = TH == 32 ? threadIdx.x % 32 : threadIdx.x;
-  const bool vec = p.vec != 0;
-  const R n = static_cast<R>(p.cols);
-  for (uint64_t row = (uint64_t)blockIdx.x * kRows +
-                      (TH == 32 ? threadIdx.x / 32 : 0);
-       row < p.rows; row += (uint64_t)gridDim.x * kRows) {
-    Pack<T> x[NE / kN];
-    load_row<T, TH, NE>(static_cast<const T *>(p.x) + row * p.ldx, p.cols, tid,
-                        vec, narrow<T>(R(0)), x);
-    R sum = 0, none = 0;
+  const R n = static_cast<R>(p.cols), inv_n = R(1) / n;
+  const T *x_rows = static_cast<const T *>(p.x);
+  const T *gamma = static_cast<const T *>(p.gamma);
+  const T *beta = static_cast<const T *>(p.beta);
+  const uint64_t step = (uint64_t)gridDim.x * kRows;
+  uint64_t row = (uint64_t)blockIdx.x * kRows + (TH == 32 ? threadIdx.x / 32 : 0);
+  if (row >= p.rows)
+    return;
+  const Lay lay(tid, p.cols, x_rows + row * p.ldx);
+  Pack<T> x[kPacks], next[kPacks];
+  lay.template load<true>(x_rows + row * p.ldx, x);
+  // Shifted rows: gamma and beta as this row's packs lie, in shared memory.
+  // Each thread reads back only what it writes here.
+  uint4 *gamma_copy = copies + (TH == 32 ? threadIdx.x / 32 : 0) * (2 * TH * kPacks);
+  uint4 *beta_copy = gamma_copy + TH * kPacks;
+  if (LAYOUT == kShifted) {
 #pragma unroll
-    for (int i = 0; i < NE / kN; ++i)
+    for (int i = 0; i < kPacks; ++i) {
+      if (gamma)
+        gamma_copy[i * TH + tid] = lay.parameter(gamma, i).w;
+      if (beta)
+        beta_copy[i * TH + tid] = lay.parameter(beta, i).w;
+    }
+  }
+  for (;; row += step) {
+    const bool more = row + step < p.rows;
+    if (more)
+      lay.template load<true>(x_rows + (row + step) * p.ldx, next);
+    Two<R> sum2 = twice(R(0));
 #pragma unroll
-      for (int j = 0; j < kN; ++j)
-        sum += widen(x[i].v[j]);
-    row_sum2<TH>(sum, none, slots[0]);
-    const R mean = sum / n;
-    R m2 = 0;
+    for (int i = 0; i < kPacks; ++i) {
+      Two<R> f[kN / 2];
+      widen_pack(x[i], f);
 #pragma unroll
-    for (int i = 0; i < NE / kN; ++i)
+      for (int j = 0; j < kN / 2; ++j)
+        sum2 = add(sum2, f[j]);
+    }
+    R sum = sum2.x + sum2.y;
+    row_sum<TH>(sum, slots[0]);
+    const R mean = sum / n;  // exact for a row of one small integer
+    Two<R> m2 = twice(R(0));
 #pragma unroll
-      for (int j = 0; j < kN; ++j) {
-        const R d = widen(x[i].v[j]) - mean;
-        m2 += column<T, TH>(i, j, tid, vec) < p.cols ? d * d : R(0);
+    for (int i = 0; i < kPacks; ++i) {
+      if (!lay.some(i))
+        continue;
+      Two<R> f[kN / 2];
+      widen_pack(x[i], f);
+      const bool whole = LAYOUT == kWhole || (LAYOUT == kShifted && !lay.cut(i));
+#pragma unroll
+      for (int j = 0; j < kN / 2; ++j) {
+        f[j] = add(f[j], twice(-mean));
+        if (!whole) {
+          if (lay.column(i, 2 * j) >= p.cols)
+            f[j].x = 0;
+          if (lay.column(i, 2 * j + 1) >= p.cols)
+            f[j].y = 0;
+        }
+        m2 = fma(f[j], f[j], m2);
       }
-    row_sum2<TH>(m2, none, slots[1]);
-    const R rstd = inv_sqrt(m2 / n + static_cast<R>(p.eps));
-    Pack<T> g[NE / kN], b[NE / kN];
-    if (p.gamma)
-      load_row<T, TH, NE>(static_cast<const T *>(p.gamma), p.cols, tid, vec,
-                          narrow<T>(R(0)), g);
-    if (p.beta)
-      load_row<T, TH, NE>(static_cast<const T *>(p.beta), p.cols, tid, vec,
-                          narrow<T>(R(0)), b);
+    }
+    R var = m2.x + m2.y;
+    row_sum<TH>(var, slots[1]);
+    const R rstd = inv_sqrt(var * inv_n + static_cast<R>(p.eps));
+    T *y = static_cast<T *>(p.y) + row * p.ldy;
 #pragma unroll
-    for (int i = 0; i < NE / kN; ++i)
+    for (int i = 0; i < kPacks; ++i) {
+      if (!lay.some(i))
+        continue;
+      Two<R> f[kN / 2], q[kN / 2];
+      Pack<T> v;
+      widen_pack(x[i], f);
 #pragma unroll
-      for (int j = 0; j < kN; ++j) {
-        R v = (widen(x[i].v[j]) - mean) * rstd;
-        if (p.gamma)
-          v *= widen(g[i].v[j]);
-        if (p.beta)
-          v += widen(b[i].v[j]);
-        x[i].v[j] = narrow<T>(v);
+      for (int j = 0; j < kN / 2; ++j)
+        f[j] = mul(add(f[j], twice(-mean)), twice(rstd));
+      if (gamma) {
+        if (LAYOUT == kShifted)
+          v.w = gamma_copy[i * TH + tid];
+        else
+          v = lay.parameter(gamma, i);
+        widen_pack(v, q);
+#pragma unroll
+        for (int j = 0; j < kN / 2; ++j)
+          f[j] = mul(f[j], q[j]);
       }
-    store_row<T, TH, NE>(static_cast<T *>(p.y) + row * p.ldy, p.cols, tid, vec, x);
+      if (beta) {
+        if (LAYOUT == kShifted)
+          v.w = beta_copy[i * TH + tid];
+        else
+          v = lay.parameter(beta, i);
+        widen_pack(v, q);
+#pragma unroll
+        for (int j = 0; j < kN / 2; ++j)
+          f[j] = add(f[j], q[j]);
+      }
+      narrow_pack(f, v);
+      lay.store(y, i, v);
+    }
     if (tid == 0) {
       if (p.mean)
         static_cast<R *>(p.mean)[row] = mean;
       if (p.rstd)
         static_cast<R *>(p.rstd)[row] = rstd;
     }
+    if (!more)
+      return;
+#pragma unroll
+    for (int i = 0; i < kPacks; ++i)
+      x[i] = next[i];
   }
 }
 
@@ -212,23 +483,23 @@ __device__ __forceinline__ void norm_rows_wide(const hexir_layer_norm_args_t &p)
   typedef real_t<T> R;
   constexpr int TH = 512;
   __shared__ R slots[2][2 * TH / 32];
-  const R n = static_cast<R>(p.cols);
+  const R n = static_cast<R>(p.cols), inv_n = R(1) / n;
   const T *gamma = static_cast<const T *>(p.gamma);
   const T *beta = static_cast<const T *>(p.beta);
   for (uint64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const T *x = static_cast<const T *>(p.x) + row * p.ldx;
     T *y = static_cast<T *>(p.y) + row * p.ldy;
-    R sum = 0, none = 0, m2 = 0;
+    R sum = 0, m2 = 0;
     for (uint64_t c = threadIdx.x; c < p.cols; c += TH)
       sum += widen(x[c]);
-    row_sum2<TH>(sum, none, slots[0]);
-    const R mean = sum / n;
+    row_sum<TH>(sum, slots[0]);
+    const R mean = sum / n;  // exact for a row of one small integer
     for (uint64_t c = threadIdx.x; c < p.cols; c += TH) {
       const R d = widen(x[c]) - mean;
       m2 += d * d;
     }
-    row_sum2<TH>(m2, none, slots[1]);
-    const R rstd = inv_sqrt(m2 / n + static_cast<R>(p.eps));
+    row_sum<TH>(m2, slots[1]);
+    const R rstd = inv_sqrt(m2 * inv_n + static_cast<R>(p.eps));
     for (uint64_t c = threadIdx.x; c < p.cols; c += TH) {
       R v = (widen(x[c]) - mean) * rstd;
       if (gamma)
@@ -248,78 +519,127 @@ __device__ __forceinline__ void norm_rows_wide(const hexir_layer_norm_args_t &p)
 }
 
 // The gradient; block b takes rows b, b + grid, ... (by warps for TH == 32)
-// and leaves its sums of dy * xhat and dy in partial row b.
-template <typename T, int TH, int NE>
+// and leaves its sums of dy * xhat and dy in partial row b.  As in the
+// forward pass, the next row's x and dy are on their way during this one's
+// (AHEAD; not where a thread's sums and rows fill its registers).
+template <typename T, int TH, int NE, int LAYOUT, bool AHEAD>
 __device__ __forceinline__ void norm_grad_rows(
     const hexir_layer_norm_grad_args_t &p) {
   typedef real_t<T> R;
-  constexpr int kN = Pack<T>::kN;
+  typedef Row<T, TH, NE, LAYOUT> Lay;
+  constexpr int kN = Lay::kN, kPacks = Lay::kPacks;
   constexpr uint32_t kRows = TH == 32 ? 8 : 1;
   __shared__ R slots[2][TH == 32 ? 1 : 2 * TH / 32];
-  __shared__ R joined[TH == 32 ? 8 * 32 * 2 : 1];
+  __shared__ R joined[TH == 32 ? 8 : 1][TH == 32 ? 32 * NE : 1];
   const uint32_t tid = TH == 32 ? threadIdx.x % 32 : threadIdx.x;
-  const bool vec = p.vec != 0;
   const R inv_n = R(1) / static_cast<R>(p.cols);
-  R dgamma[NE], dbeta[NE];
+  const T *x_rows = static_cast<const T *>(p.x);
+  const T *dy_rows = static_cast<const T *>(p.dy);
+  const R *means = static_cast<const R *>(p.mean);
+  const R *rstds = static_cast<const R *>(p.rstd);
+  const uint64_t step = (uint64_t)gridDim.x * kRows;
+  uint64_t row = (uint64_t)blockIdx.x * kRows + (TH == 32 ? threadIdx.x / 32 : 0);
+  const Lay lay(tid, p.cols, x_rows + row * p.ldx);
+  Two<R> dgamma[NE / 2], dbeta[NE / 2];
 #pragma unroll
-  for (int i = 0; i < NE; ++i)
-    dgamma[i] = dbeta[i] = 0;
-  Pack<T> g[NE / kN];
-  if (p.gamma) {
-    load_row<T, TH, NE>(static_cast<const T *>(p.gamma), p.cols, tid, vec,
-                        narrow<T>(R(0)), g);
-  } else {
+  for (int i = 0; i < NE / 2; ++i)
+    dgamma[i] = dbeta[i] = twice(R(0));
+  Pack<T> g[kPacks];
 #pragma unroll
-    for (int i = 0; i < NE / kN; ++i)
+  for (int i = 0; i < kPacks; ++i) {
+    if (!p.gamma) {
+      Two<R> one[kN / 2];
 #pragma unroll
-      for (int j = 0; j < kN; ++j)
-        g[i].v[j] = narrow<T>(R(1));
+      for (int j = 0; j < kN / 2; ++j)
+        one[j] = twice(R(1));
+      narrow_pack(one, g[i]);
+    } else {
+      g[i] = lay.parameter(static_cast<const T *>(p.gamma), i);
+    }
+  }
+  Pack<T> x[kPacks], dy[kPacks], next_x[AHEAD ? kPacks : 1],
+      next_dy[AHEAD ? kPacks : 1];
+  R mean = 0, rstd = 0, next_mean = 0, next_rstd = 0;
+  if (AHEAD && row < p.rows) {
+    lay.template load<true>(x_rows + row * p.ldx, x);
+    lay.template load<true>(dy_rows + row * p.lddy, dy);
+    mean = means[row];
+    rstd = rstds[row];
   }
   uint32_t turn = 0;
-  for (uint64_t row = (uint64_t)blockIdx.x * kRows +
-                      (TH == 32 ? threadIdx.x / 32 : 0);
-       row < p.rows; row += (uint64_t)gridDim.x * kRows, turn ^= 1u) {
-    Pack<T> x[NE / kN], dy[NE / kN];
-    load_row<T, TH, NE>(static_cast<const T *>(p.x) + row * p.ldx, p.cols, tid,
-                        vec, narrow<T>(R(0)), x);
-    load_row<T, TH, NE>(static_cast<const T *>(p.dy) + row * p.lddy, p.cols,
-                        tid, vec, narrow<T>(R(0)), dy);
-    const R mean = static_cast<const R *>(p.mean)[row];
-    const R rstd = static_cast<const R *>(p.rstd)[row];
-    R a = 0, b = 0;  // columns past the end have dy = 0
-#pragma unroll
-    for (int i = 0; i < NE / kN; ++i)
-#pragma unroll
-      for (int j = 0; j < kN; ++j) {
-        const R xhat = (widen(x[i].v[j]) - mean) * rstd;
-        const R d = widen(dy[i].v[j]);
-        const R gd = d * widen(g[i].v[j]);
-        a += gd;
-        b += gd * xhat;
-        dgamma[i * kN + j] += d * xhat;
-        dbeta[i * kN + j] += d;
+  for (; row < p.rows; row += step, turn ^= 1u) {
+    Pack<T> r[kPacks];
+    if constexpr (AHEAD) {
+      if (row + step < p.rows) {
+        lay.template load<true>(x_rows + (row + step) * p.ldx, next_x);
+        lay.template load<true>(dy_rows + (row + step) * p.lddy, next_dy);
+        next_mean = means[row + step];
+        next_rstd = rstds[row + step];
       }
+    } else {
+      lay.template load<true>(x_rows + row * p.ldx, x);
+      lay.template load<true>(dy_rows + row * p.lddy, dy);
+      mean = means[row];
+      rstd = rstds[row];
+    }
+    if (p.residual && p.dx)
+      lay.template load<true>(static_cast<const T *>(p.residual) + row * p.ldr, r);
+    Two<R> a2 = twice(R(0)), b2 = a2;  // elements outside the row: dy = 0
+#pragma unroll
+    for (int i = 0; i < kPacks; ++i) {
+      Two<R> fx[kN / 2], fd[kN / 2], fg[kN / 2];
+      widen_pack(x[i], fx);
+      widen_pack(dy[i], fd);
+      widen_pack(g[i], fg);
+#pragma unroll
+      for (int j = 0; j < kN / 2; ++j) {
+        const Two<R> xhat = mul(add(fx[j], twice(-mean)), twice(rstd));
+        const Two<R> gd = mul(fd[j], fg[j]);
+        a2 = add(a2, gd);
+        b2 = fma(gd, xhat, b2);
+        Two<R> &dg = dgamma[i * kN / 2 + j], &db = dbeta[i * kN / 2 + j];
+        dg = fma(fd[j], xhat, dg);
+        db = add(db, fd[j]);
+      }
+    }
     if (p.dx) {
+      R a = a2.x + a2.y, b = b2.x + b2.y;
       row_sum2<TH>(a, b, slots[turn]);
-      a *= inv_n;
-      b *= inv_n;
-      Pack<T> r[NE / kN];
-      if (p.residual)
-        load_row<T, TH, NE>(static_cast<const T *>(p.residual) + row * p.ldr,
-                            p.cols, tid, vec, narrow<T>(R(0)), r);
+      // rstd (g - a - xhat b), with xhat = (x - mean) rstd, as a polynomial
+      // in g and x - mean.
+      const R ca = -a * inv_n * rstd, cb = -b * inv_n * rstd * rstd;
+      T *dx = static_cast<T *>(p.dx) + row * p.lddx;
 #pragma unroll
-      for (int i = 0; i < NE / kN; ++i)
+      for (int i = 0; i < kPacks; ++i) {
+        if (!lay.some(i))
+          continue;
+        Two<R> fx[kN / 2], fd[kN / 2], fg[kN / 2];
+        widen_pack(x[i], fx);
+        widen_pack(dy[i], fd);
+        widen_pack(g[i], fg);
 #pragma unroll
-        for (int j = 0; j < kN; ++j) {
-          const R xhat = (widen(x[i].v[j]) - mean) * rstd;
-          const R gd = widen(dy[i].v[j]) * widen(g[i].v[j]);
-          R v = rstd * (gd - a - xhat * b);
-          if (p.residual)
-            v += widen(r[i].v[j]);
-          x[i].v[j] = narrow<T>(v);
+        for (int j = 0; j < kN / 2; ++j)
+          fx[j] = fma(mul(fd[j], fg[j]), twice(rstd),
+                      fma(add(fx[j], twice(-mean)), twice(cb), twice(ca)));
+        if (p.residual) {
+          widen_pack(r[i], fd);
+#pragma unroll
+          for (int j = 0; j < kN / 2; ++j)
+            fx[j] = add(fx[j], fd[j]);
         }
-      store_row<T, TH, NE>(static_cast<T *>(p.dx) + row * p.lddx, p.cols, tid,
-                           vec, x);
+        Pack<T> out;
+        narrow_pack(fx, out);
+        lay.store(dx, i, out);
+      }
+    }
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int i = 0; i < kPacks; ++i) {
+        x[i] = next_x[i];
+        dy[i] = next_dy[i];
+      }
+      mean = next_mean;
+      rstd = next_rstd;
     }
   }
   if (!p.partials)
@@ -327,36 +647,40 @@ __device__ __forceinline__ void norm_grad_rows(
   R *part = static_cast<R *>(p.partials) + (uint64_t)blockIdx.x * 2 * p.cols;
   if (TH != 32) {
 #pragma unroll
-    for (int i = 0; i < NE / kN; ++i)
+    for (int i = 0; i < kPacks; ++i)
 #pragma unroll
       for (int j = 0; j < kN; ++j) {
-        const uint32_t c = column<T, TH>(i, j, tid, vec);
+        const uint32_t c = lay.column(i, j);
         if (c < p.cols) {
-          part[c] = dgamma[i * kN + j];
-          part[(uint64_t)p.cols + c] = dbeta[i * kN + j];
+          part[c] = half_of(dgamma[(i * kN + j) / 2], j);
+          part[(uint64_t)p.cols + c] = half_of(dbeta[(i * kN + j) / 2], j);
         }
       }
     return;
   }
-  // Join the 8 warps' sums, one element of every lane at a time.
+  // The 8 warps' rows may differ in phase: their sums meet by column.
   const uint32_t warp = threadIdx.x / 32;
 #pragma unroll
-  for (int i = 0; i < NE / kN; ++i)
+  for (int which = 0; which < 2; ++which) {
 #pragma unroll
-    for (int j = 0; j < kN; ++j) {
-      joined[(warp * 32 + tid) * 2] = dgamma[i * kN + j];
-      joined[(warp * 32 + tid) * 2 + 1] = dbeta[i * kN + j];
-      __syncthreads();
-      const uint32_t c = column<T, TH>(i, j, tid, vec);
-      if (warp < 2 && c < p.cols) {
-        R s = 0;
+    for (int i = 0; i < kPacks; ++i)
 #pragma unroll
-        for (int w = 0; w < 8; ++w)
-          s += joined[(w * 32 + tid) * 2 + warp];
-        part[(uint64_t)warp * p.cols + c] = s;
+      for (int j = 0; j < kN; ++j) {
+        const uint32_t c = lay.column(i, j);
+        if (c < p.cols)
+          joined[warp][c] =
+              half_of(which ? dbeta[(i * kN + j) / 2] : dgamma[(i * kN + j) / 2], j);
       }
-      __syncthreads();
+    __syncthreads();
+    for (uint32_t c = threadIdx.x; c < p.cols; c += 256) {
+      R s = 0;
+#pragma unroll
+      for (int w = 0; w < 8; ++w)
+        s += joined[w][c];
+      part[(uint64_t)which * p.cols + c] = s;
     }
+    __syncthreads();
+  }
 }
 
 // Longer rows: dx in three passes (the later two from L2); dgamma and dbeta
@@ -426,27 +750,32 @@ __device__ __forceinline__ void norm_grad_columns(
   }
 }
 
-// out[c] = sum over parts of partials[part * stride + c], in part order within
-// each of 8 interleaved runs, the runs joined in order.
+// out[c] = sum over parts of partials[part * stride + c]: 32 interleaved runs,
+// each in part order, joined in order.
 template <typename T>
 __device__ __forceinline__ void column_sums(const real_t<T> *partials,
                                             uint64_t stride, uint32_t parts,
                                             T *out, uint64_t cols) {
   typedef real_t<T> R;
-  __shared__ R joined[8][32];
-  const uint64_t c = (uint64_t)blockIdx.x * 32 + threadIdx.x % 32;
-  const uint32_t lane = threadIdx.x / 32;
+  __shared__ R joined[32][33];
+  const uint32_t lane = threadIdx.x % 32, run = threadIdx.x / 32;
+  const uint64_t c = (uint64_t)blockIdx.x * 32 + lane;
   R s = 0;
-  if (c < cols)
-    for (uint32_t i = lane; i < parts; i += 8)
+  if (c < cols) {
+#pragma unroll 4
+    for (uint32_t i = run; i < parts; i += 32)
       s += partials[i * stride + c];
-  joined[lane][threadIdx.x % 32] = s;
-  __syncthreads();
-  if (lane == 0 && c < cols) {
-    for (int w = 1; w < 8; ++w)
-      s += joined[w][threadIdx.x];
-    out[c] = narrow<T>(s);
   }
+  joined[run][lane] = s;
+  __syncthreads();
+  // Warp w adds up column w, lane by lane in a fixed tree.
+  s = joined[lane][run];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+  const uint64_t mine = (uint64_t)blockIdx.x * 32 + run;
+  if (lane == 0 && mine < cols)
+    out[mine] = narrow<T>(s);
 }
 
 // dgamma (blockIdx.y == 0) and dbeta (1) from the partial rows.
@@ -476,55 +805,55 @@ __device__ __forceinline__ void output_grad(const hexir_output_grad_args_t &p) {
   T *dz = static_cast<T *>(p.dz) + col;
   const uint32_t row0 = blockIdx.y * p.rows_per_part;
   const uint32_t rows = row0 < p.m ? min(p.rows_per_part, p.m - row0) : 0;
-  float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  Two<float> sum[4] = {{0, 0}, {0, 0}, {0, 0}, {0, 0}};
   if (left) {
     for (uint32_t i = warp; i < rows; i += 8) {
       const uint64_t row = row0 + i;
       Pack<T> g, at;
       if (whole) {
-        g = *reinterpret_cast<const Pack<T> *>(dy + row * p.lddy);
+        g.w = __ldcs(reinterpret_cast<const uint4 *>(dy + row * p.lddy));
         if (p.activation)
-          at = *reinterpret_cast<const Pack<T> *>(z + row * p.ldp);
+          at.w = __ldcs(reinterpret_cast<const uint4 *>(z + row * p.ldp));
       } else {
+        T e[8], f[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const bool in = static_cast<uint32_t>(j) < left;
-          g.v[j] = in ? dy[row * p.lddy + j] : narrow<T>(0.0f);
-          at.v[j] = in && p.activation ? z[row * p.ldp + j] : narrow<T>(0.0f);
+          e[j] = in ? dy[row * p.lddy + j] : narrow<T>(0.0f);
+          f[j] = in && p.activation ? z[row * p.ldp + j] : narrow<T>(0.0f);
         }
+        g.w = *reinterpret_cast<const uint4 *>(e);
+        at.w = *reinterpret_cast<const uint4 *>(f);
       }
+      Two<float> v[4], s[4];
       if (p.activation) {
-        float v[8], s[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          v[j] = widen(g.v[j]);
-          s[j] = widen(at.v[j]);
-        }
-        slope_f32(p.activation, s, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          g.v[j] = narrow<T>(v[j]);
+        widen_pack(g, v);
+        widen_pack(at, s);
+        slope_f32(p.activation, reinterpret_cast<const float(&)[8]>(s),
+                  reinterpret_cast<float(&)[8]>(v));
+        narrow_pack(v, g);
       }
       if (p.dz) {
         if (whole) {
-          *reinterpret_cast<Pack<T> *>(dz + row * p.lddz) = g;
+          *reinterpret_cast<uint4 *>(dz + row * p.lddz) = g.w;
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             if (static_cast<uint32_t>(j) < left)
-              dz[row * p.lddz + j] = g.v[j];
+              dz[row * p.lddz + j] = pack_get(g, j);
         }
       }
+      widen_pack(g, v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        sum[j] += widen(g.v[j]);
+      for (int j = 0; j < 4; ++j)
+        sum[j] = add(sum[j], v[j]);
     }
   }
   if (!p.partials)
     return;
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    joined[warp][j * 32 + lane] = sum[j];
+    joined[warp][j * 32 + lane] = half_of(sum[j / 2], j);
   __syncthreads();
   float s = joined[0][threadIdx.x];
 #pragma unroll
@@ -544,26 +873,22 @@ __device__ __forceinline__ void output_grad_join(
 
 }  // namespace
 
-#define NORM(SUFFIX, T, TH, NE)                                                \
-  extern "C" __global__ void __launch_bounds__(TH == 32 ? 256 : TH)            \
-      hexir_layer_norm_##SUFFIX##_##TH##x##NE(                                 \
+// Kernels by threads per row, elements per thread and layout: w whole, h
+// shifted (16-bit types), s any (fewer shapes).  MINB blocks share an SM.
+#define NORM(SUFFIX, T, TH, NE, MODE, LAYOUT, MINB)                            \
+  extern "C" __global__ void __launch_bounds__(TH == 32 ? 256 : TH, MINB)      \
+      hexir_layer_norm_##SUFFIX##_##MODE##TH##x##NE(                           \
           const hexir_layer_norm_args_t args) {                                \
-    norm_rows<T, TH, NE>(args);                                                \
-  }                                                                            \
-  extern "C" __global__ void __launch_bounds__(TH == 32 ? 256 : TH)            \
-      hexir_layer_norm_grad_##SUFFIX##_##TH##x##NE(                            \
+    norm_rows<T, TH, NE, LAYOUT>(args);                                        \
+  }
+#define NORM_GRAD(SUFFIX, T, TH, NE, MODE, LAYOUT, MINB, AHEAD)                \
+  extern "C" __global__ void __launch_bounds__(TH == 32 ? 256 : TH, MINB)      \
+      hexir_layer_norm_grad_##SUFFIX##_##MODE##TH##x##NE(                      \
           const hexir_layer_norm_grad_args_t args) {                           \
-    norm_grad_rows<T, TH, NE>(args);                                           \
+    norm_grad_rows<T, TH, NE, LAYOUT, AHEAD>(args);                            \
   }
 
 #define NORMS(SUFFIX, T)                                                       \
-  NORM(SUFFIX, T, 32, 8)                                                       \
-  NORM(SUFFIX, T, 32, 16)                                                      \
-  NORM(SUFFIX, T, 32, 32)                                                      \
-  NORM(SUFFIX, T, 256, 8)                                                      \
-  NORM(SUFFIX, T, 256, 16)                                                     \
-  NORM(SUFFIX, T, 512, 16)                                                     \
-  NORM(SUFFIX, T, 1024, 16)                                                    \
   extern "C" __global__ void __launch_bounds__(512)                            \
       hexir_layer_norm_##SUFFIX##_wide(const hexir_layer_norm_args_t args) {   \
     norm_rows_wide<T>(args);                                                   \
@@ -578,23 +903,89 @@ __device__ __forceinline__ void output_grad_join(
           const hexir_layer_norm_grad_args_t args) {                           \
     norm_grad_columns<T>(args);                                                \
   }                                                                            \
-  extern "C" __global__ void __launch_bounds__(256)                            \
+  extern "C" __global__ void __launch_bounds__(1024)                           \
       hexir_layer_norm_grad_##SUFFIX##_join(                                   \
           const hexir_layer_norm_grad_args_t args) {                           \
     norm_grad_join<T>(args);                                                   \
   }
 
-NORMS(f64, double)
+#define NORMS_16(SUFFIX, T)                                                    \
+  NORMS(SUFFIX, T)                                                             \
+  NORM(SUFFIX, T, 32, 8, w, kWhole, 5)                                         \
+  NORM(SUFFIX, T, 32, 32, w, kWhole, 2)                                        \
+  NORM(SUFFIX, T, 256, 8, w, kWhole, 5)                                        \
+  NORM(SUFFIX, T, 256, 16, w, kWhole, 4)                                       \
+  NORM(SUFFIX, T, 256, 32, w, kWhole, 2)                                       \
+  NORM(SUFFIX, T, 512, 32, w, kWhole, 1)                                       \
+  NORM(SUFFIX, T, 32, 8, h, kShifted, 5)                                       \
+  NORM(SUFFIX, T, 32, 32, h, kShifted, 2)                                      \
+  NORM(SUFFIX, T, 256, 8, h, kShifted, 5)                                      \
+  NORM(SUFFIX, T, 256, 16, h, kShifted, 4)                                     \
+  NORM(SUFFIX, T, 256, 32, h, kShifted, 2)                                     \
+  NORM(SUFFIX, T, 512, 32, h, kShifted, 1)                                     \
+  NORM(SUFFIX, T, 32, 32, s, kAny, 2)                                          \
+  NORM(SUFFIX, T, 256, 16, s, kAny, 3)                                         \
+  NORM(SUFFIX, T, 512, 32, s, kAny, 1)                                         \
+  NORM_GRAD(SUFFIX, T, 32, 8, w, kWhole, 3, true)                              \
+  NORM_GRAD(SUFFIX, T, 32, 32, w, kWhole, 1, true)                             \
+  NORM_GRAD(SUFFIX, T, 256, 8, w, kWhole, 3, true)                             \
+  NORM_GRAD(SUFFIX, T, 256, 16, w, kWhole, 2, true)                            \
+  NORM_GRAD(SUFFIX, T, 512, 16, w, kWhole, 1, true)                            \
+  NORM_GRAD(SUFFIX, T, 1024, 16, w, kWhole, 1, false)                          \
+  NORM_GRAD(SUFFIX, T, 32, 8, h, kShifted, 3, true)                            \
+  NORM_GRAD(SUFFIX, T, 32, 32, h, kShifted, 1, true)                           \
+  NORM_GRAD(SUFFIX, T, 256, 8, h, kShifted, 3, true)                           \
+  NORM_GRAD(SUFFIX, T, 256, 16, h, kShifted, 2, true)                          \
+  NORM_GRAD(SUFFIX, T, 512, 16, h, kShifted, 1, true)                          \
+  NORM_GRAD(SUFFIX, T, 1024, 16, h, kShifted, 1, false)                        \
+  NORM_GRAD(SUFFIX, T, 32, 16, s, kAny, 1, true)                               \
+  NORM_GRAD(SUFFIX, T, 256, 16, s, kAny, 1, true)                              \
+  NORM_GRAD(SUFFIX, T, 1024, 16, s, kAny, 1, false)
+
+NORMS_16(bf16, __nv_bfloat16)
+NORMS_16(f16, __half)
+
 NORMS(f32, float)
-NORMS(bf16, __nv_bfloat16)
-NORMS(f16, __half)
+NORM(f32, float, 32, 8, w, kWhole, 5)
+NORM(f32, float, 32, 32, w, kWhole, 2)
+NORM(f32, float, 256, 8, w, kWhole, 5)
+NORM(f32, float, 256, 16, w, kWhole, 4)
+NORM(f32, float, 512, 16, w, kWhole, 2)
+NORM(f32, float, 1024, 16, w, kWhole, 1)
+NORM(f32, float, 32, 32, s, kAny, 2)
+NORM(f32, float, 256, 16, s, kAny, 2)
+NORM(f32, float, 1024, 16, s, kAny, 1)
+NORM_GRAD(f32, float, 32, 8, w, kWhole, 2, true)
+NORM_GRAD(f32, float, 32, 16, w, kWhole, 1, true)
+NORM_GRAD(f32, float, 256, 8, w, kWhole, 3, true)
+NORM_GRAD(f32, float, 256, 16, w, kWhole, 1, true)
+NORM_GRAD(f32, float, 512, 16, w, kWhole, 1, false)
+NORM_GRAD(f32, float, 32, 16, s, kAny, 1, true)
+NORM_GRAD(f32, float, 256, 16, s, kAny, 1, true)
+NORM_GRAD(f32, float, 512, 16, s, kAny, 1, false)
+
+NORMS(f64, double)
+NORM(f64, double, 32, 8, w, kWhole, 3)
+NORM(f64, double, 32, 16, w, kWhole, 2)
+NORM(f64, double, 256, 8, w, kWhole, 3)
+NORM(f64, double, 512, 8, w, kWhole, 1)
+NORM(f64, double, 512, 16, w, kWhole, 1)
+NORM(f64, double, 32, 16, s, kAny, 2)
+NORM(f64, double, 256, 8, s, kAny, 3)
+NORM(f64, double, 512, 16, s, kAny, 1)
+NORM_GRAD(f64, double, 32, 8, w, kWhole, 1, true)
+NORM_GRAD(f64, double, 256, 8, w, kWhole, 1, true)
+NORM_GRAD(f64, double, 512, 8, w, kWhole, 1, false)
+NORM_GRAD(f64, double, 32, 8, s, kAny, 1, true)
+NORM_GRAD(f64, double, 256, 8, s, kAny, 1, true)
+NORM_GRAD(f64, double, 512, 8, s, kAny, 1, false)
 
 #define OUTPUT_GRAD(SUFFIX, T)                                                 \
   extern "C" __global__ void __launch_bounds__(256)                            \
       hexir_linear_output_grad_##SUFFIX(const hexir_output_grad_args_t args) { \
     output_grad<T>(args);                                                      \
   }                                                                            \
-  extern "C" __global__ void __launch_bounds__(256)                            \
+  extern "C" __global__ void __launch_bounds__(1024)                           \
       hexir_linear_output_grad_##SUFFIX##_join(                                \
           const hexir_output_grad_args_t args) {                               \
     output_grad_join<T>(args);                                                 \

@@ -71,7 +71,7 @@ typedef struct {
   void *y, *mean, *rstd;
   uint64_t ldx, ldy, rows;
   double eps;
-  uint32_t cols, vec;
+  uint32_t cols, reserved;
 } hexir_layer_norm_args_t;
 
 typedef struct {
@@ -79,7 +79,7 @@ typedef struct {
   void *dx, *dgamma, *dbeta;
   void *partials;         /* [parts][2][cols] f32 (f64) */
   uint64_t lddy, ldx, ldr, lddx, rows;
-  uint32_t cols, vec, parts, reserved;
+  uint32_t cols, parts;
 } hexir_layer_norm_grad_args_t;
 
 #ifdef __cplusplus

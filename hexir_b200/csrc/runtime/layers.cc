@@ -22,12 +22,127 @@ namespace hexir {
 
 namespace {
 
-constexpr int kNormShapes = 7;
-// Threads per row (32: a warp, 8 rows per block) and elements per thread.
-constexpr struct {
-  uint32_t threads, elements;
-} kNorm[kNormShapes] = {{32, 8},   {32, 16},  {32, 32},  {256, 8},
-                        {256, 16}, {512, 16}, {1024, 16}};
+// How a norm's rows lie: in whole 16-byte packs; in packs that every tensor's
+// row cuts at the same place (16-bit types); or anyhow.
+enum Layout { kWhole, kShifted, kAny };
+
+// Launch shapes of the norm kernels: the shape's name in layer_norm.cu, threads per row (32: a warp, 8
+// rows per block), elements per thread, and the persistent blocks per SM its
+// registers allow.  A row runs the first shape of its kind that holds it.
+struct NormShape {
+  const char *name;
+  uint32_t threads, elements, per_sm;
+  Layout layout;
+  uint32_t block() const { return threads == 32 ? 256 : threads; }
+  uint32_t rows() const { return threads == 32 ? 8 : 1; }
+  // Shared memory of the forward's shifted gamma and beta (16-bit types).
+  uint32_t copies() const { return rows() * threads * elements * 2 * 2; }
+};
+constexpr int kMaxShapes = 15;
+// By the kind of type: 16-bit, f32, f64.
+constexpr NormShape kNorm[3][kMaxShapes] = {
+    {{"w32x8", 32, 8, 5, kWhole},
+     {"w32x32", 32, 32, 2, kWhole},
+     {"w256x8", 256, 8, 5, kWhole},
+     {"w256x16", 256, 16, 4, kWhole},
+     {"w256x32", 256, 32, 2, kWhole},
+     {"w512x32", 512, 32, 1, kWhole},
+     {"h32x8", 32, 8, 5, kShifted},
+     {"h32x32", 32, 32, 2, kShifted},
+     {"h256x8", 256, 8, 5, kShifted},
+     {"h256x16", 256, 16, 4, kShifted},
+     {"h256x32", 256, 32, 2, kShifted},
+     {"h512x32", 512, 32, 1, kShifted},
+     {"s32x32", 32, 32, 2, kAny},
+     {"s256x16", 256, 16, 3, kAny},
+     {"s512x32", 512, 32, 1, kAny}},
+    {{"w32x8", 32, 8, 5, kWhole},
+     {"w32x32", 32, 32, 2, kWhole},
+     {"w256x8", 256, 8, 5, kWhole},
+     {"w256x16", 256, 16, 4, kWhole},
+     {"w512x16", 512, 16, 2, kWhole},
+     {"w1024x16", 1024, 16, 1, kWhole},
+     {"s32x32", 32, 32, 2, kAny},
+     {"s256x16", 256, 16, 2, kAny},
+     {"s1024x16", 1024, 16, 1, kAny}},
+    {{"w32x8", 32, 8, 3, kWhole},
+     {"w32x16", 32, 16, 2, kWhole},
+     {"w256x8", 256, 8, 3, kWhole},
+     {"w512x8", 512, 8, 1, kWhole},
+     {"w512x16", 512, 16, 1, kWhole},
+     {"s32x16", 32, 16, 2, kAny},
+     {"s256x8", 256, 8, 3, kAny},
+     {"s512x16", 512, 16, 1, kAny}}};
+constexpr NormShape kNormGrad[3][kMaxShapes] = {
+    {{"w32x8", 32, 8, 3, kWhole},
+     {"w32x32", 32, 32, 1, kWhole},
+     {"w256x8", 256, 8, 3, kWhole},
+     {"w256x16", 256, 16, 2, kWhole},
+     {"w512x16", 512, 16, 1, kWhole},
+     {"w1024x16", 1024, 16, 1, kWhole},
+     {"h32x8", 32, 8, 3, kShifted},
+     {"h32x32", 32, 32, 1, kShifted},
+     {"h256x8", 256, 8, 3, kShifted},
+     {"h256x16", 256, 16, 2, kShifted},
+     {"h512x16", 512, 16, 1, kShifted},
+     {"h1024x16", 1024, 16, 1, kShifted},
+     {"s32x16", 32, 16, 1, kAny},
+     {"s256x16", 256, 16, 1, kAny},
+     {"s1024x16", 1024, 16, 1, kAny}},
+    {{"w32x8", 32, 8, 2, kWhole},
+     {"w32x16", 32, 16, 1, kWhole},
+     {"w256x8", 256, 8, 3, kWhole},
+     {"w256x16", 256, 16, 1, kWhole},
+     {"w512x16", 512, 16, 1, kWhole},
+     {"s32x16", 32, 16, 1, kAny},
+     {"s256x16", 256, 16, 1, kAny},
+     {"s512x16", 512, 16, 1, kAny}},
+    {{"w32x8", 32, 8, 1, kWhole},
+     {"w256x8", 256, 8, 1, kWhole},
+     {"w512x8", 512, 8, 1, kWhole},
+     {"s32x8", 32, 8, 1, kAny},
+     {"s256x8", 256, 8, 1, kAny},
+     {"s512x8", 512, 8, 1, kAny}}};
+
+int kind_of(uint32_t dtype) {
+  return dtype == HEXIR_DTYPE_F64 ? 2 : (dtype == HEXIR_DTYPE_F32 ? 1 : 0);
+}
+
+Layout norm_layout(uint32_t size, uint32_t cols, bool parameters16,
+                   std::initializer_list<std::pair<const void *, uint64_t>> tensors) {
+  bool whole = cols * static_cast<uint64_t>(size) % 16 == 0 && parameters16;
+  bool same = size == 2;
+  const auto first = *tensors.begin();
+  auto phase = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16; };
+  for (const auto &t : tensors) {
+    if (!t.first)
+      continue;
+    whole = whole && phase(t.first) == 0 && t.second * size % 16 == 0;
+    same = same && phase(t.first) == phase(first.first) &&
+           t.second % 8 == first.second % 8;
+  }
+  return whole ? kWhole : (same ? kShifted : kAny);
+}
+
+// -1: a longer row than any shape holds.
+int norm_shape(const NormShape (&shapes)[kMaxShapes], uint32_t cols, Layout layout) {
+  const uint64_t need = cols + (layout == kShifted ? 7ull : 0ull);
+  for (int s = 0; s < kMaxShapes && shapes[s].name; ++s)
+    if (shapes[s].layout == layout &&
+        need <= shapes[s].threads * shapes[s].elements)
+      return s;
+  return -1;
+}
+
+// Persistent blocks; those of a shifted layout stay a multiple of 8 rows
+// apart, so that all rows of a block (of a warp) are cut at the same place.
+uint64_t norm_blocks(const NormShape &shape, Layout layout, uint64_t rows,
+                     uint64_t resident) {
+  const uint64_t blocks = (rows + shape.rows() - 1) / shape.rows();
+  if (blocks <= resident)
+    return blocks;
+  return layout == kShifted ? std::max<uint64_t>(8, resident / 8 * 8) : resident;
+}
 
 const char *const kDtypeName[4] = {"f64", "f32", "bf16", "f16"};
 constexpr uint32_t kDtypeSize[4] = {8, 4, 2, 2};
@@ -40,8 +155,8 @@ struct LayersLib {
   // By HEXIR_PRODUCT_*; skinny is the forward's only.
   CUfunction pair[3] = {}, single[3] = {}, guarded[3] = {}, skinny = nullptr;
   // By dtype.
-  CUfunction norm[4][kNormShapes] = {}, norm_wide[4] = {};
-  CUfunction norm_grad[4][kNormShapes] = {}, norm_grad_wide[4] = {},
+  CUfunction norm[4][kMaxShapes] = {}, norm_wide[4] = {};
+  CUfunction norm_grad[4][kMaxShapes] = {}, norm_grad_wide[4] = {},
              norm_grad_columns[4] = {}, norm_grad_join[4] = {};
   CUfunction output_grad[4] = {}, output_grad_join[4] = {};
 };
@@ -84,11 +199,12 @@ LayersLib *layers_library(DeviceState *dev, std::string *error) {
   for (int t = 0; t < 4; ++t) {
     const std::string norm = std::string("hexir_layer_norm_") + kDtypeName[t];
     const std::string grad = std::string("hexir_layer_norm_grad_") + kDtypeName[t];
-    for (int s = 0; s < kNormShapes; ++s) {
-      const std::string shape = "_" + std::to_string(kNorm[s].threads) + "x" +
-                                std::to_string(kNorm[s].elements);
-      get(&lib->norm[t][s], norm + shape);
-      get(&lib->norm_grad[t][s], grad + shape);
+    const int kind = kind_of(t);
+    for (int s = 0; s < kMaxShapes; ++s) {
+      if (kNorm[kind][s].name)
+        get(&lib->norm[t][s], norm + "_" + kNorm[kind][s].name);
+      if (kNormGrad[kind][s].name)
+        get(&lib->norm_grad[t][s], grad + "_" + kNormGrad[kind][s].name);
     }
     get(&lib->norm_wide[t], norm + "_wide");
     get(&lib->norm_grad_wide[t], grad + "_wide");
@@ -117,6 +233,14 @@ LayersLib *layers_library(DeviceState *dev, std::string *error) {
     r = d.FuncSetAttribute(lib->skinny,
                            CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES,
                            kSmemLimit);
+  // The longest rows' copies pass the 48 KiB that need no attribute.
+  for (int t = 0; t < 4; ++t)
+    for (int s = 0; s < kMaxShapes && r == CUDA_SUCCESS; ++s)
+      if (kind_of(t) == 0 && kNorm[0][s].layout == kShifted &&
+          kNorm[0][s].copies() > 48u * 1024u)
+        r = d.FuncSetAttribute(lib->norm[t][s],
+                               CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES,
+                               static_cast<int>(kNorm[0][s].copies()));
   if (r != CUDA_SUCCESS) {
     d.ModuleUnload(lib->module);
     fail(error, cuda_message("layer kernels setup", r));
@@ -451,13 +575,6 @@ bool extents_ok(uint32_t m, uint32_t n, uint32_t k) {
 
 // ----------------------------------------------------------- the norms
 
-int norm_shape(uint32_t cols) {
-  for (int s = 0; s < kNormShapes; ++s)
-    if (cols <= kNorm[s].threads * kNorm[s].elements)
-      return s;
-  return -1;
-}
-
 constexpr uint32_t kSumsPerColumn = 640;  // hexir_cuda_grad_workspace
 
 }  // namespace
@@ -700,7 +817,7 @@ extern "C" hexir_status_t hexir_cuda_linear_output_grad(
   if (st == HEXIR_OK && c.dbias) {
     void *params[] = {&args};
     st = launch_after(call.lib->output_grad_join[c.dtype], ceil_div(c.n, 32), 1,
-                      256, s, params, "launch hexir_linear_output_grad_join",
+                      1024, s, params, "launch hexir_linear_output_grad_join",
                       &call.error);
   }
   return call.finish(st);
@@ -751,22 +868,25 @@ extern "C" hexir_status_t hexir_cuda_layer_norm(int ordinal,
   args.rows = c.rows;
   args.cols = c.cols;
   args.eps = c.eps;
-  args.vec = rows16(c.x, c.ldx, size) && rows16(c.y, c.ldy, size) &&
-             !off(c.gamma, 16) && !off(c.beta, 16);
+  const Layout layout = norm_layout(size, c.cols, !off(c.gamma, 16) && !off(c.beta, 16),
+                                    {{c.x, c.ldx}, {c.y, c.ldy}});
   void *params[] = {&args};
   ContextGuard guard(call.dev->context);
   CUstream s = static_cast<CUstream>(stream);
-  const int shape = norm_shape(c.cols);
-  const uint64_t cap = 1u << 24;  // the rest by stride
-  if (shape < 0)
+  const int kind = kind_of(c.dtype);
+  const int at = norm_shape(kNorm[kind], c.cols, layout);
+  if (at < 0)
     return call.finish(launch(call.lib->norm_wide[c.dtype],
-                              static_cast<unsigned>(std::min(c.rows, cap)), 1, 512, 0,
-                              s, params, "launch hexir_layer_norm wide", &call.error));
-  const bool warp = kNorm[shape].threads == 32;
-  const uint64_t blocks = warp ? (c.rows + 7) / 8 : c.rows;
-  return call.finish(launch(call.lib->norm[c.dtype][shape],
-                            static_cast<unsigned>(std::min(blocks, cap)), 1,
-                            warp ? 256 : kNorm[shape].threads, 0, s, params,
+                              static_cast<unsigned>(std::min<uint64_t>(c.rows, 1u << 24)),
+                              1, 512, 0, s, params, "launch hexir_layer_norm wide",
+                              &call.error));
+  const NormShape &shape = kNorm[kind][at];
+  const uint64_t resident =
+      static_cast<uint64_t>(std::max(call.dev->sm_count, 1)) * shape.per_sm;
+  const unsigned blocks =
+      static_cast<unsigned>(norm_blocks(shape, layout, c.rows, resident));
+  return call.finish(launch(call.lib->norm[c.dtype][at], blocks, 1, shape.block(),
+                            layout == kShifted ? shape.copies() : 0, s, params,
                             "launch hexir_layer_norm", &call.error));
 }
 
@@ -825,24 +945,23 @@ extern "C" hexir_status_t hexir_cuda_layer_norm_grad(
   args.partials = sums ? c.workspace : nullptr;
   args.rows = c.rows;
   args.cols = c.cols;
-  args.vec = rows16(c.x, c.ldx, size) && rows16(c.dy, c.lddy, size) &&
-             !off(c.gamma, 16) && (!c.dx || rows16(c.dx, c.lddx, size)) &&
-             (!c.residual || rows16(c.residual, c.ldr, size));
+  const Layout layout = norm_layout(
+      size, c.cols, !off(c.gamma, 16),
+      {{c.x, c.ldx}, {c.dy, c.lddy}, {c.dx, c.lddx}, {c.residual, c.ldr}});
   ContextGuard guard(call.dev->context);
   CUstream s = static_cast<CUstream>(stream);
   const uint64_t sms = static_cast<uint64_t>(std::max(call.dev->sm_count, 1));
-  const int shape = norm_shape(c.cols);
+  const int kind = kind_of(c.dtype);
+  const int at = norm_shape(kNormGrad[kind], c.cols, layout);
   hexir_status_t st = HEXIR_OK;
   void *params[] = {&args};
-  if (c.rows && shape >= 0) {
-    const bool warp = kNorm[shape].threads == 32;
-    const uint64_t blocks = warp ? (c.rows + 7) / 8 : c.rows;
-    const uint64_t resident = sms * (kNorm[shape].threads <= 256 ? 2 : 1);
+  if (c.rows && at >= 0) {
+    const NormShape &shape = kNormGrad[kind][at];
     args.parts = static_cast<uint32_t>(
-        std::min<uint64_t>({blocks, resident, uint64_t(kSumsPerColumn / 2)}));
-    st = launch(call.lib->norm_grad[c.dtype][shape], args.parts, 1,
-                warp ? 256 : kNorm[shape].threads, 0, s, params,
-                "launch hexir_layer_norm_grad", &call.error);
+        norm_blocks(shape, layout, c.rows,
+                    std::min<uint64_t>(sms * shape.per_sm, kSumsPerColumn / 2)));
+    st = launch(call.lib->norm_grad[c.dtype][at], args.parts, 1, shape.block(), 0, s,
+                params, "launch hexir_layer_norm_grad", &call.error);
   } else if (c.rows) {
     // The column sums first: dx may be dy.
     if (sums) {
@@ -859,7 +978,7 @@ extern "C" hexir_status_t hexir_cuda_layer_norm_grad(
   }
   if (st == HEXIR_OK && sums)
     st = launch_after(call.lib->norm_grad_join[c.dtype], ceil_div(c.cols, 32), 2,
-                      256, s, params, "launch hexir_layer_norm_grad_join",
+                      1024, s, params, "launch hexir_layer_norm_grad_join",
                       &call.error);
   return call.finish(st);
 }
