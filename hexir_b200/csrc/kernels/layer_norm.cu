@@ -191,18 +191,21 @@ __device__ __forceinline__ T pack_get(const Pack<T> &p, int j) {
 //   kShifted  the same packs of memory, but the row starts `phase` elements
 //             after a boundary: its first pack is filled from element `phase`
 //             on (16-bit types; every tensor of the call has the same phase,
-//             and a block's rows are a multiple of 8 apart so that they
-//             share it);
+//             and a thread's rows are a multiple of 8 apart so that they
+//             share it).  f32 and f64 gain nothing by it: their single
+//             elements make loads that are wide enough;
 //   kAny      single elements tid, tid + TH, ..., so that a warp's accesses
 //             stay consecutive.
 enum Layout { kWhole, kShifted, kAny };
 
-// The packs at the ends of a shifted row, an element at a time.  Out of line:
-// inlined, their predicated loads were more than half of the instructions
-// every pack cost (410 a warp and row of 16 elements a thread).
+// The packs at the ends of a shifted row, an element at a time.  They stand
+// behind branches that a whole warp takes or not: as predicated instructions
+// they were more than half of what every pack cost (410 instructions a warp
+// and row of 16 elements a thread, 243 without), and as calls they made their
+// warp wait for its loads in flight.
 template <typename T>
-__device__ __noinline__ uint4 gather_pack(const T *row, uint32_t column,
-                                          uint32_t cols) {
+__device__ __forceinline__ uint4 gather_pack(const T *row, uint32_t column,
+                                             uint32_t cols) {
   constexpr int kN = Pack<T>::kN;
   T e[kN];
 #pragma unroll
@@ -211,8 +214,8 @@ __device__ __noinline__ uint4 gather_pack(const T *row, uint32_t column,
   return *reinterpret_cast<const uint4 *>(e);
 }
 template <typename T>
-__device__ __noinline__ void scatter_pack(T *row, uint32_t column, uint32_t cols,
-                                          uint4 v) {
+__device__ __forceinline__ void scatter_pack(T *row, uint32_t column,
+                                             uint32_t cols, uint4 v) {
   constexpr int kN = Pack<T>::kN;
   T e[kN];
   *reinterpret_cast<uint4 *>(e) = v;
@@ -221,47 +224,98 @@ __device__ __noinline__ void scatter_pack(T *row, uint32_t column, uint32_t cols
     if (column + j < cols)
       row[column + j] = e[j];
 }
+// The elements of a tensor from its first to its last, gaps between rows
+// included: what a load may touch.
+struct Span {
+  uintptr_t first, last;
+  __device__ __forceinline__ bool holds16(const void *p) const {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    return at >= first && at + 16 <= last;
+  }
+};
+template <typename T>
+__device__ __forceinline__ Span span_of(const T *p, uint64_t ld, uint64_t rows,
+                                        uint32_t cols) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  return {at, at + ((rows - 1) * ld + cols) * sizeof(T)};
+}
 
 template <typename T, int TH, int NE, int LAYOUT>
 struct Row {
   static constexpr int kN = Pack<T>::kN;
   static constexpr int kPacks = NE / kN;
   uint32_t tid, cols, phase;
+  // Shifted rows, a bit per pack: whether it has elements of the row, whether
+  // it has others too, and whether such a one is in this warp.
+  uint32_t some_bits, cut_bits, warp_cut_bits;
 
   __device__ __forceinline__ Row(uint32_t tid_, uint32_t cols_, const void *row)
-      : tid(tid_), cols(cols_),
-        phase(LAYOUT == kShifted
-                  ? static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) % 16 /
-                                          sizeof(T))
-                  : 0) {}
+      : tid(tid_), cols(cols_), phase(0), some_bits(0), cut_bits(0),
+        warp_cut_bits(0) {
+    if (LAYOUT == kShifted) {
+      phase = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T));
+#pragma unroll
+      for (int i = 0; i < kPacks; ++i) {
+        const uint32_t c = column(i, 0);
+        const bool has = (i * TH + tid) * kN < cols + phase;
+        some_bits |= static_cast<uint32_t>(has) << i;
+        cut_bits |= static_cast<uint32_t>(has && (c >= cols || cols - c < kN)) << i;
+      }
+      warp_cut_bits = __reduce_or_sync(0xFFFFFFFFu, cut_bits);
+    }
+  }
   // Column of element j of pack i; wraps below 0 for the elements before the
   // row, so `column < cols` holds for the row's elements alone.
   __device__ __forceinline__ uint32_t column(int i, int j) const {
     return LAYOUT != kAny ? (i * TH + tid) * kN + j - phase
                           : (i * kN + j) * TH + tid;
   }
-  // Whether pack i has elements of the row; whether it has others too.
   __device__ __forceinline__ bool some(int i) const {
-    return LAYOUT == kWhole     ? column(i, 0) < cols
-           : LAYOUT == kShifted ? (i * TH + tid) * kN < cols + phase
-                                : (i * kN) * TH + tid < cols;
+    return LAYOUT == kShifted ? (some_bits >> i & 1u) != 0 : column(i, 0) < cols;
   }
   __device__ __forceinline__ bool cut(int i) const {
-    if (LAYOUT != kShifted)
-      return false;
-    const uint32_t c = column(i, 0);
-    return c >= cols || cols - c < kN;
+    return LAYOUT == kShifted && (cut_bits >> i & 1u) != 0;
   }
-  // The elements of the row as stored, zeros elsewhere.  STREAM: read once,
-  // not kept in L1.
-  template <bool STREAM>
-  __device__ __forceinline__ void load(const T *row, Pack<T> (&v)[kPacks]) const {
+  __device__ __forceinline__ bool warp_cut(int i) const {
+    return LAYOUT == kShifted && (warp_cut_bits >> i & 1u) != 0;
+  }
+  // A cut pack with the elements outside the row (its neighbours' or the
+  // gap's) zeroed.
+  __device__ __forceinline__ uint4 inside(uint4 w, int i) const {
+    const uint32_t c = column(i, 0);
+    uint32_t m[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (sizeof(T) == 2)
+        m[j] = (c + 2 * j < cols ? 0xFFFFu : 0u) |
+               (c + 2 * j + 1 < cols ? 0xFFFF0000u : 0u);
+      else
+        m[j] = c + static_cast<uint32_t>(j * 4 / sizeof(T)) < cols ? 0xFFFFFFFFu : 0u;
+    }
+    return make_uint4(w.x & m[0], w.y & m[1], w.z & m[2], w.w & m[3]);
+  }
+  // The row's packs; a cut one may carry its neighbours' elements until
+  // clean() (which a load must not wait for).  `edge`: the tensor's first or
+  // last row, where such a pack may reach outside it.
+  __device__ __forceinline__ void load(const T *row, const Span &span, bool edge,
+                                       Pack<T> (&v)[kPacks]) const {
 #pragma unroll
     for (int i = 0; i < kPacks; ++i)
-      v[i] = load_pack<STREAM>(row, i);
+      v[i] = load_pack<true>(row, i, span, edge);
   }
+  __device__ __forceinline__ void clean(Pack<T> (&v)[kPacks]) const {
+#pragma unroll
+    for (int i = 0; i < kPacks; ++i)
+      if (warp_cut(i))
+        v[i].w = inside(v[i].w, i);
+  }
+  __device__ __forceinline__ bool apart(const T *row, int i, const Span &span) const {
+    return cut(i) && !span.holds16(row + static_cast<int32_t>(column(i, 0)));
+  }
+  // STREAM: read once, not kept in L1 (where gamma and beta are).
   template <bool STREAM>
-  __device__ __forceinline__ Pack<T> load_pack(const T *row, int i) const {
+  __device__ __forceinline__ Pack<T> load_pack(const T *row, int i,
+                                               const Span &span, bool edge) const {
     Pack<T> v;
     v.w = make_uint4(0, 0, 0, 0);
     if (LAYOUT == kAny) {
@@ -272,13 +326,17 @@ struct Row {
         e[j] = c < cols ? row[c] : narrow<T>(real_t<T>(0));
       }
       v.w = *reinterpret_cast<const uint4 *>(e);
-    } else if (some(i)) {
-      if (cut(i)) {
+      return v;
+    }
+    const uint4 *at =
+        reinterpret_cast<const uint4 *>(row + static_cast<int32_t>(column(i, 0)));
+    if (LAYOUT == kShifted && edge && warp_cut(i)) {
+      if (apart(row, i, span))
         v.w = gather_pack(row, column(i, 0), cols);
-      } else {
-        const uint4 *at = reinterpret_cast<const uint4 *>(row + column(i, 0));
-        v.w = STREAM ? __ldcs(at) : *at;
-      }
+      else if (some(i))
+        v.w = *at;
+    } else if (some(i)) {
+      v.w = STREAM ? __ldcs(at) : *at;
     }
     return v;
   }
@@ -290,27 +348,42 @@ struct Row {
         if (c < cols)
           row[c] = pack_get(v, j);
       }
-    } else if (some(i)) {
+      return;
+    }
+    uint4 *at = reinterpret_cast<uint4 *>(row + static_cast<int32_t>(column(i, 0)));
+    if (warp_cut(i)) {
       if (cut(i))
         scatter_pack(row, column(i, 0), cols, v.w);
-      else
-        __stcs(reinterpret_cast<uint4 *>(row + column(i, 0)), v.w);
+      else if (some(i))
+        __stcs(at, v.w);
+    } else if (some(i)) {
+      __stcs(at, v.w);
     }
   }
   // Pack i of gamma or beta, which start at column 0: as the row's packs
   // lie.
   __device__ __forceinline__ Pack<T> parameter(const T *p, int i) const {
     if (LAYOUT != kShifted)
-      return load_pack<false>(p, i);
+      return load_pack<false>(p, i, Span{}, false);
     Pack<T> v;
     v.w = gather_pack(p, column(i, 0), cols);
     return v;
   }
 };
 
+// Every thread of a row: all of the block's, or, where a block has several
+// rows, of a named barrier per row.
+template <int TH>
+__device__ __forceinline__ void row_sync() {
+  if (TH >= 256)
+    __syncthreads();
+  else
+    asm volatile("bar.sync %0, %1;" ::"r"(threadIdx.x / TH + 1), "n"(TH) : "memory");
+}
+
 // Sum over the TH threads of a row, in an order that depends on TH alone.
-// `slot` holds TH / 32 values (2 * TH / 32 for row_sum2); calls alternate
-// between two slots, so one barrier per call is enough.
+// `slot` holds a value per warp of the block (two for row_sum2); calls
+// alternate between two slots, so one barrier per call is enough.
 template <int TH, typename R>
 __device__ __forceinline__ void row_sum(R &a, R *slot) {
 #pragma unroll
@@ -320,7 +393,8 @@ __device__ __forceinline__ void row_sum(R &a, R *slot) {
     return;
   if (threadIdx.x % 32 == 0)
     slot[threadIdx.x / 32] = a;
-  __syncthreads();
+  row_sync<TH>();
+  slot += threadIdx.x / TH * (TH / 32);
   a = slot[0];
 #pragma unroll
   for (int w = 1; w < TH / 32; ++w)
@@ -340,7 +414,8 @@ __device__ __forceinline__ void row_sum2(R &a, R &b, R *slot) {
     slot[2 * (threadIdx.x / 32)] = a;
     slot[2 * (threadIdx.x / 32) + 1] = b;
   }
-  __syncthreads();
+  row_sync<TH>();
+  slot += threadIdx.x / TH * (2 * TH / 32);
   a = slot[0];
   b = slot[1];
 #pragma unroll
@@ -353,7 +428,8 @@ __device__ __forceinline__ void row_sum2(R &a, R &b, R *slot) {
 __device__ __forceinline__ float inv_sqrt(float v) { return rsqrtf(v); }
 __device__ __forceinline__ double inv_sqrt(double v) { return rsqrt(v); }
 
-// Rows of up to TH * NE columns; TH == 32: a warp per row, 8 rows per block.
+// Rows of up to TH * NE columns, several to a block of 256 threads where TH is
+// less.
 // Blocks are persistent and load their next row before they work on the
 // present one, so that HBM is read while the row's sums and barriers run; the
 // row stays packed in registers, which lets several blocks share an SM.
@@ -362,24 +438,26 @@ __device__ __forceinline__ void norm_rows(const hexir_layer_norm_args_t &p) {
   typedef real_t<T> R;
   typedef Row<T, TH, NE, LAYOUT> Lay;
   constexpr int kN = Lay::kN, kPacks = Lay::kPacks;
-  constexpr uint32_t kRows = TH == 32 ? 8 : 1;
-  __shared__ R slots[2][TH == 32 ? 1 : TH / 32];
+  constexpr uint32_t kRows = TH < 256 ? 256 / TH : 1;
+  __shared__ R slots[2][kRows * TH / 32];
   extern __shared__ uint4 copies[];  // gamma and beta as this block's rows lie
-  const uint32_t tid = TH == 32 ? threadIdx.x % 32 : threadIdx.x;
+  const uint32_t tid = threadIdx.x % TH, group = threadIdx.x / TH;
   const R n = static_cast<R>(p.cols), inv_n = R(1) / n;
   const T *x_rows = static_cast<const T *>(p.x);
   const T *gamma = static_cast<const T *>(p.gamma);
   const T *beta = static_cast<const T *>(p.beta);
   const uint64_t step = (uint64_t)gridDim.x * kRows;
-  uint64_t row = (uint64_t)blockIdx.x * kRows + (TH == 32 ? threadIdx.x / 32 : 0);
+  uint64_t row = (uint64_t)blockIdx.x * kRows + group;
   if (row >= p.rows)
     return;
   const Lay lay(tid, p.cols, x_rows + row * p.ldx);
+  const uint64_t last = p.rows - 1;
+  const Span span = span_of(x_rows, p.ldx, p.rows, p.cols);
   Pack<T> x[kPacks], next[kPacks];
-  lay.template load<true>(x_rows + row * p.ldx, x);
+  lay.load(x_rows + row * p.ldx, span, row == 0 || row == last, x);
   // Shifted rows: gamma and beta as this row's packs lie, in shared memory.
   // Each thread reads back only what it writes here.
-  uint4 *gamma_copy = copies + (TH == 32 ? threadIdx.x / 32 : 0) * (2 * TH * kPacks);
+  uint4 *gamma_copy = copies + group * (2 * TH * kPacks);
   uint4 *beta_copy = gamma_copy + TH * kPacks;
   if (LAYOUT == kShifted) {
 #pragma unroll
@@ -392,8 +470,9 @@ __device__ __forceinline__ void norm_rows(const hexir_layer_norm_args_t &p) {
   }
   for (;; row += step) {
     const bool more = row + step < p.rows;
+    lay.clean(x);
     if (more)
-      lay.template load<true>(x_rows + (row + step) * p.ldx, next);
+      lay.load(x_rows + (row + step) * p.ldx, span, row + step == last, next);
     Two<R> sum2 = twice(R(0));
 #pragma unroll
     for (int i = 0; i < kPacks; ++i) {
@@ -409,22 +488,23 @@ __device__ __forceinline__ void norm_rows(const hexir_layer_norm_args_t &p) {
     Two<R> m2 = twice(R(0));
 #pragma unroll
     for (int i = 0; i < kPacks; ++i) {
-      if (!lay.some(i))
+      if (LAYOUT != kAny && !lay.some(i))
         continue;
       Two<R> f[kN / 2];
       widen_pack(x[i], f);
-      const bool whole = LAYOUT == kWhole || (LAYOUT == kShifted && !lay.cut(i));
 #pragma unroll
-      for (int j = 0; j < kN / 2; ++j) {
+      for (int j = 0; j < kN / 2; ++j)
         f[j] = add(f[j], twice(-mean));
-        if (!whole) {
-          if (lay.column(i, 2 * j) >= p.cols)
-            f[j].x = 0;
-          if (lay.column(i, 2 * j + 1) >= p.cols)
-            f[j].y = 0;
+      if (LAYOUT == kAny || lay.warp_cut(i)) {
+#pragma unroll
+        for (int j = 0; j < kN / 2; ++j) {
+          f[j].x = lay.column(i, 2 * j) < p.cols ? f[j].x : R(0);
+          f[j].y = lay.column(i, 2 * j + 1) < p.cols ? f[j].y : R(0);
         }
-        m2 = fma(f[j], f[j], m2);
       }
+#pragma unroll
+      for (int j = 0; j < kN / 2; ++j)
+        m2 = fma(f[j], f[j], m2);
     }
     R var = m2.x + m2.y;
     row_sum<TH>(var, slots[1]);
@@ -432,7 +512,7 @@ __device__ __forceinline__ void norm_rows(const hexir_layer_norm_args_t &p) {
     T *y = static_cast<T *>(p.y) + row * p.ldy;
 #pragma unroll
     for (int i = 0; i < kPacks; ++i) {
-      if (!lay.some(i))
+      if (LAYOUT != kAny && !lay.some(i))
         continue;
       Two<R> f[kN / 2], q[kN / 2];
       Pack<T> v;
@@ -518,28 +598,55 @@ __device__ __forceinline__ void norm_rows_wide(const hexir_layer_norm_args_t &p)
   }
 }
 
-// The gradient; block b takes rows b, b + grid, ... (by warps for TH == 32)
-// and leaves its sums of dy * xhat and dy in partial row b.  As in the
-// forward pass, the next row's x and dy are on their way during this one's
-// (AHEAD; not where a thread's sums and rows fill its registers).
-template <typename T, int TH, int NE, int LAYOUT, bool AHEAD>
+// cp.async of `bytes` (4, 8 or 16) from global to shared memory.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void *src) {
+  if (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src)
+                 : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src),
+                 "n"(BYTES)
+                 : "memory");
+}
+
+// The gradient; block b takes rows b * kRows on, every kRows * grid, and leaves
+// its sums of dy * xhat and dy in partial row b.
+//
+// The rows to come (x, dy and the residual) are copied into a ring of DEPTH
+// rows in shared memory.  Every thread copies and reads its own packs alone,
+// so the ring needs no barrier, and the registers hold the column sums
+// instead of rows in flight (with one row ahead in registers, two blocks fit
+// an SM and the loads' latency was 5 of 9 cycles between instructions).
+template <typename T, int TH, int NE, int LAYOUT, int DEPTH>
 __device__ __forceinline__ void norm_grad_rows(
     const hexir_layer_norm_grad_args_t &p) {
   typedef real_t<T> R;
   typedef Row<T, TH, NE, LAYOUT> Lay;
   constexpr int kN = Lay::kN, kPacks = Lay::kPacks;
-  constexpr uint32_t kRows = TH == 32 ? 8 : 1;
-  __shared__ R slots[2][TH == 32 ? 1 : 2 * TH / 32];
-  __shared__ R joined[TH == 32 ? 8 : 1][TH == 32 ? 32 * NE : 1];
-  const uint32_t tid = TH == 32 ? threadIdx.x % 32 : threadIdx.x;
+  constexpr uint32_t kRows = TH < 256 ? 256 / TH : 1;
+  constexpr uint32_t kBlock = kRows * TH;
+  constexpr uint32_t kTensor = kPacks * kBlock;  // packs of a tensor's rows
+  __shared__ R slots[2][kRows * 2 * TH / 32];
+  extern __shared__ uint4 ring[];  // [DEPTH][tensors][kPacks][kBlock]
+  const uint32_t tid = threadIdx.x % TH, group = threadIdx.x / TH;
   const R inv_n = R(1) / static_cast<R>(p.cols);
   const T *x_rows = static_cast<const T *>(p.x);
   const T *dy_rows = static_cast<const T *>(p.dy);
+  const T *res_rows = p.dx ? static_cast<const T *>(p.residual) : nullptr;
   const R *means = static_cast<const R *>(p.mean);
   const R *rstds = static_cast<const R *>(p.rstd);
   const uint64_t step = (uint64_t)gridDim.x * kRows;
-  uint64_t row = (uint64_t)blockIdx.x * kRows + (TH == 32 ? threadIdx.x / 32 : 0);
+  uint64_t row = (uint64_t)blockIdx.x * kRows + group;
   const Lay lay(tid, p.cols, x_rows + row * p.ldx);
+  const uint32_t tensors = res_rows ? 3 : 2;
+  uint4 *mine = ring + threadIdx.x;
+  // Rows of single elements: the ring holds them one by one, so that a warp's
+  // accesses fall into different banks.
+  constexpr bool kSingles = LAYOUT == kAny && sizeof(T) >= 4;
+  T *singles = reinterpret_cast<T *>(ring) + threadIdx.x;
+  const uint64_t last = p.rows - 1;
+
   Two<R> dgamma[NE / 2], dbeta[NE / 2];
 #pragma unroll
   for (int i = 0; i < NE / 2; ++i)
@@ -557,39 +664,91 @@ __device__ __forceinline__ void norm_grad_rows(
       g[i] = lay.parameter(static_cast<const T *>(p.gamma), i);
     }
   }
-  Pack<T> x[kPacks], dy[kPacks], next_x[AHEAD ? kPacks : 1],
-      next_dy[AHEAD ? kPacks : 1];
-  R mean = 0, rstd = 0, next_mean = 0, next_rstd = 0;
-  if (AHEAD && row < p.rows) {
-    lay.template load<true>(x_rows + row * p.ldx, x);
-    lay.template load<true>(dy_rows + row * p.lddy, dy);
+  // Places that no copy fills stay 0.
+  for (uint32_t i = 0; i < DEPTH * tensors * kPacks; ++i)
+    mine[i * kBlock] = make_uint4(0, 0, 0, 0);
+
+  auto fetch = [&](uint64_t at, uint32_t stage) {
+    if (at < p.rows) {
+      const T *src[3] = {x_rows + at * p.ldx, dy_rows + at * p.lddy,
+                         res_rows ? res_rows + at * p.ldr : nullptr};
+      const Span spans[3] = {span_of(x_rows, p.ldx, p.rows, p.cols),
+                             span_of(dy_rows, p.lddy, p.rows, p.cols),
+                             span_of(res_rows, p.ldr, p.rows, p.cols)};
+#pragma unroll
+      for (uint32_t t = 0; t < 3; ++t) {
+        if (t == 2 && !res_rows)
+          break;
+#pragma unroll
+        for (int i = 0; i < kPacks; ++i) {
+          const uint32_t at_pack = (stage * tensors + t) * kPacks + i;
+          uint4 *dst = mine + at_pack * kBlock;
+          if (kSingles) {
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+              const uint32_t c = lay.column(i, j);
+              if (c < p.cols)
+                copy_async<sizeof(T) >= 4 ? sizeof(T) : 4>(
+                    smem_addr(singles + (at_pack * kN + j) * kBlock), src[t] + c);
+            }
+          } else if (LAYOUT == kAny) {
+            *dst = lay.template load_pack<true>(src[t], i, spans[t], false).w;
+          } else {
+            const T *from = src[t] + static_cast<int32_t>(lay.column(i, 0));
+            if (LAYOUT == kShifted && (at == 0 || at == last) && lay.warp_cut(i)) {
+              if (lay.apart(src[t], i, spans[t]))
+                *dst = gather_pack(src[t], lay.column(i, 0), p.cols);
+              else if (lay.some(i))
+                copy_async<16>(smem_addr(dst), from);
+            } else if (lay.some(i)) {
+              copy_async<16>(smem_addr(dst), from);
+            }
+          }
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto place = [&](uint32_t stage, uint32_t t, int i) {
+    Pack<T> v;
+    const uint32_t at_pack = (stage * tensors + t) * kPacks + i;
+    if (kSingles) {
+      T e[kN];
+#pragma unroll
+      for (int j = 0; j < kN; ++j)
+        e[j] = singles[(at_pack * kN + j) * kBlock];
+      v.w = *reinterpret_cast<const uint4 *>(e);
+    } else {
+      v.w = mine[at_pack * kBlock];
+    }
+    if (lay.warp_cut(i))
+      v.w = lay.inside(v.w, i);
+    return v;
+  };
+
+#pragma unroll
+  for (uint32_t s = 0; s + 1 < DEPTH; ++s)
+    fetch(row + s * step, s);
+  R mean = 0, rstd = 0;
+  if (row < p.rows) {
     mean = means[row];
     rstd = rstds[row];
   }
-  uint32_t turn = 0;
+  uint32_t turn = 0, stage = 0;
   for (; row < p.rows; row += step, turn ^= 1u) {
-    Pack<T> r[kPacks];
-    if constexpr (AHEAD) {
-      if (row + step < p.rows) {
-        lay.template load<true>(x_rows + (row + step) * p.ldx, next_x);
-        lay.template load<true>(dy_rows + (row + step) * p.lddy, next_dy);
-        next_mean = means[row + step];
-        next_rstd = rstds[row + step];
-      }
-    } else {
-      lay.template load<true>(x_rows + row * p.ldx, x);
-      lay.template load<true>(dy_rows + row * p.lddy, dy);
-      mean = means[row];
-      rstd = rstds[row];
+    fetch(row + (DEPTH - 1) * step, stage == 0 ? DEPTH - 1 : stage - 1);
+    R next_mean = 0, next_rstd = 0;
+    if (row + step < p.rows) {
+      next_mean = means[row + step];
+      next_rstd = rstds[row + step];
     }
-    if (p.residual && p.dx)
-      lay.template load<true>(static_cast<const T *>(p.residual) + row * p.ldr, r);
+    asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
     Two<R> a2 = twice(R(0)), b2 = a2;  // elements outside the row: dy = 0
 #pragma unroll
     for (int i = 0; i < kPacks; ++i) {
       Two<R> fx[kN / 2], fd[kN / 2], fg[kN / 2];
-      widen_pack(x[i], fx);
-      widen_pack(dy[i], fd);
+      widen_pack(place(stage, 0, i), fx);
+      widen_pack(place(stage, 1, i), fd);
       widen_pack(g[i], fg);
 #pragma unroll
       for (int j = 0; j < kN / 2; ++j) {
@@ -611,18 +770,18 @@ __device__ __forceinline__ void norm_grad_rows(
       T *dx = static_cast<T *>(p.dx) + row * p.lddx;
 #pragma unroll
       for (int i = 0; i < kPacks; ++i) {
-        if (!lay.some(i))
+        if (LAYOUT != kAny && !lay.some(i))
           continue;
         Two<R> fx[kN / 2], fd[kN / 2], fg[kN / 2];
-        widen_pack(x[i], fx);
-        widen_pack(dy[i], fd);
+        widen_pack(place(stage, 0, i), fx);
+        widen_pack(place(stage, 1, i), fd);
         widen_pack(g[i], fg);
 #pragma unroll
         for (int j = 0; j < kN / 2; ++j)
           fx[j] = fma(mul(fd[j], fg[j]), twice(rstd),
                       fma(add(fx[j], twice(-mean)), twice(cb), twice(ca)));
-        if (p.residual) {
-          widen_pack(r[i], fd);
+        if (res_rows) {
+          widen_pack(place(stage, 2, i), fd);
 #pragma unroll
           for (int j = 0; j < kN / 2; ++j)
             fx[j] = add(fx[j], fd[j]);
@@ -632,20 +791,15 @@ __device__ __forceinline__ void norm_grad_rows(
         lay.store(dx, i, out);
       }
     }
-    if constexpr (AHEAD) {
-#pragma unroll
-      for (int i = 0; i < kPacks; ++i) {
-        x[i] = next_x[i];
-        dy[i] = next_dy[i];
-      }
-      mean = next_mean;
-      rstd = next_rstd;
-    }
+    mean = next_mean;
+    rstd = next_rstd;
+    stage = stage + 1 == DEPTH ? 0 : stage + 1;
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
   if (!p.partials)
     return;
   R *part = static_cast<R *>(p.partials) + (uint64_t)blockIdx.x * 2 * p.cols;
-  if (TH != 32) {
+  if (kRows == 1) {
 #pragma unroll
     for (int i = 0; i < kPacks; ++i)
 #pragma unroll
@@ -658,8 +812,10 @@ __device__ __forceinline__ void norm_grad_rows(
       }
     return;
   }
-  // The 8 warps' rows may differ in phase: their sums meet by column.
-  const uint32_t warp = threadIdx.x / 32;
+  // The block's rows may differ in phase: their sums meet by column, in the
+  // ring's place.
+  R(*joined)[TH * NE] = reinterpret_cast<R(*)[TH * NE]>(ring);
+  __syncthreads();
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
 #pragma unroll
@@ -668,14 +824,14 @@ __device__ __forceinline__ void norm_grad_rows(
       for (int j = 0; j < kN; ++j) {
         const uint32_t c = lay.column(i, j);
         if (c < p.cols)
-          joined[warp][c] =
+          joined[group][c] =
               half_of(which ? dbeta[(i * kN + j) / 2] : dgamma[(i * kN + j) / 2], j);
       }
     __syncthreads();
     for (uint32_t c = threadIdx.x; c < p.cols; c += 256) {
       R s = 0;
 #pragma unroll
-      for (int w = 0; w < 8; ++w)
+      for (uint32_t w = 0; w < kRows; ++w)
         s += joined[w][c];
       part[(uint64_t)which * p.cols + c] = s;
     }
@@ -873,19 +1029,19 @@ __device__ __forceinline__ void output_grad_join(
 
 }  // namespace
 
-// Kernels by threads per row, elements per thread and layout: w whole, h
-// shifted (16-bit types), s any (fewer shapes).  MINB blocks share an SM.
+// Kernels by threads per row, elements per thread and layout (w whole, h
+// shifted, s any); MINB blocks share an SM, DEPTH rows the gradient's ring.
 #define NORM(SUFFIX, T, TH, NE, MODE, LAYOUT, MINB)                            \
-  extern "C" __global__ void __launch_bounds__(TH == 32 ? 256 : TH, MINB)      \
+  extern "C" __global__ void __launch_bounds__(TH < 256 ? 256 : TH, MINB)      \
       hexir_layer_norm_##SUFFIX##_##MODE##TH##x##NE(                           \
           const hexir_layer_norm_args_t args) {                                \
     norm_rows<T, TH, NE, LAYOUT>(args);                                        \
   }
-#define NORM_GRAD(SUFFIX, T, TH, NE, MODE, LAYOUT, MINB, AHEAD)                \
-  extern "C" __global__ void __launch_bounds__(TH == 32 ? 256 : TH, MINB)      \
+#define NORM_GRAD(SUFFIX, T, TH, NE, MODE, LAYOUT, MINB, DEPTH)                \
+  extern "C" __global__ void __launch_bounds__(TH < 256 ? 256 : TH, MINB)      \
       hexir_layer_norm_grad_##SUFFIX##_##MODE##TH##x##NE(                      \
           const hexir_layer_norm_grad_args_t args) {                           \
-    norm_grad_rows<T, TH, NE, LAYOUT, AHEAD>(args);                            \
+    norm_grad_rows<T, TH, NE, LAYOUT, DEPTH>(args);                            \
   }
 
 #define NORMS(SUFFIX, T)                                                       \
@@ -912,73 +1068,98 @@ __device__ __forceinline__ void output_grad_join(
 #define NORMS_16(SUFFIX, T)                                                    \
   NORMS(SUFFIX, T)                                                             \
   NORM(SUFFIX, T, 32, 8, w, kWhole, 5)                                         \
+  NORM(SUFFIX, T, 32, 16, w, kWhole, 3)                                        \
+  NORM(SUFFIX, T, 32, 24, w, kWhole, 2)                                        \
   NORM(SUFFIX, T, 32, 32, w, kWhole, 2)                                        \
-  NORM(SUFFIX, T, 256, 8, w, kWhole, 5)                                        \
+  NORM(SUFFIX, T, 128, 16, w, kWhole, 4)                                       \
   NORM(SUFFIX, T, 256, 16, w, kWhole, 4)                                       \
+  NORM(SUFFIX, T, 256, 24, w, kWhole, 2)                                       \
   NORM(SUFFIX, T, 256, 32, w, kWhole, 2)                                       \
   NORM(SUFFIX, T, 512, 32, w, kWhole, 1)                                       \
   NORM(SUFFIX, T, 32, 8, h, kShifted, 5)                                       \
+  NORM(SUFFIX, T, 32, 16, h, kShifted, 3)                                      \
+  NORM(SUFFIX, T, 32, 24, h, kShifted, 2)                                      \
   NORM(SUFFIX, T, 32, 32, h, kShifted, 2)                                      \
-  NORM(SUFFIX, T, 256, 8, h, kShifted, 5)                                      \
+  NORM(SUFFIX, T, 128, 16, h, kShifted, 4)                                     \
   NORM(SUFFIX, T, 256, 16, h, kShifted, 4)                                     \
+  NORM(SUFFIX, T, 256, 24, h, kShifted, 2)                                     \
   NORM(SUFFIX, T, 256, 32, h, kShifted, 2)                                     \
   NORM(SUFFIX, T, 512, 32, h, kShifted, 1)                                     \
   NORM(SUFFIX, T, 32, 32, s, kAny, 2)                                          \
   NORM(SUFFIX, T, 256, 16, s, kAny, 3)                                         \
   NORM(SUFFIX, T, 512, 32, s, kAny, 1)                                         \
-  NORM_GRAD(SUFFIX, T, 32, 8, w, kWhole, 3, true)                              \
-  NORM_GRAD(SUFFIX, T, 32, 32, w, kWhole, 1, true)                             \
-  NORM_GRAD(SUFFIX, T, 256, 8, w, kWhole, 3, true)                             \
-  NORM_GRAD(SUFFIX, T, 256, 16, w, kWhole, 2, true)                            \
-  NORM_GRAD(SUFFIX, T, 512, 16, w, kWhole, 1, true)                            \
-  NORM_GRAD(SUFFIX, T, 1024, 16, w, kWhole, 1, false)                          \
-  NORM_GRAD(SUFFIX, T, 32, 8, h, kShifted, 3, true)                            \
-  NORM_GRAD(SUFFIX, T, 32, 32, h, kShifted, 1, true)                           \
-  NORM_GRAD(SUFFIX, T, 256, 8, h, kShifted, 3, true)                           \
-  NORM_GRAD(SUFFIX, T, 256, 16, h, kShifted, 2, true)                          \
-  NORM_GRAD(SUFFIX, T, 512, 16, h, kShifted, 1, true)                          \
-  NORM_GRAD(SUFFIX, T, 1024, 16, h, kShifted, 1, false)                        \
-  NORM_GRAD(SUFFIX, T, 32, 16, s, kAny, 1, true)                               \
-  NORM_GRAD(SUFFIX, T, 256, 16, s, kAny, 1, true)                              \
-  NORM_GRAD(SUFFIX, T, 1024, 16, s, kAny, 1, false)
+  NORM_GRAD(SUFFIX, T, 32, 8, w, kWhole, 2, 6)                                 \
+  NORM_GRAD(SUFFIX, T, 32, 16, w, kWhole, 2, 4)                                \
+  NORM_GRAD(SUFFIX, T, 64, 16, w, kWhole, 2, 4)                                \
+  NORM_GRAD(SUFFIX, T, 128, 16, w, kWhole, 2, 4)                               \
+  NORM_GRAD(SUFFIX, T, 256, 16, w, kWhole, 2, 4)                               \
+  NORM_GRAD(SUFFIX, T, 384, 16, w, kWhole, 1, 4)                               \
+  NORM_GRAD(SUFFIX, T, 512, 16, w, kWhole, 1, 3)                               \
+  NORM_GRAD(SUFFIX, T, 1024, 16, w, kWhole, 1, 2)                              \
+  NORM_GRAD(SUFFIX, T, 32, 8, h, kShifted, 2, 6)                               \
+  NORM_GRAD(SUFFIX, T, 32, 16, h, kShifted, 2, 4)                              \
+  NORM_GRAD(SUFFIX, T, 64, 16, h, kShifted, 2, 4)                              \
+  NORM_GRAD(SUFFIX, T, 128, 16, h, kShifted, 2, 4)                             \
+  NORM_GRAD(SUFFIX, T, 256, 16, h, kShifted, 2, 4)                             \
+  NORM_GRAD(SUFFIX, T, 384, 16, h, kShifted, 1, 4)                             \
+  NORM_GRAD(SUFFIX, T, 512, 16, h, kShifted, 1, 3)                             \
+  NORM_GRAD(SUFFIX, T, 1024, 16, h, kShifted, 1, 2)                            \
+  NORM_GRAD(SUFFIX, T, 32, 32, s, kAny, 1, 2)                                  \
+  NORM_GRAD(SUFFIX, T, 1024, 16, s, kAny, 1, 2)
 
 NORMS_16(bf16, __nv_bfloat16)
 NORMS_16(f16, __half)
 
 NORMS(f32, float)
 NORM(f32, float, 32, 8, w, kWhole, 5)
+NORM(f32, float, 32, 16, w, kWhole, 3)
 NORM(f32, float, 32, 32, w, kWhole, 2)
-NORM(f32, float, 256, 8, w, kWhole, 5)
-NORM(f32, float, 256, 16, w, kWhole, 4)
+NORM(f32, float, 128, 16, w, kWhole, 3)
+NORM(f32, float, 256, 16, w, kWhole, 3)
 NORM(f32, float, 512, 16, w, kWhole, 2)
 NORM(f32, float, 1024, 16, w, kWhole, 1)
-NORM(f32, float, 32, 32, s, kAny, 2)
-NORM(f32, float, 256, 16, s, kAny, 2)
+NORM(f32, float, 32, 8, s, kAny, 5)
+NORM(f32, float, 32, 16, s, kAny, 3)
+NORM(f32, float, 128, 8, s, kAny, 4)
+NORM(f32, float, 320, 8, s, kAny, 3)
+NORM(f32, float, 512, 8, s, kAny, 2)
+NORM(f32, float, 512, 16, s, kAny, 1)
 NORM(f32, float, 1024, 16, s, kAny, 1)
-NORM_GRAD(f32, float, 32, 8, w, kWhole, 2, true)
-NORM_GRAD(f32, float, 32, 16, w, kWhole, 1, true)
-NORM_GRAD(f32, float, 256, 8, w, kWhole, 3, true)
-NORM_GRAD(f32, float, 256, 16, w, kWhole, 1, true)
-NORM_GRAD(f32, float, 512, 16, w, kWhole, 1, false)
-NORM_GRAD(f32, float, 32, 16, s, kAny, 1, true)
-NORM_GRAD(f32, float, 256, 16, s, kAny, 1, true)
-NORM_GRAD(f32, float, 512, 16, s, kAny, 1, false)
+NORM_GRAD(f32, float, 32, 8, w, kWhole, 2, 4)
+NORM_GRAD(f32, float, 64, 8, w, kWhole, 2, 4)
+NORM_GRAD(f32, float, 128, 8, w, kWhole, 2, 4)
+NORM_GRAD(f32, float, 256, 8, w, kWhole, 2, 4)
+NORM_GRAD(f32, float, 512, 8, w, kWhole, 1, 3)
+NORM_GRAD(f32, float, 512, 16, w, kWhole, 1, 2)
+NORM_GRAD(f32, float, 64, 8, s, kAny, 2, 4)
+NORM_GRAD(f32, float, 128, 8, s, kAny, 2, 4)
+NORM_GRAD(f32, float, 320, 8, s, kAny, 1, 4)
+NORM_GRAD(f32, float, 512, 8, s, kAny, 1, 3)
+NORM_GRAD(f32, float, 512, 16, s, kAny, 1, 2)
 
 NORMS(f64, double)
 NORM(f64, double, 32, 8, w, kWhole, 3)
-NORM(f64, double, 32, 16, w, kWhole, 2)
+NORM(f64, double, 64, 8, w, kWhole, 3)
+NORM(f64, double, 128, 8, w, kWhole, 3)
 NORM(f64, double, 256, 8, w, kWhole, 3)
 NORM(f64, double, 512, 8, w, kWhole, 1)
 NORM(f64, double, 512, 16, w, kWhole, 1)
-NORM(f64, double, 32, 16, s, kAny, 2)
+NORM(f64, double, 32, 8, s, kAny, 3)
+NORM(f64, double, 64, 8, s, kAny, 3)
+NORM(f64, double, 192, 8, s, kAny, 3)
 NORM(f64, double, 256, 8, s, kAny, 3)
+NORM(f64, double, 512, 8, s, kAny, 1)
 NORM(f64, double, 512, 16, s, kAny, 1)
-NORM_GRAD(f64, double, 32, 8, w, kWhole, 1, true)
-NORM_GRAD(f64, double, 256, 8, w, kWhole, 1, true)
-NORM_GRAD(f64, double, 512, 8, w, kWhole, 1, false)
-NORM_GRAD(f64, double, 32, 8, s, kAny, 1, true)
-NORM_GRAD(f64, double, 256, 8, s, kAny, 1, true)
-NORM_GRAD(f64, double, 512, 8, s, kAny, 1, false)
+NORM_GRAD(f64, double, 32, 8, w, kWhole, 2, 3)
+NORM_GRAD(f64, double, 64, 8, w, kWhole, 2, 3)
+NORM_GRAD(f64, double, 128, 8, w, kWhole, 2, 3)
+NORM_GRAD(f64, double, 256, 8, w, kWhole, 2, 3)
+NORM_GRAD(f64, double, 512, 8, w, kWhole, 1, 2)
+NORM_GRAD(f64, double, 32, 8, s, kAny, 1, 3)
+NORM_GRAD(f64, double, 64, 8, s, kAny, 2, 3)
+NORM_GRAD(f64, double, 192, 8, s, kAny, 2, 3)
+NORM_GRAD(f64, double, 256, 8, s, kAny, 2, 3)
+NORM_GRAD(f64, double, 512, 8, s, kAny, 1, 2)
 
 #define OUTPUT_GRAD(SUFFIX, T)                                                 \
   extern "C" __global__ void __launch_bounds__(256)                            \

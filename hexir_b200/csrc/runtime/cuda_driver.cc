@@ -83,6 +83,7 @@ void load() {
             bind(lib, d.ModuleGetFunction, "cuModuleGetFunction", e) &&
             bind(lib, d.ModuleGetGlobal, "cuModuleGetGlobal_v2", e) &&
             bind(lib, d.FuncSetAttribute, "cuFuncSetAttribute", e) &&
+            bind(lib, d.FuncGetAttribute, "cuFuncGetAttribute", e) &&
             bind(lib, d.LaunchKernel, "cuLaunchKernel", e) &&
             bind(lib, d.EventCreate, "cuEventCreate", e) &&
             bind(lib, d.EventDestroy, "cuEventDestroy_v2", e) &&

@@ -69,6 +69,7 @@ struct Driver {
   CUresult (*ModuleGetGlobal)(CUdeviceptr *, size_t *, CUmodule,
                               const char *) = nullptr;
   CUresult (*FuncSetAttribute)(CUfunction, CUfunction_attribute, int) = nullptr;
+  CUresult (*FuncGetAttribute)(int *, CUfunction_attribute, CUfunction) = nullptr;
   CUresult (*LaunchKernel)(CUfunction, unsigned, unsigned, unsigned, unsigned,
                            unsigned, unsigned, unsigned, CUstream, void **,
                            void **) = nullptr;

@@ -26,83 +26,107 @@ namespace {
 // row cuts at the same place (16-bit types); or anyhow.
 enum Layout { kWhole, kShifted, kAny };
 
-// Launch shapes of the norm kernels: the shape's name in layer_norm.cu, threads per row (32: a warp, 8
-// rows per block), elements per thread, and the persistent blocks per SM its
-// registers allow.  A row runs the first shape of its kind that holds it.
+// The norm kernels: the name's end in layer_norm.cu, threads per row (blocks
+// have 256 at least, several rows where a row has less), elements per thread,
+// layout, and the gradient's rows of the ring.  A row runs the first kernel of its layout that holds it.
 struct NormShape {
   const char *name;
-  uint32_t threads, elements, per_sm;
+  uint32_t threads, elements;
   Layout layout;
-  uint32_t block() const { return threads == 32 ? 256 : threads; }
-  uint32_t rows() const { return threads == 32 ? 8 : 1; }
-  // Shared memory of the forward's shifted gamma and beta (16-bit types).
-  uint32_t copies() const { return rows() * threads * elements * 2 * 2; }
+  uint32_t depth;
+  uint32_t rows() const { return threads < 256 ? 256 / threads : 1; }
+  uint32_t block() const { return rows() * threads; }
 };
-constexpr int kMaxShapes = 15;
+constexpr int kMaxShapes = 21;
 // By the kind of type: 16-bit, f32, f64.
 constexpr NormShape kNorm[3][kMaxShapes] = {
-    {{"w32x8", 32, 8, 5, kWhole},
-     {"w32x32", 32, 32, 2, kWhole},
-     {"w256x8", 256, 8, 5, kWhole},
-     {"w256x16", 256, 16, 4, kWhole},
-     {"w256x32", 256, 32, 2, kWhole},
-     {"w512x32", 512, 32, 1, kWhole},
-     {"h32x8", 32, 8, 5, kShifted},
-     {"h32x32", 32, 32, 2, kShifted},
-     {"h256x8", 256, 8, 5, kShifted},
-     {"h256x16", 256, 16, 4, kShifted},
-     {"h256x32", 256, 32, 2, kShifted},
-     {"h512x32", 512, 32, 1, kShifted},
-     {"s32x32", 32, 32, 2, kAny},
-     {"s256x16", 256, 16, 3, kAny},
-     {"s512x32", 512, 32, 1, kAny}},
-    {{"w32x8", 32, 8, 5, kWhole},
-     {"w32x32", 32, 32, 2, kWhole},
-     {"w256x8", 256, 8, 5, kWhole},
-     {"w256x16", 256, 16, 4, kWhole},
-     {"w512x16", 512, 16, 2, kWhole},
-     {"w1024x16", 1024, 16, 1, kWhole},
-     {"s32x32", 32, 32, 2, kAny},
-     {"s256x16", 256, 16, 2, kAny},
-     {"s1024x16", 1024, 16, 1, kAny}},
-    {{"w32x8", 32, 8, 3, kWhole},
-     {"w32x16", 32, 16, 2, kWhole},
-     {"w256x8", 256, 8, 3, kWhole},
-     {"w512x8", 512, 8, 1, kWhole},
-     {"w512x16", 512, 16, 1, kWhole},
-     {"s32x16", 32, 16, 2, kAny},
-     {"s256x8", 256, 8, 3, kAny},
-     {"s512x16", 512, 16, 1, kAny}}};
+    {{"w32x8", 32, 8, kWhole, 0},
+     {"w32x16", 32, 16, kWhole, 0},
+     {"w32x24", 32, 24, kWhole, 0},
+     {"w32x32", 32, 32, kWhole, 0},
+     {"w128x16", 128, 16, kWhole, 0},
+     {"w256x16", 256, 16, kWhole, 0},
+     {"w256x24", 256, 24, kWhole, 0},
+     {"w256x32", 256, 32, kWhole, 0},
+     {"w512x32", 512, 32, kWhole, 0},
+     {"h32x8", 32, 8, kShifted, 0},
+     {"h32x16", 32, 16, kShifted, 0},
+     {"h32x24", 32, 24, kShifted, 0},
+     {"h32x32", 32, 32, kShifted, 0},
+     {"h128x16", 128, 16, kShifted, 0},
+     {"h256x16", 256, 16, kShifted, 0},
+     {"h256x24", 256, 24, kShifted, 0},
+     {"h256x32", 256, 32, kShifted, 0},
+     {"h512x32", 512, 32, kShifted, 0},
+     {"s32x32", 32, 32, kAny, 0},
+     {"s256x16", 256, 16, kAny, 0},
+     {"s512x32", 512, 32, kAny, 0}},
+    {{"w32x8", 32, 8, kWhole, 0},
+     {"w32x16", 32, 16, kWhole, 0},
+     {"w32x32", 32, 32, kWhole, 0},
+     {"w128x16", 128, 16, kWhole, 0},
+     {"w256x16", 256, 16, kWhole, 0},
+     {"w512x16", 512, 16, kWhole, 0},
+     {"w1024x16", 1024, 16, kWhole, 0},
+     {"s32x8", 32, 8, kAny, 0},
+     {"s32x16", 32, 16, kAny, 0},
+     {"s128x8", 128, 8, kAny, 0},
+     {"s320x8", 320, 8, kAny, 0},
+     {"s512x8", 512, 8, kAny, 0},
+     {"s512x16", 512, 16, kAny, 0},
+     {"s1024x16", 1024, 16, kAny, 0}},
+    {{"w32x8", 32, 8, kWhole, 0},
+     {"w64x8", 64, 8, kWhole, 0},
+     {"w128x8", 128, 8, kWhole, 0},
+     {"w256x8", 256, 8, kWhole, 0},
+     {"w512x8", 512, 8, kWhole, 0},
+     {"w512x16", 512, 16, kWhole, 0},
+     {"s32x8", 32, 8, kAny, 0},
+     {"s64x8", 64, 8, kAny, 0},
+     {"s192x8", 192, 8, kAny, 0},
+     {"s256x8", 256, 8, kAny, 0},
+     {"s512x8", 512, 8, kAny, 0},
+     {"s512x16", 512, 16, kAny, 0}}};
 constexpr NormShape kNormGrad[3][kMaxShapes] = {
-    {{"w32x8", 32, 8, 3, kWhole},
-     {"w32x32", 32, 32, 1, kWhole},
-     {"w256x8", 256, 8, 3, kWhole},
-     {"w256x16", 256, 16, 2, kWhole},
-     {"w512x16", 512, 16, 1, kWhole},
-     {"w1024x16", 1024, 16, 1, kWhole},
-     {"h32x8", 32, 8, 3, kShifted},
-     {"h32x32", 32, 32, 1, kShifted},
-     {"h256x8", 256, 8, 3, kShifted},
-     {"h256x16", 256, 16, 2, kShifted},
-     {"h512x16", 512, 16, 1, kShifted},
-     {"h1024x16", 1024, 16, 1, kShifted},
-     {"s32x16", 32, 16, 1, kAny},
-     {"s256x16", 256, 16, 1, kAny},
-     {"s1024x16", 1024, 16, 1, kAny}},
-    {{"w32x8", 32, 8, 2, kWhole},
-     {"w32x16", 32, 16, 1, kWhole},
-     {"w256x8", 256, 8, 3, kWhole},
-     {"w256x16", 256, 16, 1, kWhole},
-     {"w512x16", 512, 16, 1, kWhole},
-     {"s32x16", 32, 16, 1, kAny},
-     {"s256x16", 256, 16, 1, kAny},
-     {"s512x16", 512, 16, 1, kAny}},
-    {{"w32x8", 32, 8, 1, kWhole},
-     {"w256x8", 256, 8, 1, kWhole},
-     {"w512x8", 512, 8, 1, kWhole},
-     {"s32x8", 32, 8, 1, kAny},
-     {"s256x8", 256, 8, 1, kAny},
-     {"s512x8", 512, 8, 1, kAny}}};
+    {{"w32x8", 32, 8, kWhole, 6},
+     {"w32x16", 32, 16, kWhole, 4},
+     {"w64x16", 64, 16, kWhole, 4},
+     {"w128x16", 128, 16, kWhole, 4},
+     {"w256x16", 256, 16, kWhole, 4},
+     {"w384x16", 384, 16, kWhole, 4},
+     {"w512x16", 512, 16, kWhole, 3},
+     {"w1024x16", 1024, 16, kWhole, 2},
+     {"h32x8", 32, 8, kShifted, 6},
+     {"h32x16", 32, 16, kShifted, 4},
+     {"h64x16", 64, 16, kShifted, 4},
+     {"h128x16", 128, 16, kShifted, 4},
+     {"h256x16", 256, 16, kShifted, 4},
+     {"h384x16", 384, 16, kShifted, 4},
+     {"h512x16", 512, 16, kShifted, 3},
+     {"h1024x16", 1024, 16, kShifted, 2},
+     {"s32x32", 32, 32, kAny, 2},
+     {"s1024x16", 1024, 16, kAny, 2}},
+    {{"w32x8", 32, 8, kWhole, 4},
+     {"w64x8", 64, 8, kWhole, 4},
+     {"w128x8", 128, 8, kWhole, 4},
+     {"w256x8", 256, 8, kWhole, 4},
+     {"w512x8", 512, 8, kWhole, 3},
+     {"w512x16", 512, 16, kWhole, 2},
+     {"s64x8", 64, 8, kAny, 4},
+     {"s128x8", 128, 8, kAny, 4},
+     {"s320x8", 320, 8, kAny, 4},
+     {"s512x8", 512, 8, kAny, 3},
+     {"s512x16", 512, 16, kAny, 2}},
+    {{"w32x8", 32, 8, kWhole, 3},
+     {"w64x8", 64, 8, kWhole, 3},
+     {"w128x8", 128, 8, kWhole, 3},
+     {"w256x8", 256, 8, kWhole, 3},
+     {"w512x8", 512, 8, kWhole, 2},
+     {"s32x8", 32, 8, kAny, 3},
+     {"s64x8", 64, 8, kAny, 3},
+     {"s192x8", 192, 8, kAny, 3},
+     {"s256x8", 256, 8, kAny, 3},
+     {"s512x8", 512, 8, kAny, 2}}};
 
 int kind_of(uint32_t dtype) {
   return dtype == HEXIR_DTYPE_F64 ? 2 : (dtype == HEXIR_DTYPE_F32 ? 1 : 0);
@@ -119,29 +143,39 @@ Layout norm_layout(uint32_t size, uint32_t cols, bool parameters16,
       continue;
     whole = whole && phase(t.first) == 0 && t.second * size % 16 == 0;
     same = same && phase(t.first) == phase(first.first) &&
-           t.second % 8 == first.second % 8;
+           t.second * size % 16 == first.second * size % 16;
   }
   return whole ? kWhole : (same ? kShifted : kAny);
 }
 
-// -1: a longer row than any shape holds.
-int norm_shape(const NormShape (&shapes)[kMaxShapes], uint32_t cols, Layout layout) {
-  const uint64_t need = cols + (layout == kShifted ? 7ull : 0ull);
+// -1: a longer row than any kernel holds.
+int norm_shape(const NormShape (&shapes)[kMaxShapes], uint32_t cols, uint32_t size,
+               Layout layout) {
+  // A shifted row may begin and end inside a pack.
+  const uint64_t need = cols + (layout == kShifted ? 16ull / size - 1 : 0ull);
   for (int s = 0; s < kMaxShapes && shapes[s].name; ++s)
-    if (shapes[s].layout == layout &&
-        need <= shapes[s].threads * shapes[s].elements)
+    if (shapes[s].layout == layout && need <= shapes[s].threads * shapes[s].elements)
       return s;
   return -1;
 }
 
 // Persistent blocks; those of a shifted layout stay a multiple of 8 rows
-// apart, so that all rows of a block (of a warp) are cut at the same place.
+// apart, so that all rows of a thread are cut at the same place.
 uint64_t norm_blocks(const NormShape &shape, Layout layout, uint64_t rows,
                      uint64_t resident) {
   const uint64_t blocks = (rows + shape.rows() - 1) / shape.rows();
   if (blocks <= resident)
     return blocks;
   return layout == kShifted ? std::max<uint64_t>(8, resident / 8 * 8) : resident;
+}
+
+// Blocks of a kernel that fit an SM, by its registers and shared memory.
+uint32_t blocks_per_sm(uint32_t registers, uint32_t threads, uint32_t smem) {
+  const uint32_t per_warp = (registers + 7) / 8 * 8 * 32;
+  const uint32_t warps = 65536u / std::max(per_warp, 1u) / 4 * 4;
+  uint32_t n = std::min(2048u / threads, warps / ((threads + 31) / 32));
+  n = std::min(n, 227u * 1024u / (smem + 9216u));
+  return std::max(n, 1u);
 }
 
 const char *const kDtypeName[4] = {"f64", "f32", "bf16", "f16"};
@@ -155,8 +189,12 @@ struct LayersLib {
   // By HEXIR_PRODUCT_*; skinny is the forward's only.
   CUfunction pair[3] = {}, single[3] = {}, guarded[3] = {}, skinny = nullptr;
   // By dtype.
-  CUfunction norm[4][kMaxShapes] = {}, norm_wide[4] = {};
-  CUfunction norm_grad[4][kMaxShapes] = {}, norm_grad_wide[4] = {},
+  struct Sized {
+    CUfunction fn = nullptr;
+    int registers = 0;
+  };
+  Sized norm[4][kMaxShapes] = {}, norm_grad[4][kMaxShapes] = {};
+  CUfunction norm_wide[4] = {}, norm_grad_wide[4] = {},
              norm_grad_columns[4] = {}, norm_grad_join[4] = {};
   CUfunction output_grad[4] = {}, output_grad_join[4] = {};
 };
@@ -166,7 +204,9 @@ CUdeviceptr layers_error_word(const LayersLib *lib) { return lib->error_word; }
 namespace {
 
 // The most dynamic shared memory any of the product kernels is launched with.
-constexpr uint32_t kSmemLimit = 227u * 1024u - 1024u;
+constexpr uint32_t kSmemLimit = 227u * 1024u - 2048u;
+// The same of the norm kernels, beside up to 8 KiB of their own.
+constexpr uint32_t kNormSmemLimit = 218u * 1024u;
 
 LayersLib *layers_library(DeviceState *dev, std::string *error) {
   std::lock_guard<std::mutex> lock(dev->mu);
@@ -202,9 +242,9 @@ LayersLib *layers_library(DeviceState *dev, std::string *error) {
     const int kind = kind_of(t);
     for (int s = 0; s < kMaxShapes; ++s) {
       if (kNorm[kind][s].name)
-        get(&lib->norm[t][s], norm + "_" + kNorm[kind][s].name);
+        get(&lib->norm[t][s].fn, norm + "_" + kNorm[kind][s].name);
       if (kNormGrad[kind][s].name)
-        get(&lib->norm_grad[t][s], grad + "_" + kNormGrad[kind][s].name);
+        get(&lib->norm_grad[t][s].fn, grad + "_" + kNormGrad[kind][s].name);
     }
     get(&lib->norm_wide[t], norm + "_wide");
     get(&lib->norm_grad_wide[t], grad + "_wide");
@@ -233,14 +273,17 @@ LayersLib *layers_library(DeviceState *dev, std::string *error) {
     r = d.FuncSetAttribute(lib->skinny,
                            CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES,
                            kSmemLimit);
-  // The longest rows' copies pass the 48 KiB that need no attribute.
   for (int t = 0; t < 4; ++t)
-    for (int s = 0; s < kMaxShapes && r == CUDA_SUCCESS; ++s)
-      if (kind_of(t) == 0 && kNorm[0][s].layout == kShifted &&
-          kNorm[0][s].copies() > 48u * 1024u)
-        r = d.FuncSetAttribute(lib->norm[t][s],
-                               CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES,
-                               static_cast<int>(kNorm[0][s].copies()));
+    for (int s = 0; s < kMaxShapes; ++s)
+      for (LayersLib::Sized *k : {&lib->norm[t][s], &lib->norm_grad[t][s]}) {
+        if (!k->fn || r != CUDA_SUCCESS)
+          continue;
+        r = d.FuncGetAttribute(&k->registers, CU_FUNC_ATTRIBUTE_NUM_REGS, k->fn);
+        if (r == CUDA_SUCCESS)
+          r = d.FuncSetAttribute(k->fn,
+                                 CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES,
+                                 kNormSmemLimit);
+      }
   if (r != CUDA_SUCCESS) {
     d.ModuleUnload(lib->module);
     fail(error, cuda_message("layer kernels setup", r));
@@ -874,20 +917,24 @@ extern "C" hexir_status_t hexir_cuda_layer_norm(int ordinal,
   ContextGuard guard(call.dev->context);
   CUstream s = static_cast<CUstream>(stream);
   const int kind = kind_of(c.dtype);
-  const int at = norm_shape(kNorm[kind], c.cols, layout);
+  const int at = norm_shape(kNorm[kind], c.cols, size, layout);
   if (at < 0)
     return call.finish(launch(call.lib->norm_wide[c.dtype],
                               static_cast<unsigned>(std::min<uint64_t>(c.rows, 1u << 24)),
                               1, 512, 0, s, params, "launch hexir_layer_norm wide",
                               &call.error));
   const NormShape &shape = kNorm[kind][at];
+  const LayersLib::Sized &kernel = call.lib->norm[c.dtype][at];
+  // Shifted rows: gamma and beta as the rows lie.
+  const uint32_t copies =
+      layout == kShifted ? 2 * shape.block() * shape.elements * size : 0;
   const uint64_t resident =
-      static_cast<uint64_t>(std::max(call.dev->sm_count, 1)) * shape.per_sm;
-  const unsigned blocks =
-      static_cast<unsigned>(norm_blocks(shape, layout, c.rows, resident));
-  return call.finish(launch(call.lib->norm[c.dtype][at], blocks, 1, shape.block(),
-                            layout == kShifted ? shape.copies() : 0, s, params,
-                            "launch hexir_layer_norm", &call.error));
+      static_cast<uint64_t>(std::max(call.dev->sm_count, 1)) *
+      blocks_per_sm(kernel.registers, shape.block(), copies);
+  return call.finish(
+      launch(kernel.fn,
+             static_cast<unsigned>(norm_blocks(shape, layout, c.rows, resident)), 1,
+             shape.block(), copies, s, params, "launch hexir_layer_norm", &call.error));
 }
 
 extern "C" hexir_status_t hexir_cuda_layer_norm_grad(
@@ -952,16 +999,23 @@ extern "C" hexir_status_t hexir_cuda_layer_norm_grad(
   CUstream s = static_cast<CUstream>(stream);
   const uint64_t sms = static_cast<uint64_t>(std::max(call.dev->sm_count, 1));
   const int kind = kind_of(c.dtype);
-  const int at = norm_shape(kNormGrad[kind], c.cols, layout);
+  const int at = norm_shape(kNormGrad[kind], c.cols, size, layout);
   hexir_status_t st = HEXIR_OK;
   void *params[] = {&args};
   if (c.rows && at >= 0) {
     const NormShape &shape = kNormGrad[kind][at];
-    args.parts = static_cast<uint32_t>(
-        norm_blocks(shape, layout, c.rows,
-                    std::min<uint64_t>(sms * shape.per_sm, kSumsPerColumn / 2)));
-    st = launch(call.lib->norm_grad[c.dtype][at], args.parts, 1, shape.block(), 0, s,
-                params, "launch hexir_layer_norm_grad", &call.error);
+    const LayersLib::Sized &kernel = call.lib->norm_grad[c.dtype][at];
+    // The ring of rows; then the column sums of a block's rows.
+    const uint32_t row = shape.block() * shape.elements;
+    const uint32_t ring =
+        std::max<uint32_t>(shape.depth * (c.residual && c.dx ? 3 : 2) * row * size,
+                           shape.rows() > 1 ? row * real : 0);
+    const uint64_t resident = std::min<uint64_t>(
+        sms * blocks_per_sm(kernel.registers, shape.block(), ring), kSumsPerColumn / 2);
+    args.parts =
+        static_cast<uint32_t>(norm_blocks(shape, layout, c.rows, resident));
+    st = launch(kernel.fn, args.parts, 1, shape.block(), ring, s, params,
+                "launch hexir_layer_norm_grad", &call.error);
   } else if (c.rows) {
     // The column sums first: dx may be dy.
     if (sums) {
