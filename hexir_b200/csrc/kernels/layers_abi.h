@@ -23,15 +23,22 @@ extern "C" {
 /* One stage holds 64 of the summed index (128 bytes, the swizzle's span). */
 #define HEXIR_PRODUCT_BK 64
 #define HEXIR_PRODUCT_BM 128 /* rows per CTA: the lanes of TMEM */
-/* CTA pair: 6 stages of A 16 KiB + B 16 KiB (each CTA holds half of the 256
+/* Slots of 1 KiB (32 rows x 16 columns) an epilogue warp fetches ahead into,
+ * and one more for stores. */
+#define HEXIR_EPILOGUE_SLOTS 6
+#define HEXIR_EPILOGUE_BYTES(WARPS) ((WARPS) * (HEXIR_EPILOGUE_SLOTS + 1) * 1024)
+/* CTA pair: 5 stages of A 16 KiB + B 16 KiB (each CTA holds half of the 256
  * columns), 4 warps of loads and MMA, 8 of epilogue. */
-#define HEXIR_PAIR_STAGES 6
+#define HEXIR_PAIR_STAGES 5
 #define HEXIR_PAIR_STAGE_BYTES 32768
 #define HEXIR_PAIR_THREADS 384
-#define HEXIR_PAIR_SMEM_BYTES (HEXIR_PAIR_STAGES * HEXIR_PAIR_STAGE_BYTES + 1024 + 512)
-/* Single CTAs: a load warp, an MMA warp and 4 epilogue (or guarded load)
+#define HEXIR_PAIR_SMEM_BYTES                           \
+  (HEXIR_PAIR_STAGES * HEXIR_PAIR_STAGE_BYTES + 1024 + \
+   HEXIR_EPILOGUE_BYTES(8))
+/* Single CTAs: a load warp, an MMA warp and 8 epilogue (or guarded load)
  * warps. */
-#define HEXIR_SINGLE_THREADS 192
+#define HEXIR_SINGLE_EPILOGUE_WARPS 8
+#define HEXIR_SINGLE_THREADS (64 + HEXIR_SINGLE_EPILOGUE_WARPS * 32)
 #define HEXIR_SINGLE_MAX_STAGES 12
 
 typedef struct {
@@ -53,6 +60,8 @@ typedef struct {
   uint32_t split, k_tiles_per_split;
   uint32_t stages;        /* single: pipeline stages */
   uint32_t tmem_cols;     /* single: TMEM columns (a power of two >= 32) */
+  uint32_t ring_bytes;    /* single: the stages, or the sums of a split tile */
+  uint32_t tma_operands;  /* guarded: bit 0 a, bit 1 b come by TMA */
   uint64_t timeout_ns;
 } hexir_product_args_t;
 

@@ -11,7 +11,13 @@
 // issues tcgen05.mma, sums stay f32 in TMEM, and the epilogue warps read them
 // from there and write the finished rows.
 //
-// Every wait is bounded (common.cuh): a wait that runs out sets the error
+// The load and MMA warps run their loops converged and one lane issues: what
+// the instructions take is then the same for the warp as far as the compiler
+// can tell and goes to them without a detour.  Issued by one thread of its own,
+// with a wait of ~100 cycles before each stage, the MMAs of a stage took 660
+// cycles instead of 512.
+//
+// Every wait is bounded (tcgen05.cuh): a wait that runs out sets the error
 // word, its role stops, and the block still frees its TMEM and ends.
 
 #include <cuda_bf16.h>
@@ -62,93 +68,276 @@ __device__ __forceinline__ void unpack2(uint32_t w, float &lo, float &hi,
   }
 }
 
-// 16 consecutive elements at p, of which the first `left` are the row's.
-__device__ __forceinline__ void load16(const uint16_t *p, uint32_t left,
-                                       bool vec, bool is_f16, float (&v)[16]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (vec && left >= 8u * h + 8u) {
-      const uint4 w = *reinterpret_cast<const uint4 *>(p + 8 * h);
-      unpack2(w.x, v[8 * h], v[8 * h + 1], is_f16);
-      unpack2(w.y, v[8 * h + 2], v[8 * h + 3], is_f16);
-      unpack2(w.z, v[8 * h + 4], v[8 * h + 5], is_f16);
-      unpack2(w.w, v[8 * h + 6], v[8 * h + 7], is_f16);
-    } else {
-#pragma unroll
-      for (int i = 8 * h; i < 8 * h + 8; ++i)
-        v[i] = static_cast<uint32_t>(i) < left ? from_bits(p[i], is_f16) : 0.0f;
-    }
-  }
+// 16 bytes as 8 f32 and back.
+__device__ __forceinline__ void unpack8(const uint4 &w, bool is_f16, float *v) {
+  unpack2(w.x, v[0], v[1], is_f16);
+  unpack2(w.y, v[2], v[3], is_f16);
+  unpack2(w.z, v[4], v[5], is_f16);
+  unpack2(w.w, v[6], v[7], is_f16);
+}
+__device__ __forceinline__ uint4 pack8(const float *v, bool is_f16) {
+  return make_uint4(pack2(v[0], v[1], is_f16), pack2(v[2], v[3], is_f16),
+                    pack2(v[4], v[5], is_f16), pack2(v[6], v[7], is_f16));
 }
 
-__device__ __forceinline__ void store16(uint16_t *p, uint32_t left, bool vec,
-                                        bool is_f16, const float (&v)[16]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (vec && left >= 8u * h + 8u) {
-      uint4 w;
-      w.x = pack2(v[8 * h], v[8 * h + 1], is_f16);
-      w.y = pack2(v[8 * h + 2], v[8 * h + 3], is_f16);
-      w.z = pack2(v[8 * h + 4], v[8 * h + 5], is_f16);
-      w.w = pack2(v[8 * h + 6], v[8 * h + 7], is_f16);
-      *reinterpret_cast<uint4 *>(p + 8 * h) = w;
-    } else {
-#pragma unroll
-      for (int i = 8 * h; i < 8 * h + 8; ++i)
-        if (static_cast<uint32_t>(i) < left)
-          p[i] = to_bits(v[i], is_f16);
-    }
-  }
+// -------------------------------------------------------------- epilogue
+//
+// An epilogue warp finishes 32 rows x 16 columns at a time: a lane has one
+// row's 16 sums from TMEM, adds the bias, applies the activation (or the slope
+// at the stored preactivations), adds the residual and stores.  What it reads
+// besides (residual, preactivations) it fetches several such blocks ahead, into
+// slots of its own in shared memory, while the main loop still runs: read when
+// needed, each block waited for memory, which made the epilogue of a 256 x 256
+// tile 26 k cycles long.
+//
+// Rows on 16-byte boundaries (p.vec) are fetched and stored a lane's row at a
+// time, 16 bytes an access; any others by the whole warp, two rows of 16
+// elements an access, through the slots.
+
+constexpr uint32_t kSlotBytes = 1024u;  // 32 rows x 32 bytes
+
+// Where lane's row keeps its 16-byte half h: rows 4 apart swap halves, so that
+// 8 lanes' accesses fall into different banks.
+__device__ __forceinline__ uint32_t slot_at(uint32_t row, uint32_t h) {
+  return row * 32u + ((h ^ (row >> 2 & 1u)) << 4);
 }
 
-// The epilogue of 16 consecutive columns of one row, from the f32 sums to
-// the stored row; each stored value is rounded once.
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void copies_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Tensors an epilogue reads: the residual, then the preactivations.
 template <int FORM>
-__device__ __forceinline__ void finish16(const Args &p, float (&v)[16],
-                                         uint32_t row, uint32_t col) {
-  if (row >= p.rows || col >= p.cols)
+__device__ __forceinline__ uint32_t epilogue_tensors(const Args &p) {
+  return (FORM != HEXIR_PRODUCT_WEIGHT_GRAD && p.residual ? 1u : 0u) +
+         (FORM == HEXIR_PRODUCT_INPUT_GRAD && p.slope_at ? 1u : 0u);
+}
+
+// Blocks fetched ahead: 6 of one tensor or 3 of two.
+constexpr uint32_t kAhead1 = HEXIR_EPILOGUE_SLOTS, kAhead2 = HEXIR_EPILOGUE_SLOTS / 2;
+
+__device__ __forceinline__ void fetch_tensor(const Args &p, const void *base,
+                                             uint64_t ld, uint8_t *slot,
+                                             uint32_t row0, uint32_t col,
+                                             uint32_t lane) {
+  const uint16_t *src = static_cast<const uint16_t *>(base);
+  if (p.vec) {
+    const uint32_t row = row0 + lane;
+    if (row < p.rows) {
+      src += row * ld + col;
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t c = col + 8 * h;
+        if (c + 8 <= p.cols) {
+          copy_async16(smem_addr(slot + slot_at(lane, h)), src + 8 * h);
+        } else if (c < p.cols) {
+          uint16_t e[8];
+#pragma unroll
+          for (uint32_t i = 0; i < 8; ++i)
+            e[i] = src[8 * h + min(i, p.cols - c - 1)];
+          uint16_t *dst = reinterpret_cast<uint16_t *>(slot + slot_at(lane, h));
+#pragma unroll
+          for (uint32_t i = 0; i < 8; ++i)
+            dst[i] = e[i];
+        }
+      }
+    }
+  } else {
+    const uint32_t c = lane % 16;
+    const uint32_t col_in = min(col + c, p.cols - 1);
+    uint16_t e[16];
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i)
+      e[i] = src[min(row0 + 2 * i + lane / 16, p.rows - 1) * ld + col_in];
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i)
+      *reinterpret_cast<uint16_t *>(slot + slot_at(2 * i + lane / 16, c / 8) +
+                                    c % 8 * 2) = e[i];
+  }
+}
+
+// Fetch the block at (row0, col) into `slot` (a slot per tensor); blocks
+// outside the output fetch nothing.
+template <int FORM>
+__device__ __forceinline__ void fetch_block(const Args &p, uint8_t *slot,
+                                            uint32_t row0, uint32_t col,
+                                            uint32_t lane) {
+  if (row0 >= p.rows || col >= p.cols)
     return;
-  const uint32_t left = p.cols - col;
-  const bool vec = p.vec != 0, f16 = p.is_f16 != 0;
+  if (FORM != HEXIR_PRODUCT_WEIGHT_GRAD && p.residual) {
+    fetch_tensor(p, p.residual, p.ldr, slot, row0, col, lane);
+    slot += kSlotBytes;
+  }
+  if (FORM == HEXIR_PRODUCT_INPUT_GRAD && p.slope_at)
+    fetch_tensor(p, p.slope_at, p.lds, slot, row0, col, lane);
+}
+
+__device__ __forceinline__ void read_slot(const uint8_t *slot, uint32_t lane,
+                                          bool is_f16, float (&v)[16]) {
+#pragma unroll
+  for (uint32_t h = 0; h < 2; ++h)
+    unpack8(*reinterpret_cast<const uint4 *>(slot + slot_at(lane, h)), is_f16,
+            v + 8 * h);
+}
+
+// Store a block's rows; `out` is a slot for rows off 16 bytes.
+__device__ __forceinline__ void store_block(const Args &p, void *base, uint64_t ld,
+                                            uint8_t *out, uint32_t row0,
+                                            uint32_t col, uint32_t lane,
+                                            const float (&v)[16]) {
+  const bool f16 = p.is_f16 != 0;
+  uint16_t *dst = static_cast<uint16_t *>(base);
+  if (p.vec) {
+    const uint32_t row = row0 + lane;
+    if (row >= p.rows)
+      return;
+    dst += row * ld + col;
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+      const uint32_t c = col + 8 * h;
+      if (c + 8 <= p.cols) {
+        *reinterpret_cast<uint4 *>(dst + 8 * h) = pack8(v + 8 * h, f16);
+      } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+          if (c + i < p.cols)
+            dst[8 * h + i] = to_bits(v[8 * h + i], f16);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (uint32_t h = 0; h < 2; ++h)
+    *reinterpret_cast<uint4 *>(out + slot_at(lane, h)) = pack8(v + 8 * h, f16);
+  __syncwarp();
+  const uint32_t c = lane % 16;
+#pragma unroll
+  for (uint32_t i = 0; i < 16; ++i) {
+    const uint32_t r = 2 * i + lane / 16;
+    if (row0 + r < p.rows && col + c < p.cols)
+      dst[(row0 + r) * ld + col + c] = *reinterpret_cast<const uint16_t *>(
+          out + slot_at(r, c / 8) + c % 8 * 2);
+  }
+  __syncwarp();
+}
+
+// Finish the block at (row0, col), whose tensors are in `slot`; each stored
+// value is rounded once.  `bias` has the tile's bias in f32 from this block's
+// column on.
+template <int FORM>
+__device__ __forceinline__ void finish_block(const Args &p, float (&v)[16],
+                                             const float *bias,
+                                             const uint8_t *slot, uint8_t *out,
+                                             uint32_t row0, uint32_t col,
+                                             uint32_t lane) {
+  if (row0 >= p.rows || col >= p.cols)
+    return;
+  const bool f16 = p.is_f16 != 0;
   if (FORM == HEXIR_PRODUCT_FORWARD) {
     if (p.bias) {
-      float b[16];
-      load16(static_cast<const uint16_t *>(p.bias) + col, left, vec, f16, b);
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        v[i] += b[i];
+      for (int i = 0; i < 16; i += 4) {
+        const float4 b = *reinterpret_cast<const float4 *>(bias + i);
+        v[i] += b.x;
+        v[i + 1] += b.y;
+        v[i + 2] += b.z;
+        v[i + 3] += b.w;
+      }
     }
     if (p.preact_out)
-      store16(static_cast<uint16_t *>(p.preact_out) + row * p.ldp + col, left,
-              vec, f16, v);
+      store_block(p, p.preact_out, p.ldp, out, row0, col, lane, v);
     act_f32(p.activation, v);
   }
+  float r[16];
   if (FORM == HEXIR_PRODUCT_INPUT_GRAD && p.slope_at) {
-    float z[16];
-    load16(static_cast<const uint16_t *>(p.slope_at) + row * p.lds + col, left,
-           vec, f16, z);
-    slope_f32(p.activation, z, v);
+    read_slot(slot + (p.residual ? kSlotBytes : 0u), lane, f16, r);
+    slope_f32(p.activation, r, v);
   }
   if (FORM != HEXIR_PRODUCT_WEIGHT_GRAD && p.residual) {
-    float r[16];
-    load16(static_cast<const uint16_t *>(p.residual) + row * p.ldr + col, left,
-           vec, f16, r);
+    read_slot(slot, lane, f16, r);
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       v[i] += r[i];
   }
-  store16(static_cast<uint16_t *>(p.out) + row * p.ldo + col, left, vec, f16, v);
+  store_block(p, p.out, p.ldo, out, row0, col, lane, v);
 }
 
-// The same for one column of 16 consecutive rows (the skinny forward, whose
-// tile is the transposed product: lanes are columns, so a warp's store of one
-// row covers 32 consecutive columns).
+// The bias of columns col0 .. col0 + count into a warp's own shared memory;
+// zeros beyond the row.
+__device__ __forceinline__ void stage_bias(const Args &p, float *bias, uint32_t col0,
+                                           uint32_t count, uint32_t lane) {
+  __syncwarp();
+  for (uint32_t c = lane; c < count; c += 32)
+    bias[c] = col0 + c < p.cols
+                  ? from_bits(static_cast<const uint16_t *>(p.bias)[col0 + c],
+                              p.is_f16 != 0)
+                  : 0.0f;
+  __syncwarp();
+}
+
+// A warp's blocks in order, fetched ahead of their use.
+template <int FORM>
+struct Ahead {
+  const Args &p;
+  uint8_t *slots;  // this warp's: kAhead1 slots, and one for stores
+  uint32_t tensors, lane, depth, put = 0, got = 0;
+  __device__ __forceinline__ Ahead(const Args &args, uint8_t *area, uint32_t lane_)
+      : p(args), slots(area), tensors(epilogue_tensors<FORM>(args)), lane(lane_),
+        depth(tensors == 2 ? kAhead2 : kAhead1) {}
+  __device__ __forceinline__ uint8_t *out() const {
+    return slots + kAhead1 * kSlotBytes;
+  }
+  __device__ __forceinline__ uint8_t *slot(uint32_t i) const {
+    return slots + i * tensors * kSlotBytes;
+  }
+  // The next block to come (`exists`: there is one).
+  __device__ __forceinline__ void fetch(uint32_t row0, uint32_t col, bool exists) {
+    if (tensors) {
+      if (exists)
+        fetch_block<FORM>(p, slot(put), row0, col, lane);
+      copies_commit();
+      put = put + 1 == depth ? 0 : put + 1;
+    }
+  }
+  // The oldest fetched block has arrived.
+  __device__ __forceinline__ uint8_t *arrived() {
+    if (tensors == 2)
+      copies_wait<kAhead2 - 1>();
+    else if (tensors == 1)
+      copies_wait<kAhead1 - 1>();
+    __syncwarp();
+    uint8_t *at = slot(got);
+    got = got + 1 == depth ? 0 : got + 1;
+    return at;
+  }
+};
+
+// Columns of 16 consecutive rows (the skinny forward, whose tile is the
+// transposed product: lanes are columns, so a warp's access of one row covers
+// 32 consecutive columns).  Rows past the last are read as the last, so that
+// the loads need no branches and are in flight together.
 __device__ __forceinline__ void finish_column16(const Args &p, float (&v)[16],
                                                 uint32_t row, uint32_t col) {
   if (col >= p.cols || row >= p.rows)
     return;
   const bool f16 = p.is_f16 != 0;
   const uint32_t left = p.rows - row;
+  uint16_t r[16];
+  if (p.residual) {
+    const uint16_t *src =
+        static_cast<const uint16_t *>(p.residual) + row * p.ldr + col;
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i)
+      r[i] = src[min(i, left - 1) * p.ldr];
+  }
   if (p.bias) {
     const float b = from_bits(static_cast<const uint16_t *>(p.bias)[col], f16);
 #pragma unroll
@@ -158,23 +347,20 @@ __device__ __forceinline__ void finish_column16(const Args &p, float (&v)[16],
   if (p.preact_out) {
     uint16_t *z = static_cast<uint16_t *>(p.preact_out) + row * p.ldp + col;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (static_cast<uint32_t>(i) < left)
+    for (uint32_t i = 0; i < 16; ++i)
+      if (i < left)
         z[i * p.ldp] = to_bits(v[i], f16);
   }
   act_f32(p.activation, v);
   if (p.residual) {
-    const uint16_t *r =
-        static_cast<const uint16_t *>(p.residual) + row * p.ldr + col;
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (static_cast<uint32_t>(i) < left)
-        v[i] += from_bits(r[i * p.ldr], f16);
+      v[i] += from_bits(r[i], f16);
   }
   uint16_t *y = static_cast<uint16_t *>(p.out) + row * p.ldo + col;
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
-    if (static_cast<uint32_t>(i) < left)
+  for (uint32_t i = 0; i < 16; ++i)
+    if (i < left)
       y[i * p.ldo] = to_bits(v[i], f16);
 }
 
@@ -226,8 +412,11 @@ __device__ __forceinline__ void product_pair(const CUtensorMap *map_a,
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kStages], empty[kStages], sums_full[2], sums_empty[2];
   __shared__ uint32_t tmem_slot;
+  __shared__ alignas(16) float bias[kEpilogueWarps][128];
   uint8_t *ring = align1024(smem_raw);
-  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  uint8_t *slots = ring + kStages * HEXIR_PAIR_STAGE_BYTES;
+  const uint32_t warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x / 32, 0);
+  const uint32_t lane = threadIdx.x % 32;
   const uint32_t rank = cluster_ctarank();
   const uint32_t half_n = p.tile_n / 2;
   const uint32_t stage_bytes = kABytes + half_n * 128u;
@@ -257,25 +446,25 @@ __device__ __forceinline__ void product_pair(const CUtensorMap *map_a,
   const uint32_t first = blockIdx.x / 2, step = gridDim.x / 2;
 
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      for (uint32_t tile = first; tile < tiles && ok; tile += step) {
-        uint32_t tm, tn;
-        tile_of(tile, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
-        const uint32_t row0 = tm * 2 * kBM + rank * kBM;
-        const uint32_t col0 = tn * p.tile_n + rank * half_n;
-        for (uint32_t kt = 0; kt < p.k_tiles; ++kt, ++it) {
-          const uint32_t s = it % kStages;
-          if (!mbar_wait_bounded(&empty[s], (it / kStages & 1u) ^ 1u,
-                                 p.timeout_ns)) {
-            ok = false;
-            break;
-          }
+    const bool leader = elect_one();
+    RingPlace at;
+    uint32_t fills = 0;
+    bool ok = true;
+    for (uint32_t tile = first; tile < tiles && ok; tile += step) {
+      uint32_t tm, tn;
+      tile_of(tile, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
+      const uint32_t row0 = tm * 2 * kBM + rank * kBM;
+      const uint32_t col0 = tn * p.tile_n + rank * half_n;
+      for (uint32_t kt = 0; kt < p.k_tiles; ++kt, ++fills, at.next(kStages)) {
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait_pipeline(&empty[at.stage],
+                                                        at.parity ^ 1u, p.timeout_ns));
+        if (!ok)
+          break;
+        if (leader) {
           if (rank == 0)
-            mbar_arrive_expect_tx(&full[s], 2 * stage_bytes);
-          uint8_t *dst = ring + s * HEXIR_PAIR_STAGE_BYTES;
-          const uint32_t bar = cluster_addr(&full[s], 0);
+            mbar_arrive_expect_tx(&full[at.stage], 2 * stage_bytes);
+          uint8_t *dst = ring + at.stage * HEXIR_PAIR_STAGE_BYTES;
+          const uint32_t bar = cluster_addr(&full[at.stage], 0);
           load_operand<A_MN>(dst, kBM, row0, kt * kBK,
                              [&](uint8_t *d, int32_t x, int32_t y) {
                                tma_load_2d_pair(d, map_a, x, y, bar);
@@ -285,65 +474,102 @@ __device__ __forceinline__ void product_pair(const CUtensorMap *map_a,
                                tma_load_2d_pair(d, map_b, x, y, bar);
                              });
         }
+        __syncwarp();
       }
-      // Given up: the copies in flight land before the block ends.
-      if (!ok && rank == 0)
-        for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i)
-          mbar_wait_bounded(&full[i % kStages], i / kStages & 1u, p.timeout_ns);
     }
-  } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      const uint32_t desc = mma_desc<A_MN, B_MN>(2 * kBM, p.tile_n, p.is_f16 != 0);
-      uint32_t it = 0, t = 0;
-      bool ok = true;
-      for (uint32_t tile = first; tile < tiles && ok; tile += step, ++t) {
-        const uint32_t set = t & 1u;
-        if (!mbar_wait_bounded(&sums_empty[set], (t >> 1 & 1u) ^ 1u,
-                               p.timeout_ns))
+    // Given up: the copies in flight land before the block ends.
+    if (!ok && rank == 0)
+      for (uint32_t i = fills > kStages ? fills - kStages : 0; i < fills; ++i)
+        mbar_wait_pipeline(&full[i % kStages], i / kStages & 1u, p.timeout_ns);
+  } else if (warp == 1 && rank == 0) {
+    const bool leader = elect_one();
+    const uint32_t desc = mma_desc<A_MN, B_MN>(2 * kBM, p.tile_n, p.is_f16 != 0);
+    const uint32_t ring_addr = smem_addr(ring);
+    RingPlace at;
+    uint32_t t = 0;
+    bool ok = true, ready = false;
+    for (uint32_t tile = first; tile < tiles && ok; tile += step, ++t) {
+      const uint32_t set = t & 1u;
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait_pipeline(&sums_empty[set],
+                                                      (t >> 1 & 1u) ^ 1u,
+                                                      p.timeout_ns));
+      if (!ok)
+        break;
+      tc_fence_after();
+      for (uint32_t kt = 0; kt < p.k_tiles; ++kt) {
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait_pipeline(&full[at.stage], at.parity,
+                                                        p.timeout_ns, ready));
+        if (!ok)
           break;
         tc_fence_after();
-        for (uint32_t kt = 0; kt < p.k_tiles; ++kt, ++it) {
-          const uint32_t s = it % kStages;
-          if (!mbar_wait_bounded(&full[s], it / kStages & 1u, p.timeout_ns)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t a = smem_addr(ring + s * HEXIR_PAIR_STAGE_BYTES);
-          mma_stage<2, A_MN, B_MN>(tmem + set * 256u, a, a + kABytes, desc,
-                                   kt == 0);
-          mma_commit_pair(&empty[s]);
+        const uint32_t stage = at.stage;
+        const uint32_t a = ring_addr + stage * HEXIR_PAIR_STAGE_BYTES;
+        at.next(kStages);
+        // The next stage's barrier is tried under this one's MMAs.
+        ready = mbar_test(&full[at.stage], at.parity);
+        if (leader) {
+          mma_stage<2, A_MN, B_MN>(tmem + set * 256u, a, a + kABytes, desc, kt == 0);
+          mma_commit_pair(&empty[stage]);
+          if (kt + 1 == p.k_tiles)
+            mma_commit_pair(&sums_full[set]);
         }
-        if (ok)
-          mma_commit_pair(&sums_full[set]);
+        __syncwarp();
       }
     }
   } else if (warp >= 4) {
     const uint32_t quarter = warp & 3u, side = (warp - 4) / 4;
+    const uint32_t blocks = half_n / 16;  // of this warp in a tile
+    const uint32_t row_in = rank * kBM + quarter * 32;
+    Ahead<FORM> ahead(p, slots + (warp - 4) * (kAhead1 + 1) * kSlotBytes, lane);
+    uint32_t next_tile = first, next_block = 0;
+    auto fetch_next = [&] {
+      uint32_t tm = 0, tn = 0;
+      if (next_tile < tiles)
+        tile_of(next_tile, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
+      ahead.fetch(tm * 2 * kBM + row_in,
+                  tn * p.tile_n + side * half_n + next_block * 16, next_tile < tiles);
+      if (++next_block == blocks) {
+        next_block = 0;
+        next_tile += step;
+      }
+    };
+    for (uint32_t i = 0; i < ahead.depth; ++i)
+      fetch_next();
     uint32_t t = 0;
     for (uint32_t tile = first; tile < tiles; tile += step, ++t) {
       uint32_t tm, tn;
       tile_of(tile, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
-      const uint32_t row = tm * 2 * kBM + rank * kBM + quarter * 32 + lane;
+      const uint32_t row0 = tm * 2 * kBM + row_in;
       const uint32_t set = t & 1u;
+      if (FORM == HEXIR_PRODUCT_FORWARD && p.bias)
+        stage_bias(p, bias[warp - 4], tn * p.tile_n + side * half_n, half_n, lane);
       // The whole warp leaves together: its TMEM loads are warp-wide.
       if (!__all_sync(0xFFFFFFFFu,
-                      mbar_wait_bounded(&sums_full[set], t >> 1 & 1u,
-                                        4 * p.timeout_ns)))
+                      mbar_wait_pipeline(&sums_full[set], t >> 1 & 1u,
+                                         4 * p.timeout_ns)))
         break;
       tc_fence_after();
       const uint32_t src = tmem + (quarter * 32u << 16) + set * 256u;
-      for (uint32_t c = side * half_n; c < side * half_n + half_n; c += 16) {
+      for (uint32_t i = 0; i < blocks; ++i) {
+        const uint32_t c = side * half_n + i * 16;
         float v[16];
         __syncwarp();
         tmem_load16(src + c, v);
-        finish16<FORM>(p, v, row, tn * p.tile_n + c);
+        if (i + 1 == blocks) {
+          // The sums are in registers: the next tile but one may begin.
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0)
+            mbar_arrive_cluster(cluster_addr(&sums_empty[set], 0));
+        }
+        uint8_t *slot = ahead.arrived();
+        finish_block<FORM>(p, v, bias[warp - 4] + i * 16, slot, ahead.out(), row0,
+                           tn * p.tile_n + c, lane);
+        __syncwarp();
+        fetch_next();
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0)
-        mbar_arrive_cluster(cluster_addr(&sums_empty[set], 0));
     }
+    copies_wait<0>();
   }
   __syncthreads();
   __syncwarp();
@@ -366,56 +592,110 @@ __device__ __forceinline__ void product_pair(const CUtensorMap *map_a,
 //
 // GUARDED: rows that TMA cannot describe (a stride or base off 16 bytes).
 // The epilogue warps load the operands with bounds checks, into the layout
-// TMA would have written, and become the epilogue afterwards.
+// TMA would have written, and become the epilogue afterwards.  An operand
+// that TMA can describe still comes by TMA.
 
-// One 16-byte chunk: 8 elements of row `major` from `minor` on, zero beyond
-// the operand.
-__device__ __forceinline__ uint4 guarded_chunk(const uint16_t *base, uint64_t ld,
-                                               uint32_t major, uint32_t majors,
-                                               uint32_t minor, uint32_t minors) {
-  uint4 w = make_uint4(0, 0, 0, 0);
-  if (major >= majors || minor >= minors)
-    return w;
-  const uint16_t *src = base + major * ld + minor;
-  const uint32_t left = minors - minor;
-  const uintptr_t at = reinterpret_cast<uintptr_t>(src);
-  if (left >= 8 && (at & 15u) == 0)
-    return *reinterpret_cast<const uint4 *>(src);
-  uint32_t e[8];
-  if (left >= 8 && (at & 3u) == 0) {
-    const uint32_t *q = reinterpret_cast<const uint32_t *>(src);
-    return make_uint4(q[0], q[1], q[2], q[3]);
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    e[i] = static_cast<uint32_t>(i) < left ? src[i] : 0u;
-  w.x = e[0] | e[1] << 16;
-  w.y = e[2] | e[3] << 16;
-  w.z = e[4] | e[5] << 16;
-  w.w = e[6] | e[7] << 16;
-  return w;
+// 8 elements of an operand's row that may start anywhere: the one or two
+// 16-byte blocks of memory they lie in, and where.
+struct Chunk {
+  uint4 lo, hi;
+  uint32_t shift;  // bytes into lo; 16: taken element by element, in place
+  uint32_t count;  // elements of the operand, the rest are 0
+};
+
+// The operand's memory, gaps between rows included: what a load may touch.
+struct Side {
+  const uint16_t *base;
+  uint64_t ld;
+  uintptr_t first, last;
+  uint32_t majors, minors;  // rows, elements of a row
+};
+__device__ __forceinline__ Side side_of(const void *p, uint64_t ld, uint32_t majors,
+                                        uint32_t minors) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  return {static_cast<const uint16_t *>(p), ld, at,
+          at + ((majors - 1) * ld + minors) * 2, majors, minors};
 }
 
-// size x 64 of an operand (side from `side0`, summed index from k0) into the
-// swizzled layout of a stage, by 128 threads.
+// Start the loads of 8 elements of row `major` from `minor` on.
+__device__ __forceinline__ void chunk_load(const Side &s, uint32_t major,
+                                           uint32_t minor, Chunk &c) {
+  c.lo = c.hi = make_uint4(0, 0, 0, 0);
+  c.shift = 0;
+  c.count = major < s.majors && minor < s.minors ? min(8u, s.minors - minor) : 0u;
+  if (!c.count)
+    return;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(s.base + major * s.ld + minor);
+  const uintptr_t block = at & ~static_cast<uintptr_t>(15);
+  c.shift = static_cast<uint32_t>(at - block);
+  const bool two = c.shift + 2 * c.count > 16;
+  if (block >= s.first && block + (two ? 32 : 16) <= s.last) {
+    c.lo = __ldg(reinterpret_cast<const uint4 *>(block));
+    if (two)
+      c.hi = __ldg(reinterpret_cast<const uint4 *>(block + 16));
+    return;
+  }
+  // At the ends of the tensor.
+  const uint16_t *src = reinterpret_cast<const uint16_t *>(at);
+  uint32_t e[8];
+#pragma unroll
+  for (uint32_t i = 0; i < 8; ++i)
+    e[i] = src[min(i, c.count - 1)];
+  c.lo = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16,
+                    e[6] | e[7] << 16);
+  c.shift = 16;
+}
+
+// The 8 elements, those beyond the operand 0.
+__device__ __forceinline__ uint4 chunk_value(const Chunk &c) {
+  uint32_t w[8] = {c.lo.x, c.lo.y, c.lo.z, c.lo.w, c.hi.x, c.hi.y, c.hi.z, c.hi.w};
+  const uint32_t words = c.shift / 4;  // 4: in place
+  if (words & 2u) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i)
+      w[i] = w[i + 2];
+  }
+  if (words & 1u) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i)
+      w[i] = w[i + 1];
+  }
+  const uint32_t bits = (c.shift & 2u) * 8u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = __funnelshift_r(w[i], w[i + 1], bits);
+    const uint32_t n = c.count > 2u * i ? c.count - 2u * i : 0u;
+    w[i] &= n >= 2 ? 0xFFFFFFFFu : (n == 1 ? 0xFFFFu : 0u);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+constexpr uint32_t kLoaders = 256;                // threads
+constexpr uint32_t kChunks = kBM * 8 / kLoaders;  // of an operand's tile, a thread
+
+// This thread's chunks of a 128 x 64 operand tile (side from `side0`, summed
+// index from k0).
 template <bool MN>
-__device__ __forceinline__ void guarded_operand(uint8_t *dst, const void *base,
-                                                uint64_t ld, uint32_t size,
-                                                uint32_t side0, uint32_t sides,
-                                                uint32_t k0, uint32_t depth,
-                                                uint32_t tid) {
-  const uint16_t *src = static_cast<const uint16_t *>(base);
-  const uint32_t chunks = size * 8;
-#pragma unroll 4
-  for (uint32_t i = tid; i < chunks; i += 128) {
-    const uint32_t r = i / 8, c = i % 8;  // 128-byte row of the stage, chunk
-    uint4 w;
+__device__ __forceinline__ void operand_load(const Side &s, uint32_t side0,
+                                             uint32_t k0, uint32_t tid,
+                                             Chunk (&c)[kChunks]) {
+#pragma unroll
+  for (uint32_t i = 0; i < kChunks; ++i) {
+    const uint32_t r = (i * kLoaders + tid) / 8, j = tid % 8;
     if (MN)
-      w = guarded_chunk(src, ld, k0 + r % 64, depth, side0 + r / 64 * 64 + c * 8,
-                        sides);
+      chunk_load(s, k0 + r % 64, side0 + r / 64 * 64 + j * 8, c[i]);
     else
-      w = guarded_chunk(src, ld, side0 + r, sides, k0 + c * 8, depth);
-    *reinterpret_cast<uint4 *>(dst + r * 128 + ((c ^ (r & 7u)) << 4)) = w;
+      chunk_load(s, side0 + r, k0 + j * 8, c[i]);
+  }
+}
+// Into the stage, as TMA's 128-byte swizzle would have it.
+__device__ __forceinline__ void operand_store(uint8_t *dst, uint32_t tid,
+                                              const Chunk (&c)[kChunks]) {
+#pragma unroll
+  for (uint32_t i = 0; i < kChunks; ++i) {
+    const uint32_t r = (i * kLoaders + tid) / 8, j = tid % 8;
+    *reinterpret_cast<uint4 *>(dst + r * 128 + ((j ^ (r & 7u)) << 4)) =
+        chunk_value(c[i]);
   }
 }
 
@@ -426,22 +706,31 @@ __device__ __forceinline__ void product_single(const CUtensorMap *map_a,
   constexpr bool A_MN = SWAP || FORM == HEXIR_PRODUCT_WEIGHT_GRAD;
   constexpr bool B_MN = !SWAP && FORM != HEXIR_PRODUCT_INPUT_GRAD;
   constexpr uint32_t kMax = HEXIR_SINGLE_MAX_STAGES;
+  constexpr uint32_t kWarps = HEXIR_SINGLE_EPILOGUE_WARPS;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kMax], empty[kMax], done;
   __shared__ uint32_t tmem_slot;
+  __shared__ alignas(16) float bias[SWAP ? 1 : kWarps][64];
   uint8_t *ring = align1024(smem_raw);
-  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  uint8_t *slots = ring + p.ring_bytes;
+  const uint32_t warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x / 32, 0);
+  const uint32_t lane = threadIdx.x % 32;
   const uint32_t rank = p.split > 1 ? cluster_ctarank() : 0;
   const uint32_t stages = p.stages;
-  const uint32_t stage_bytes = kABytes + p.tile_n * 128u;
+  const uint32_t b_bytes = p.tile_n * 128u;
+  const uint32_t stage_bytes = kABytes + b_bytes;
+  // Which operands come by TMA.
+  const bool tma_a = !GUARDED || (p.tma_operands & 1u);
+  const bool tma_b = !GUARDED || (p.tma_operands & 2u);
+  const uint32_t tma_bytes = (tma_a ? kABytes : 0u) + (tma_b ? b_bytes : 0u);
 
   if (threadIdx.x == 0) {
-    if (!GUARDED) {
+    if (tma_a)
       prefetch_tensormap(map_a);
+    if (tma_b)
       prefetch_tensormap(map_b);
-    }
     for (uint32_t s = 0; s < stages; ++s) {
-      mbar_init(&full[s], GUARDED ? 128 : 1);
+      mbar_init(&full[s], (GUARDED ? kLoaders : 0u) + (tma_bytes ? 1u : 0u));
       mbar_init(&empty[s], 1);
     }
     mbar_init(&done, 1);
@@ -462,79 +751,150 @@ __device__ __forceinline__ void product_single(const CUtensorMap *map_a,
   const uint32_t kt1 = static_cast<uint32_t>(
       static_cast<uint64_t>(p.k_tiles) * (rank + 1) / p.split);
   const uint32_t lane0 = tm * kBM, col0 = tn * p.tile_n;
+  // The epilogue warps: 32 lanes' rows, and every other block of 16 columns
+  // (of the cluster's share of them, once the sums are joined).
+  const uint32_t quarter = warp & 3u, side = warp >= 2 ? (warp - 2) / 4 : 0;
+  const uint32_t row0 = lane0 + quarter * 32;
+  const uint32_t blocks = p.tile_n / 16;
+  const uint32_t block0 = rank * 2 + side, block_step = 2 * p.split;
+  Ahead<FORM> ahead(p, slots + (warp >= 2 ? warp - 2 : 0) * (kAhead1 + 1) * kSlotBytes,
+                    lane);
+  uint32_t next_block = block0;
+  auto fetch_next = [&] {
+    ahead.fetch(row0, col0 + next_block * 16, next_block < blocks);
+    next_block += block_step;
+  };
   bool ok = true;
 
   if (warp == 0) {
-    if (!GUARDED && lane == 0) {
-      uint32_t it = 0;
-      for (uint32_t kt = kt0; kt < kt1; ++kt, ++it) {
-        const uint32_t s = it % stages;
-        if (!mbar_wait_bounded(&empty[s], (it / stages & 1u) ^ 1u,
-                               p.timeout_ns)) {
-          ok = false;
+    if (tma_bytes) {
+      const bool leader = elect_one();
+      RingPlace at;
+      uint32_t fills = 0;
+      for (uint32_t kt = kt0; kt < kt1; ++kt, ++fills, at.next(stages)) {
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait_pipeline(&empty[at.stage],
+                                                        at.parity ^ 1u, p.timeout_ns));
+        if (!ok)
           break;
+        if (leader) {
+          uint64_t *bar = &full[at.stage];
+          mbar_arrive_expect_tx(bar, tma_bytes);
+          uint8_t *dst = ring + at.stage * stage_bytes;
+          if (tma_a)
+            load_operand<A_MN>(dst, kBM, lane0, kt * kBK,
+                               [&](uint8_t *d, int32_t x, int32_t y) {
+                                 tma_load_2d(d, map_a, x, y, bar);
+                               });
+          if (tma_b)
+            load_operand<B_MN>(dst + kABytes, p.tile_n, col0, kt * kBK,
+                               [&](uint8_t *d, int32_t x, int32_t y) {
+                                 tma_load_2d(d, map_b, x, y, bar);
+                               });
         }
-        mbar_arrive_expect_tx(&full[s], stage_bytes);
-        uint8_t *dst = ring + s * stage_bytes;
-        load_operand<A_MN>(dst, kBM, lane0, kt * kBK,
-                           [&](uint8_t *d, int32_t x, int32_t y) {
-                             tma_load_2d(d, map_a, x, y, &full[s]);
-                           });
-        load_operand<B_MN>(dst + kABytes, p.tile_n, col0, kt * kBK,
-                           [&](uint8_t *d, int32_t x, int32_t y) {
-                             tma_load_2d(d, map_b, x, y, &full[s]);
-                           });
+        __syncwarp();
       }
+      // Given up: the copies in flight land before the block ends (with loads
+      // beside them the phase may not complete: the wait is bounded).
       if (!ok)
-        for (uint32_t i = it > stages ? it - stages : 0; i < it; ++i)
-          mbar_wait_bounded(&full[i % stages], i / stages & 1u, p.timeout_ns);
+        for (uint32_t i = fills > stages ? fills - stages : 0; i < fills; ++i)
+          mbar_wait_pipeline(&full[i % stages], i / stages & 1u, p.timeout_ns);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t desc = mma_desc<A_MN, B_MN>(kBM, p.tile_n, p.is_f16 != 0);
-      uint32_t it = 0;
-      for (uint32_t kt = kt0; kt < kt1; ++kt, ++it) {
-        const uint32_t s = it % stages;
-        if (!mbar_wait_bounded(&full[s], it / stages & 1u, p.timeout_ns))
-          break;
-        tc_fence_after();
-        const uint32_t a = smem_addr(ring + s * stage_bytes);
+    const bool leader = elect_one();
+    const uint32_t desc = mma_desc<A_MN, B_MN>(kBM, p.tile_n, p.is_f16 != 0);
+    const uint32_t ring_addr = smem_addr(ring);
+    RingPlace at;
+    bool ready = false;
+    for (uint32_t kt = kt0; kt < kt1; ++kt) {
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait_pipeline(&full[at.stage], at.parity,
+                                                      p.timeout_ns, ready)))
+        break;
+      tc_fence_after();
+      const uint32_t stage = at.stage;
+      const uint32_t a = ring_addr + stage * stage_bytes;
+      at.next(stages);
+      // The next stage's barrier is tried under this one's MMAs.
+      ready = mbar_test(&full[at.stage], at.parity);
+      if (leader) {
         mma_stage<1, A_MN, B_MN>(tmem, a, a + kABytes, desc, kt == kt0);
-        mma_commit(&empty[s]);
+        mma_commit(&empty[stage]);
       }
-      mma_commit(&done);  // also after a wait that ran out: nothing in flight
+      __syncwarp();
     }
+    if (leader)
+      mma_commit(&done);  // also after a wait that ran out: nothing in flight
   } else {
-    const uint32_t tid = threadIdx.x - 64;
+    if (!SWAP) {
+      for (uint32_t i = 0; i < ahead.depth; ++i)
+        fetch_next();
+      if (FORM == HEXIR_PRODUCT_FORWARD && p.bias) {
+        // Block i of this warp has bias[16 i ..].
+        __syncwarp();
+        for (uint32_t i = lane; i < blocks * 8; i += 32) {
+          const uint32_t c = col0 + (block0 + i / 16 * block_step) * 16 + i % 16;
+          bias[warp - 2][i] =
+              block0 + i / 16 * block_step < blocks && c < p.cols
+                  ? from_bits(static_cast<const uint16_t *>(p.bias)[c], p.is_f16 != 0)
+                  : 0.0f;
+        }
+        __syncwarp();
+      }
+    }
     if (GUARDED) {
-      uint32_t it = 0;
-      for (uint32_t kt = kt0; kt < kt1; ++kt, ++it) {
-        const uint32_t s = it % stages;
-        if (!mbar_wait_bounded(&empty[s], (it / stages & 1u) ^ 1u, p.timeout_ns))
-          break;
-        uint8_t *dst = ring + s * stage_bytes;
-        guarded_operand<A_MN>(dst, p.a, p.lda, kBM, lane0, p.rows, kt * kBK,
-                              p.depth, tid);
-        guarded_operand<B_MN>(dst + kABytes, p.b, p.ldb, p.tile_n, col0, p.cols,
-                              kt * kBK, p.depth, tid);
+      // The loads of one stage are in flight while the last one's are shifted
+      // into place and stored.
+      const uint32_t tid = threadIdx.x - 64;
+      const Side side_a = A_MN ? side_of(p.a, p.lda, p.depth, p.rows)
+                               : side_of(p.a, p.lda, p.rows, p.depth);
+      const Side side_b = B_MN ? side_of(p.b, p.ldb, p.depth, p.cols)
+                               : side_of(p.b, p.ldb, p.cols, p.depth);
+      Chunk ca[2][kChunks], cb[2][kChunks];
+      RingPlace at;
+      auto load = [&](uint32_t kt, Chunk (&a)[kChunks], Chunk (&b)[kChunks]) {
+        if (kt < kt1) {
+          if (!tma_a)
+            operand_load<A_MN>(side_a, lane0, kt * kBK, tid, a);
+          if (!tma_b)
+            operand_load<B_MN>(side_b, col0, kt * kBK, tid, b);
+        }
+      };
+      auto settle = [&](const Chunk (&a)[kChunks], const Chunk (&b)[kChunks]) {
+        if (!mbar_wait_pipeline(&empty[at.stage], at.parity ^ 1u, p.timeout_ns))
+          return false;
+        uint8_t *dst = ring + at.stage * stage_bytes;
+        if (!tma_a)
+          operand_store(dst, tid, a);
+        if (!tma_b)
+          operand_store(dst + kABytes, tid, b);
         fence_async_smem();
-        mbar_arrive(&full[s]);
+        mbar_arrive(&full[at.stage]);
+        at.next(stages);
+        return true;
+      };
+      load(kt0, ca[0], cb[0]);
+      for (uint32_t kt = kt0; kt < kt1; kt += 2) {
+        load(kt + 1, ca[1], cb[1]);
+        if (!settle(ca[0], cb[0]))
+          break;
+        load(kt + 2, ca[0], cb[0]);
+        if (kt + 1 < kt1 && !settle(ca[1], cb[1]))
+          break;
       }
       __syncwarp();
     }
     ok = __all_sync(0xFFFFFFFFu,
-                    mbar_wait_bounded(&done, 0, 4 * p.timeout_ns));
+                    mbar_wait_pipeline(&done, 0, 4 * p.timeout_ns));
     tc_fence_after();
-    const uint32_t quarter = warp & 3u;
     const uint32_t src = tmem + (quarter * 32u << 16);
     const uint32_t my = quarter * 32 + lane;
-    float *sums = reinterpret_cast<float *>(ring);  // [tile_n][128], split > 1
+    // split > 1: this CTA's sums, [tile_n / 4][128] of 4.
+    float4 *sums = reinterpret_cast<float4 *>(ring);
     if (ok) {
-      for (uint32_t c = 0; c < p.tile_n; c += 16) {
+      for (uint32_t n = side; n < blocks; n += 2) {
         float v[16];
         __syncwarp();
         if (kt1 > kt0) {
-          tmem_load16(src + c, v);
+          tmem_load16(src + n * 16, v);
         } else {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
@@ -542,12 +902,17 @@ __device__ __forceinline__ void product_single(const CUtensorMap *map_a,
         }
         if (p.split > 1) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            sums[(c + i) * kBM + my] = v[i];
+          for (int i = 0; i < 4; ++i)
+            sums[(n * 4 + i) * kBM + my] =
+                make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
         } else if (SWAP) {
-          finish_column16(p, v, col0 + c, lane0 + my);
+          finish_column16(p, v, col0 + n * 16, lane0 + my);
         } else {
-          finish16<FORM>(p, v, lane0 + my, col0 + c);
+          uint8_t *slot = ahead.arrived();
+          finish_block<FORM>(p, v, bias[warp - 2] + n / 2 * 16, slot, ahead.out(),
+                             row0, col0 + n * 16, lane);
+          __syncwarp();
+          fetch_next();
         }
       }
     }
@@ -557,28 +922,45 @@ __device__ __forceinline__ void product_single(const CUtensorMap *map_a,
     __syncwarp();
     cluster_sync();
     if (warp >= 2 && ok) {
-      const uint32_t my = (warp & 3u) * 32 + lane;
-      const float *sums = reinterpret_cast<const float *>(ring);
-      for (uint32_t c = rank * 16; c < p.tile_n; c += p.split * 16) {
+      const uint32_t my = quarter * 32 + lane;
+      const float4 *sums = reinterpret_cast<const float4 *>(ring);
+      uint32_t nth = 0;
+      for (uint32_t n = block0; n < blocks; n += block_step, ++nth) {
         float v[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           v[i] = 0.0f;
+#pragma unroll 2
         for (uint32_t r = 0; r < p.split; ++r) {
-          const uint32_t from = cluster_addr(sums + c * kBM + my, r);
+          const uint32_t from = cluster_addr(sums + n * 4 * kBM + my, r);
+          float4 q[4];
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            v[i] += ld_cluster_f32(from + i * (kBM * 4u));
+          for (int i = 0; i < 4; ++i)
+            q[i] = ld_cluster_v4(from + i * (kBM * 16u));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            v[4 * i] += q[i].x;
+            v[4 * i + 1] += q[i].y;
+            v[4 * i + 2] += q[i].z;
+            v[4 * i + 3] += q[i].w;
+          }
         }
-        if (SWAP)
-          finish_column16(p, v, col0 + c, lane0 + my);
-        else
-          finish16<FORM>(p, v, lane0 + my, col0 + c);
+        if (SWAP) {
+          finish_column16(p, v, col0 + n * 16, lane0 + my);
+        } else {
+          uint8_t *slot = ahead.arrived();
+          finish_block<FORM>(p, v, bias[warp - 2] + nth * 16, slot, ahead.out(), row0,
+                             col0 + n * 16, lane);
+          __syncwarp();
+          fetch_next();
+        }
       }
     }
     __syncwarp();
     cluster_sync();  // the peers have read this CTA's sums
   }
+  if (warp >= 2)
+    copies_wait<0>();
   tc_fence_before();
   __syncthreads();
   __syncwarp();
@@ -598,15 +980,16 @@ __device__ __forceinline__ void product_single(const CUtensorMap *map_a,
     product_pair<FORM>(&map_a, &map_b, args);                                 \
   }
 #define PRODUCT_SINGLE(NAME, FORM, SWAP)                                      \
-  extern "C" __global__ void __launch_bounds__(HEXIR_SINGLE_THREADS)          \
+  extern "C" __global__ void __launch_bounds__(HEXIR_SINGLE_THREADS, 2)       \
       NAME(const __grid_constant__ CUtensorMap map_a,                         \
            const __grid_constant__ CUtensorMap map_b, const Args args) {      \
     product_single<FORM, false, SWAP>(&map_a, &map_b, args);                  \
   }
 #define PRODUCT_GUARDED(NAME, FORM)                                           \
   extern "C" __global__ void __launch_bounds__(HEXIR_SINGLE_THREADS)          \
-      NAME(const Args args) {                                                 \
-    product_single<FORM, true, false>(nullptr, nullptr, args);                \
+      NAME(const __grid_constant__ CUtensorMap map_a,                         \
+           const __grid_constant__ CUtensorMap map_b, const Args args) {      \
+    product_single<FORM, true, false>(&map_a, &map_b, args);                  \
   }
 
 PRODUCT_PAIR(hexir_linear_16_pair, HEXIR_PRODUCT_FORWARD)

@@ -8,6 +8,66 @@
 
 namespace hexir {
 
+// mbar_wait_bounded for the main loops: `tried` says that the phase was seen
+// complete already (a try issued earlier, whose answer took its ~100 cycles
+// under other work).  The timer is read only after 64 tries.
+__device__ __forceinline__ bool mbar_wait_pipeline(uint64_t *bar, uint32_t parity,
+                                                   uint64_t timeout_ns,
+                                                   bool tried = false) {
+  if (tried)
+    return true;
+  uint64_t start = 0;
+  for (uint32_t spin = 1;; ++spin) {
+    if (mbar_try_wait(bar, parity))
+      return true;
+    if ((spin & 63u) == 0u) {
+      const uint64_t now = global_timer_ns();
+      if (start == 0) {
+        start = now;
+      } else if (now - start > timeout_ns) {
+        atomicOr(&hexir_device_error_word, HEXIR_KERR_WAIT_TIMEOUT);
+        return false;
+      }
+    }
+  }
+}
+
+// Whether the phase with the given parity has completed, without waiting (a
+// try_wait may hold the thread for a while).
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
+// One lane of a converged warp, the same at every call.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xFFFFFFFF;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
+// A place in a ring of stages: the stage, and the parity of its use.
+struct RingPlace {
+  uint32_t stage = 0, parity = 0;
+  __device__ __forceinline__ void next(uint32_t stages) {
+    if (++stage == stages) {
+      stage = 0;
+      parity ^= 1u;
+    }
+  }
+};
+
 template <int CG>
 __device__ __forceinline__ void tmem_alloc(uint32_t *slot, uint32_t cols) {
   if (CG == 1) {
@@ -146,9 +206,12 @@ __device__ __forceinline__ uint32_t cluster_addr(const void *p, uint32_t rank) {
   return remote;
 }
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 

@@ -203,8 +203,9 @@ CUdeviceptr layers_error_word(const LayersLib *lib) { return lib->error_word; }
 
 namespace {
 
-// The most dynamic shared memory any of the product kernels is launched with.
-constexpr uint32_t kSmemLimit = 227u * 1024u - 2048u;
+// The most dynamic shared memory a product kernel is launched with, beside up
+// to 5 KiB of its own.
+constexpr uint32_t kSmemLimit = 221u * 1024u;
 // The same of the norm kernels, beside up to 8 KiB of their own.
 constexpr uint32_t kNormSmemLimit = 218u * 1024u;
 
@@ -391,7 +392,7 @@ struct ProductPlan {
   uint32_t variant = 0;
   uint32_t tile_n = 0, split = 1, stages = 0;
   uint32_t tiles_m = 0, tiles_n = 0;
-  uint32_t tmem_cols = 0, smem = 0;
+  uint32_t tmem_cols = 0, ring = 0, smem = 0;
   std::string refusal;  // a forced kernel that cannot run this
 };
 
@@ -399,8 +400,9 @@ uint32_t stage_bytes(uint32_t tile_n) {
   return HEXIR_PRODUCT_BM * 128u + tile_n * 128u;
 }
 
+// slots: the epilogue reads or stores through shared memory.
 ProductPlan plan_product(uint32_t op, uint32_t m, uint32_t n, uint32_t k,
-                         bool aligned, uint32_t flags, uint32_t sms) {
+                         bool aligned, bool slots, uint32_t flags, uint32_t sms) {
   // out [rows][cols], summed over depth.
   const uint32_t rows = op == HEXIR_PRODUCT_WEIGHT_GRAD ? k : m;
   const uint32_t cols = op == HEXIR_PRODUCT_INPUT_GRAD ? k : n;
@@ -439,8 +441,6 @@ ProductPlan plan_product(uint32_t op, uint32_t m, uint32_t n, uint32_t k,
     // The weight stream is the cost: CTAs for every SM, two per SM.
     while (p.split < max_split && p.tiles_m * p.split * 2 <= 2 * sms)
       p.split *= 2;
-    p.stages = std::min<uint32_t>(HEXIR_SINGLE_MAX_STAGES,
-                                  100u * 1024u / stage_bytes(p.tile_n));
     p.tmem_cols = p.tile_n <= 32 ? 32 : 64;
   } else {
     if (p.variant == 0 || p.variant == kPair) {
@@ -497,21 +497,27 @@ ProductPlan plan_product(uint32_t op, uint32_t m, uint32_t n, uint32_t k,
     }
     p.tiles_m = ceil_div(rows, HEXIR_PRODUCT_BM);
     p.tiles_n = ceil_div(cols, p.tile_n);
-    // One CTA per SM with a deep ring, or two whose main loops and epilogues
-    // overlap.
-    const uint64_t ctas = static_cast<uint64_t>(p.tiles_m) * p.tiles_n * p.split;
-    p.stages = (ctas <= sms ? 196u : 100u) * 1024u / stage_bytes(p.tile_n);
-    p.stages = std::min<uint32_t>(p.stages, HEXIR_SINGLE_MAX_STAGES);
     p.tmem_cols = p.tile_n;
   }
   if (forced_split)
     p.split = forced_split;
+  // One CTA per SM with a deep ring, or, where there are more and their
+  // epilogues need no slots, two whose main loops and epilogues overlap.
+  const uint64_t ctas = static_cast<uint64_t>(p.tiles_m) * p.tiles_n * p.split;
+  const uint32_t epilogue =
+      slots && p.variant != kSkinny
+          ? HEXIR_EPILOGUE_BYTES(HEXIR_SINGLE_EPILOGUE_WARPS) : 0u;
+  const bool two = p.variant == kSkinny || (ctas > sms && !epilogue);
+  const uint32_t room = (two ? 108u : 216u) * 1024u - epilogue;
+  p.stages = std::min<uint32_t>(HEXIR_SINGLE_MAX_STAGES, room / stage_bytes(p.tile_n));
+  // The ring also holds a split tile's sums.
+  p.ring = std::max<uint32_t>(p.stages * stage_bytes(p.tile_n),
+                              p.split > 1 ? HEXIR_PRODUCT_BM * p.tile_n * 4u : 0u);
   // Shared memory: at least what keeps the TMEM columns of the CTAs that fit
   // an SM within its 512 (a CTA that waits for columns while it holds a place
   // in a cluster could wait on a cluster that waits for it): 227 KiB / 512
   // columns = 454 bytes per column.
-  const uint32_t ring = p.stages * stage_bytes(p.tile_n);
-  p.smem = std::max<uint32_t>(ring, p.tmem_cols * 512u) + 1024u;
+  p.smem = std::max<uint32_t>(p.ring + epilogue, p.tmem_cols * 512u) + 1024u;
   return p;
 }
 
@@ -543,10 +549,16 @@ hexir_status_t launch_product(Call &call, uint32_t op, uint32_t m, uint32_t n,
     return HEXIR_OK;
   const bool a_mn = op == HEXIR_PRODUCT_WEIGHT_GRAD;
   const bool b_mn = op != HEXIR_PRODUCT_INPUT_GRAD;
-  const bool aligned = rows16(args.a, args.lda, 2) && rows16(args.b, args.ldb, 2) &&
-                       args.lda < 1ull << 39 && args.ldb < 1ull << 39;
+  const bool aligned_a = rows16(args.a, args.lda, 2) && args.lda < 1ull << 39;
+  const bool aligned_b = rows16(args.b, args.ldb, 2) && args.ldb < 1ull << 39;
+  const bool aligned = aligned_a && aligned_b;
   const uint32_t sms = static_cast<uint32_t>(std::max(call.dev->sm_count, 2));
-  const ProductPlan p = plan_product(op, m, n, k, aligned, flags, sms);
+  args.vec = rows16(args.out, args.ldo, 2) &&
+             (!args.preact_out || rows16(args.preact_out, args.ldp, 2)) &&
+             (!args.residual || rows16(args.residual, args.ldr, 2)) &&
+             (!args.slope_at || rows16(args.slope_at, args.lds, 2));
+  const bool slots = !args.vec || args.residual || args.slope_at;
+  const ProductPlan p = plan_product(op, m, n, k, aligned, slots, flags, sms);
   if (!p.refusal.empty())
     return fail(&call.error, "linear: " + p.refusal, HEXIR_ERROR_INVALID_ARGUMENT);
   const uint64_t tiles = static_cast<uint64_t>(p.tiles_m) * p.tiles_n;
@@ -561,24 +573,10 @@ hexir_status_t launch_product(Call &call, uint32_t op, uint32_t m, uint32_t n,
   args.split = p.split;
   args.stages = p.stages;
   args.tmem_cols = p.tmem_cols;
+  args.ring_bytes = p.ring;
   args.timeout_ns = kWaitTimeoutNs;
-  args.vec = rows16(args.out, args.ldo, 2) &&
-             (!args.preact_out || rows16(args.preact_out, args.ldp, 2)) &&
-             (!args.bias || !off(args.bias, 16)) &&
-             (!args.residual || rows16(args.residual, args.ldr, 2)) &&
-             (!args.slope_at || rows16(args.slope_at, args.lds, 2));
 
   const unsigned grid = static_cast<unsigned>(tiles * p.split);
-  if (p.variant == kGuardedLoads) {
-    void *params[] = {&args};
-    const char *what = "launch hexir_linear_16 guarded";
-    return p.split > 1
-               ? launch_cluster(call.lib->guarded[op], grid, p.split,
-                                HEXIR_SINGLE_THREADS, p.smem, stream, params,
-                                what, &call.error)
-               : launch(call.lib->guarded[op], grid, 1, HEXIR_SINGLE_THREADS,
-                        p.smem, stream, params, what, &call.error);
-  }
   Operand a = {args.a, args.lda, a_mn, args.rows, HEXIR_PRODUCT_BM};
   Operand b = {args.b, args.ldb, b_mn, args.cols,
                p.variant == kPair ? p.tile_n / 2 : p.tile_n};
@@ -588,9 +586,18 @@ hexir_status_t launch_product(Call &call, uint32_t op, uint32_t m, uint32_t n,
     a = {args.b, args.ldb, true, args.cols, HEXIR_PRODUCT_BM};
     b = x;
   }
+  // Guarded: by TMA what TMA can describe (forced: neither).
+  if (p.variant != kGuardedLoads)
+    args.tma_operands = 3;
+  else if (!(flags & HEXIR_LINEAR_FORCE_GUARDED) && args.depth)
+    args.tma_operands = (aligned_a ? 1u : 0u) | (aligned_b ? 2u : 0u);
   CUtensorMap map_a, map_b;
-  CUresult r = encode(&map_a, a, args.depth, args.is_f16 != 0);
-  if (r == CUDA_SUCCESS)
+  std::memset(&map_a, 0, sizeof(map_a));
+  std::memset(&map_b, 0, sizeof(map_b));
+  CUresult r = CUDA_SUCCESS;
+  if (args.tma_operands & 1u)
+    r = encode(&map_a, a, args.depth, args.is_f16 != 0);
+  if (r == CUDA_SUCCESS && (args.tma_operands & 2u))
     r = encode(&map_b, b, args.depth, args.is_f16 != 0);
   if (r != CUDA_SUCCESS)
     return fail(&call.error, cuda_message("cuTensorMapEncodeTiled", r));
@@ -601,9 +608,12 @@ hexir_status_t launch_product(Call &call, uint32_t op, uint32_t m, uint32_t n,
                   HEXIR_PAIR_THREADS, p.smem, stream, params,
                   "launch hexir_linear_16 pair", &call.error);
   }
-  CUfunction fn = p.variant == kSkinny ? call.lib->skinny : call.lib->single[op];
-  const char *what = p.variant == kSkinny ? "launch hexir_linear_16 skinny"
-                                          : "launch hexir_linear_16 single";
+  CUfunction fn = p.variant == kSkinny         ? call.lib->skinny
+                  : p.variant == kGuardedLoads ? call.lib->guarded[op]
+                                               : call.lib->single[op];
+  const char *what = p.variant == kSkinny         ? "launch hexir_linear_16 skinny"
+                     : p.variant == kGuardedLoads ? "launch hexir_linear_16 guarded"
+                                                  : "launch hexir_linear_16 single";
   return p.split > 1 ? launch_cluster(fn, grid, p.split, HEXIR_SINGLE_THREADS,
                                       p.smem, stream, params, what, &call.error)
                      : launch(fn, grid, 1, HEXIR_SINGLE_THREADS, p.smem, stream,
@@ -642,7 +652,8 @@ extern "C" hexir_status_t hexir_cuda_linear_plan(
   // Without a GPU: B200's 148 SMs.
   std::string error;
   DeviceState *dev = device_state(ordinal, &error);
-  const ProductPlan p = plan_product(op, m, n, k, aligned != 0, flags,
+  const ProductPlan p = plan_product(op, m, n, k, aligned != 0,
+                                     op != HEXIR_PRODUCT_WEIGHT_GRAD, flags,
                                      dev ? std::max(dev->sm_count, 2) : 148);
   if (!p.refusal.empty())
     return call.refuse("linear_plan: " + p.refusal);
