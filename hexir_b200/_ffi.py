@@ -59,6 +59,10 @@ def LINEAR_SPLIT(s: int) -> int:
     return (s & 0xFF) << 16
 
 
+def LINEAR_TILE(n: int) -> int:
+    return (n // 16 & 0xFF) << 24
+
+
 def MATMUL_SPLIT_K(s: int) -> int:
     return (s & 0xFF) << 16
 

@@ -595,109 +595,182 @@ __device__ __forceinline__ void product_pair(const CUtensorMap *map_a,
 // TMA would have written, and become the epilogue afterwards.  An operand
 // that TMA can describe still comes by TMA.
 
-// 8 elements of an operand's row that may start anywhere: the one or two
-// 16-byte blocks of memory they lie in, and where.
-struct Chunk {
-  uint4 lo, hi;
-  uint32_t shift;  // bytes into lo; 16: taken element by element, in place
-  uint32_t count;  // elements of the operand, the rest are 0
-};
-
-// The operand's memory, gaps between rows included: what a load may touch.
-struct Side {
-  const uint16_t *base;
-  uint64_t ld;
-  uintptr_t first, last;
-  uint32_t majors, minors;  // rows, elements of a row
-};
-__device__ __forceinline__ Side side_of(const void *p, uint64_t ld, uint32_t majors,
-                                        uint32_t minors) {
-  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
-  return {static_cast<const uint16_t *>(p), ld, at,
-          at + ((majors - 1) * ld + minors) * 2, majors, minors};
-}
-
-// Start the loads of 8 elements of row `major` from `minor` on.
-__device__ __forceinline__ void chunk_load(const Side &s, uint32_t major,
-                                           uint32_t minor, Chunk &c) {
-  c.lo = c.hi = make_uint4(0, 0, 0, 0);
-  c.shift = 0;
-  c.count = major < s.majors && minor < s.minors ? min(8u, s.minors - minor) : 0u;
-  if (!c.count)
-    return;
-  const uintptr_t at = reinterpret_cast<uintptr_t>(s.base + major * s.ld + minor);
-  const uintptr_t block = at & ~static_cast<uintptr_t>(15);
-  c.shift = static_cast<uint32_t>(at - block);
-  const bool two = c.shift + 2 * c.count > 16;
-  if (block >= s.first && block + (two ? 32 : 16) <= s.last) {
-    c.lo = __ldg(reinterpret_cast<const uint4 *>(block));
-    if (two)
-      c.hi = __ldg(reinterpret_cast<const uint4 *>(block + 16));
-    return;
-  }
-  // At the ends of the tensor.
-  const uint16_t *src = reinterpret_cast<const uint16_t *>(at);
-  uint32_t e[8];
-#pragma unroll
-  for (uint32_t i = 0; i < 8; ++i)
-    e[i] = src[min(i, c.count - 1)];
-  c.lo = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16,
-                    e[6] | e[7] << 16);
-  c.shift = 16;
-}
-
-// The 8 elements, those beyond the operand 0.
-__device__ __forceinline__ uint4 chunk_value(const Chunk &c) {
-  uint32_t w[8] = {c.lo.x, c.lo.y, c.lo.z, c.lo.w, c.hi.x, c.hi.y, c.hi.z, c.hi.w};
-  const uint32_t words = c.shift / 4;  // 4: in place
-  if (words & 2u) {
-#pragma unroll
-    for (int i = 0; i < 6; ++i)
-      w[i] = w[i + 2];
-  }
-  if (words & 1u) {
-#pragma unroll
-    for (int i = 0; i < 5; ++i)
-      w[i] = w[i + 1];
-  }
-  const uint32_t bits = (c.shift & 2u) * 8u;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w[i] = __funnelshift_r(w[i], w[i + 1], bits);
-    const uint32_t n = c.count > 2u * i ? c.count - 2u * i : 0u;
-    w[i] &= n >= 2 ? 0xFFFFFFFFu : (n == 1 ? 0xFFFFu : 0u);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 constexpr uint32_t kLoaders = 256;                // threads
 constexpr uint32_t kChunks = kBM * 8 / kLoaders;  // of an operand's tile, a thread
 
-// This thread's chunks of a 128 x 64 operand tile (side from `side0`, summed
-// index from k0).
+// The two 16-byte blocks of memory that each of a stage's chunks (8 elements of
+// a row, which may start anywhere) lies in, as loaded.
+struct Blocks {
+  uint4 lo[kChunks], hi[kChunks];
+  uint32_t apart;  // bit i: chunk i is to be taken element by element
+};
+
+// A load that stays where it is written.
+__device__ __forceinline__ uint4 load_now(uintptr_t at) {
+  uint4 w;
+  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+               : "l"(at)
+               : "memory");
+  return w;
+}
+
+// One thread's chunks of an operand's 128 x 64 tiles: chunk i is 8 elements of
+// 128-byte row (i * 32 + tid / 8) of the stage.  A thread's chunks, in every
+// tile, start at the same byte of a 16-byte block: they are 32 rows, 64
+// elements or 64 values of the sum apart, and each of these is a multiple of 16
+// bytes whatever the stride.
+//
+// A k tile wholly inside the operand along the sum, whose blocks lie wholly
+// inside the tensor's memory (from its first element to its last, gaps between
+// rows included), needs no checks but those along the side, which stay the
+// same for the whole launch: 25 instructions a chunk.  In the others (the last
+// k tile, and the first at the tensor's start) every chunk is checked, and the
+// few whose blocks reach outside the memory are taken element by element.  With
+// all checks on every chunk (126 instructions, few of them independent) a stage
+// took 3.6 us instead of 1.4.
 template <bool MN>
-__device__ __forceinline__ void operand_load(const Side &s, uint32_t side0,
-                                             uint32_t k0, uint32_t tid,
-                                             Chunk (&c)[kChunks]) {
+struct GuardedOperand {
+  uintptr_t at0;                // chunk 0 of k tile 0
+  uintptr_t low, high;          // the whole tile's first element and last
+  uintptr_t first, last, safe;  // the tensor; its first whole block
+  uint64_t step, row32;         // bytes to the next k tile, and 32 rows on
+  uint32_t sides, depth;        // extents along the tile's side and the sum
+  uint32_t side0, tid;
+  bool whole;                   // the tile lies inside the operand's side
+  uint32_t side_counts;         // 4 bits a chunk: elements inside the side
+
+  __device__ __forceinline__ GuardedOperand(const void *p, uint64_t ld,
+                                            uint32_t side_extent, uint32_t depth_,
+                                            uint32_t side0_, uint32_t tid_)
+      : sides(side_extent), depth(depth_), side0(side0_), tid(tid_) {
+    const uint32_t majors = MN ? depth : sides, minors = MN ? sides : depth;
+    first = reinterpret_cast<uintptr_t>(p);
+    last = majors ? first + ((majors - 1) * ld + minors) * 2 : first;
+    safe = (first + 15) & ~static_cast<uintptr_t>(15);
+    step = MN ? ld * (2 * kBK) : 2 * kBK;
+    row32 = ld * 64;
+    at0 = address(side_of(0), k_of(0), ld);
+    low = address(side0, 0, ld);
+    whole = side0 + kBM <= sides;
+    high = address(whole ? side0 + kBM - 1 : sides - 1, kBK - 1, ld);
+    side_counts = 0;
 #pragma unroll
-  for (uint32_t i = 0; i < kChunks; ++i) {
-    const uint32_t r = (i * kLoaders + tid) / 8, j = tid % 8;
-    if (MN)
-      chunk_load(s, k0 + r % 64, side0 + r / 64 * 64 + j * 8, c[i]);
-    else
-      chunk_load(s, side0 + r, k0 + j * 8, c[i]);
+    for (uint32_t i = 0; i < kChunks; ++i) {
+      const uint32_t s = side_of(i);
+      const uint32_t n = s >= sides ? 0u : (MN ? min(8u, sides - s) : 8u);
+      side_counts |= n << 4 * i;
+    }
   }
-}
-// Into the stage, as TMA's 128-byte swizzle would have it.
-__device__ __forceinline__ void operand_store(uint8_t *dst, uint32_t tid,
-                                              const Chunk (&c)[kChunks]) {
+  __device__ __forceinline__ uintptr_t address(uint32_t s, uint32_t k,
+                                               uint64_t ld) const {
+    return first + (MN ? k * ld + s : s * ld + k) * 2;
+  }
+  // Stage row of chunk i; its first element along the side and along the sum
+  // (of k tile 0); its address.
+  __device__ __forceinline__ uint32_t row(uint32_t i) const {
+    return (i * kLoaders + tid) / 8;
+  }
+  __device__ __forceinline__ uint32_t side_of(uint32_t i) const {
+    return side0 + (MN ? row(i) / 64 * 64 + tid % 8 * 8 : row(i));
+  }
+  __device__ __forceinline__ uint32_t k_of(uint32_t i) const {
+    return MN ? row(i) % 64 : tid % 8 * 8;
+  }
+  __device__ __forceinline__ uintptr_t where(uint32_t i, uint32_t kt) const {
+    return at0 + kt * step + (MN ? i % 2 * row32 + i / 2 * 128 : i * row32);
+  }
+  // Whether a k tile needs no checks (the same for the whole block).
+  __device__ __forceinline__ bool interior(uint32_t kt) const {
+    const uintptr_t lo = low + kt * step, hi = high + kt * step;
+    return (kt + 1) * kBK <= depth &&
+           (lo & ~static_cast<uintptr_t>(15)) >= first && hi + 32 <= last;
+  }
+  __device__ __forceinline__ uint32_t side_count(uint32_t i) const {
+    return side_counts >> 4 * i & 15u;
+  }
+  // Elements of chunk i that the operand has.
+  __device__ __forceinline__ uint32_t count(uint32_t i, uint32_t kt) const {
+    const uint32_t k = kt * kBK + k_of(i), n = side_count(i);
+    return k >= depth ? 0u : (MN ? n : min(n, depth - k));
+  }
+
+  __device__ __forceinline__ void load(uint32_t kt, Blocks &b) const {
+    b.apart = 0;
+    if (interior(kt)) {
 #pragma unroll
-  for (uint32_t i = 0; i < kChunks; ++i) {
-    const uint32_t r = (i * kLoaders + tid) / 8, j = tid % 8;
-    *reinterpret_cast<uint4 *>(dst + r * 128 + ((j ^ (r & 7u)) << 4)) =
-        chunk_value(c[i]);
+      for (uint32_t i = 0; i < kChunks; ++i) {
+        uintptr_t block = where(i, kt) & ~static_cast<uintptr_t>(15);
+        if (!whole)
+          block = side_count(i) ? block : safe;
+        b.lo[i] = load_now(block);
+        b.hi[i] = load_now(block + 16);
+      }
+      return;
+    }
+    const bool any = safe + 16 <= last;
+#pragma unroll
+    for (uint32_t i = 0; i < kChunks; ++i) {
+      const uint32_t n = count(i, kt);
+      const uintptr_t block = where(i, kt) & ~static_cast<uintptr_t>(15);
+      const bool two = (static_cast<uint32_t>(where(i, kt)) & 15u) + 2 * n > 16;
+      const bool inside = block >= first && block + (two ? 32 : 16) <= last;
+      b.apart |= static_cast<uint32_t>(n && !inside) << i;
+      const bool use = n && inside;
+      if (any) {
+        b.lo[i] = load_now(use ? block : safe);
+        b.hi[i] = load_now(use && two ? block + 16 : safe);
+      }
+    }
   }
-}
+  // Into the stage, as TMA's 128-byte swizzle would have it; elements beyond
+  // the operand are 0.
+  __device__ __forceinline__ void store(uint32_t kt, const Blocks &b,
+                                        uint8_t *dst) const {
+    const uint32_t shift = static_cast<uint32_t>(at0) & 15u;
+    const bool inner = interior(kt);
+    // The rows of a thread's chunks are 32 apart, so they swizzle alike.
+    dst += row(0) * 128 + ((tid % 8 ^ (row(0) & 7u)) << 4);
+#pragma unroll
+    for (uint32_t i = 0; i < kChunks; ++i) {
+      uint32_t w[8] = {b.lo[i].x, b.lo[i].y, b.lo[i].z, b.lo[i].w,
+                       b.hi[i].x, b.hi[i].y, b.hi[i].z, b.hi[i].w};
+#pragma unroll
+      for (int j = 0; j < 6; ++j)
+        w[j] = shift & 8u ? w[j + 2] : w[j];
+#pragma unroll
+      for (int j = 0; j < 5; ++j)
+        w[j] = shift & 4u ? w[j + 1] : w[j];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[j] = __funnelshift_r(w[j], w[j + 1], (shift & 2u) * 8u);
+      if (!inner || !whole) {
+        const uint32_t n = inner ? side_count(i) : count(i, kt);
+        if (b.apart >> i & 1u) {
+          const uint16_t *src = reinterpret_cast<const uint16_t *>(where(i, kt));
+          uint32_t e[8];
+#pragma unroll
+          for (uint32_t j = 0; j < 8; ++j)
+            e[j] = src[min(j, n - 1)];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            w[j] = e[2 * j] | e[2 * j + 1] << 16;
+        }
+        if (MN || !inner) {
+#pragma unroll
+          for (uint32_t j = 0; j < 4; ++j)
+            w[j] = n >= 2 * j + 2 ? w[j] : (n == 2 * j + 1 ? w[j] & 0xFFFFu : 0u);
+        } else {
+#pragma unroll
+          for (uint32_t j = 0; j < 4; ++j)
+            w[j] = n ? w[j] : 0u;
+        }
+      }
+      *reinterpret_cast<uint4 *>(dst + i * (kLoaders * 16)) =
+          make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+};
 
 template <int FORM, bool GUARDED, bool SWAP>
 __device__ __forceinline__ void product_single(const CUtensorMap *map_a,
@@ -730,7 +803,7 @@ __device__ __forceinline__ void product_single(const CUtensorMap *map_a,
     if (tma_b)
       prefetch_tensormap(map_b);
     for (uint32_t s = 0; s < stages; ++s) {
-      mbar_init(&full[s], (GUARDED ? kLoaders : 0u) + (tma_bytes ? 1u : 0u));
+      mbar_init(&full[s], (GUARDED ? kLoaders / 32 : 0u) + (tma_bytes ? 1u : 0u));
       mbar_init(&empty[s], 1);
     }
     mbar_init(&done, 1);
@@ -844,40 +917,41 @@ __device__ __forceinline__ void product_single(const CUtensorMap *map_a,
       // The loads of one stage are in flight while the last one's are shifted
       // into place and stored.
       const uint32_t tid = threadIdx.x - 64;
-      const Side side_a = A_MN ? side_of(p.a, p.lda, p.depth, p.rows)
-                               : side_of(p.a, p.lda, p.rows, p.depth);
-      const Side side_b = B_MN ? side_of(p.b, p.ldb, p.depth, p.cols)
-                               : side_of(p.b, p.ldb, p.cols, p.depth);
-      Chunk ca[2][kChunks], cb[2][kChunks];
+      const GuardedOperand<A_MN> a(p.a, p.lda, p.rows, p.depth, lane0, tid);
+      const GuardedOperand<B_MN> b(p.b, p.ldb, p.cols, p.depth, col0, tid);
+      Blocks ra[2], rb[2];
       RingPlace at;
-      auto load = [&](uint32_t kt, Chunk (&a)[kChunks], Chunk (&b)[kChunks]) {
+      auto load = [&](uint32_t kt, Blocks &xa, Blocks &xb) {
         if (kt < kt1) {
           if (!tma_a)
-            operand_load<A_MN>(side_a, lane0, kt * kBK, tid, a);
+            a.load(kt, xa);
           if (!tma_b)
-            operand_load<B_MN>(side_b, col0, kt * kBK, tid, b);
+            b.load(kt, xb);
         }
       };
-      auto settle = [&](const Chunk (&a)[kChunks], const Chunk (&b)[kChunks]) {
-        if (!mbar_wait_pipeline(&empty[at.stage], at.parity ^ 1u, p.timeout_ns))
+      auto settle = [&](uint32_t kt, const Blocks &xa, const Blocks &xb) {
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait_pipeline(&empty[at.stage],
+                                                        at.parity ^ 1u, p.timeout_ns)))
           return false;
         uint8_t *dst = ring + at.stage * stage_bytes;
         if (!tma_a)
-          operand_store(dst, tid, a);
+          a.store(kt, xa, dst);
         if (!tma_b)
-          operand_store(dst + kABytes, tid, b);
+          b.store(kt, xb, dst + kABytes);
         fence_async_smem();
-        mbar_arrive(&full[at.stage]);
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive(&full[at.stage]);
         at.next(stages);
         return true;
       };
-      load(kt0, ca[0], cb[0]);
+      load(kt0, ra[0], rb[0]);
       for (uint32_t kt = kt0; kt < kt1; kt += 2) {
-        load(kt + 1, ca[1], cb[1]);
-        if (!settle(ca[0], cb[0]))
+        load(kt + 1, ra[1], rb[1]);
+        if (!settle(kt, ra[0], rb[0]))
           break;
-        load(kt + 2, ca[0], cb[0]);
-        if (kt + 1 < kt1 && !settle(ca[1], cb[1]))
+        load(kt + 2, ra[0], rb[0]);
+        if (kt + 1 < kt1 && !settle(kt + 1, ra[1], rb[1]))
           break;
       }
       __syncwarp();

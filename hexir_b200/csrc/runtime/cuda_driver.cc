@@ -126,8 +126,12 @@ std::string cuda_message(const char *call, CUresult result) {
 
 ContextGuard::ContextGuard(CUcontext ctx) {
   const Driver &d = driver();
-  if (d.ok && ctx)
-    pushed_ = d.CtxPushCurrent(ctx) == CUDA_SUCCESS;
+  if (!d.ok || !ctx)
+    return;
+  CUcontext current = nullptr;  // nothing to do where it is current already
+  if (d.CtxGetCurrent(&current) == CUDA_SUCCESS && current == ctx)
+    return;
+  pushed_ = d.CtxPushCurrent(ctx) == CUDA_SUCCESS;
 }
 
 ContextGuard::~ContextGuard() {

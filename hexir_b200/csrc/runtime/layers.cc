@@ -376,9 +376,13 @@ std::string check_linear(const char *op, uint32_t dtype, uint32_t activation,
     return std::string(op) + ": no such elementwise activation " +
            std::to_string(activation);
   const uint32_t forces = flags & 0xF00u;
-  if ((flags & ~0xFF0F00u) || (forces & (forces - 1)))
+  if ((flags & ~0xFFFF0F00u) || (forces & (forces - 1)))
     return std::string(op) + ": unknown flags";
-  const uint32_t split = flags >> 16;
+  const uint32_t split = flags >> 16 & 0xFFu;
+  const uint32_t tile = flags >> 24 << 4;
+  if (tile && !((forces == HEXIR_LINEAR_FORCE_PAIR && (tile == 256 || tile == 128)) ||
+                (forces == HEXIR_LINEAR_FORCE_SINGLE && (tile == 128 || tile == 64))))
+    return std::string(op) + ": no such tile of the kernel asked for";
   if (split && split != 1 && split != 2 && split != 4 && split != 8)
     return std::string(op) + ": the split is 1, 2, 4 or 8";
   return std::string();
@@ -400,9 +404,46 @@ uint32_t stage_bytes(uint32_t tile_n) {
   return HEXIR_PRODUCT_BM * 128u + tile_n * 128u;
 }
 
+// Modelled microseconds of a product: a base, and per wave of tiles (of pairs,
+// or of clusters of `split` CTAs, resident at once) a fixed part and a part per
+// 64 of the summed index.  Fitted on B200 to 27 shapes of 65-8192 rows and
+// 256-8192 columns and depths, each in its three forms and every tile and
+// split (within 6-15 % of the measured times; what it chose took 0.6 % more
+// than the best, on average).  An epilogue that reads or stores through shared
+// memory (slots) costs more per tile and leaves one single CTA per SM.
+double modelled_us(uint32_t variant, uint32_t tile_n, uint32_t split, uint32_t rows,
+                   uint32_t cols, uint32_t k_tiles, bool slots, uint32_t guarded,
+                   uint32_t sms) {
+  struct Cost {
+    double k_tile, wave, base;
+  };
+  static constexpr Cost kPairCost[2][2] = {{{0.219, 1.9, 4.1}, {0.312, 3.2, 4.4}},
+                                           {{0.230, 3.1, 4.4}, {0.322, 5.2, 5.1}}};
+  static constexpr Cost kSingleCost[2][4] = {
+      {{0.224, 4.0, 0.8}, {0.227, 4.9, 1.1}, {0.264, 5.3, 1.9}, {0.381, 6.4, 3.4}},
+      {{0.272, 5.5, 1.0}, {0.283, 6.1, 1.3}, {0.311, 7.4, 0.6}, {0.631, 6.7, 2.8}}};
+  const uint32_t wide = tile_n >= (variant == kPair ? 256u : 128u) ? 1 : 0;
+  if (variant == kPair) {
+    const Cost &c = kPairCost[slots][wide];
+    const uint64_t tiles =
+        static_cast<uint64_t>(ceil_div(rows, 256)) * ceil_div(cols, tile_n);
+    const uint64_t waves = (tiles + sms / 2 - 1) / (sms / 2);
+    return c.base + waves * (k_tiles * c.k_tile + c.wave);
+  }
+  const Cost &c = kSingleCost[wide][split >= 8 ? 3 : split / 2];
+  const uint64_t ctas =
+      static_cast<uint64_t>(ceil_div(rows, 128)) * ceil_div(cols, tile_n) * split;
+  // Clusters are placed inside a GPC: 32 of 4 CTAs and 16 of 8 are resident.
+  const uint64_t resident = split >= 4 ? sms * 7 / 8 / split * split : sms;
+  const uint64_t waves = (ctas + resident - 1) / std::max<uint64_t>(resident, 1);
+  const double k_tile = c.k_tile + 0.8 * guarded;  // operands of guarded loads
+  return c.base + waves * (ceil_div(k_tiles, split) * k_tile + c.wave);
+}
+
 // slots: the epilogue reads or stores through shared memory.
+// guarded: operands that TMA cannot describe.
 ProductPlan plan_product(uint32_t op, uint32_t m, uint32_t n, uint32_t k,
-                         bool aligned, bool slots, uint32_t flags, uint32_t sms) {
+                         uint32_t guarded, bool slots, uint32_t flags, uint32_t sms) {
   // out [rows][cols], summed over depth.
   const uint32_t rows = op == HEXIR_PRODUCT_WEIGHT_GRAD ? k : m;
   const uint32_t cols = op == HEXIR_PRODUCT_INPUT_GRAD ? k : n;
@@ -410,9 +451,10 @@ ProductPlan plan_product(uint32_t op, uint32_t m, uint32_t n, uint32_t k,
                          : op == HEXIR_PRODUCT_INPUT_GRAD ? n
                                                           : m;
   const uint32_t k_tiles = ceil_div(depth, HEXIR_PRODUCT_BK);
-  const uint32_t forced_split = flags >> 16;
+  const uint32_t forced_split = flags >> 16 & 0xFFu;
+  const uint32_t forced_tile = flags >> 24 << 4;
   ProductPlan p;
-  const bool tma = aligned && depth > 0;
+  const bool tma = !guarded && depth > 0;
   const bool skinny = tma && op == HEXIR_PRODUCT_FORWARD && m <= 64;
   if (flags & HEXIR_LINEAR_FORCE_GUARDED) {
     p.variant = kGuardedLoads;
@@ -432,9 +474,9 @@ ProductPlan plan_product(uint32_t op, uint32_t m, uint32_t n, uint32_t k,
   if (!p.refusal.empty())
     return p;
 
-  const uint32_t max_split = std::max<uint32_t>(
-      1, k_tiles >= 32 ? 8 : (k_tiles >= 16 ? 4 : (k_tiles >= 8 ? 2 : 1)));
   if (p.variant == kSkinny) {
+    const uint32_t max_split = std::max<uint32_t>(
+        1, k_tiles >= 32 ? 8 : (k_tiles >= 16 ? 4 : (k_tiles >= 8 ? 2 : 1)));
     p.tile_n = (std::max<uint32_t>(m, 1) + 15) / 16 * 16;
     p.tiles_m = ceil_div(n, HEXIR_PRODUCT_BM);
     p.tiles_n = 1;
@@ -443,56 +485,39 @@ ProductPlan plan_product(uint32_t op, uint32_t m, uint32_t n, uint32_t k,
       p.split *= 2;
     p.tmem_cols = p.tile_n <= 32 ? 32 : 64;
   } else {
-    if (p.variant == 0 || p.variant == kPair) {
-      // Modelled cycles: waves of tiles, each its k-tiles plus a fill and an
-      // epilogue.
-      double best = 0;
-      uint32_t best_variant = 0, best_n = 0, best_split = 1;
-      for (uint32_t tile_n : {256u, 128u}) {
-        const uint64_t tiles = static_cast<uint64_t>(ceil_div(rows, 256)) *
-                               ceil_div(cols, tile_n);
-        const uint64_t waves = (tiles + sms / 2 - 1) / std::max<uint32_t>(sms / 2, 1);
-        const double t = waves * (k_tiles * 2.15 * tile_n + 600.0) + 3500.0;
-        if (best_variant == 0 || t < best) {
-          best = t;
-          best_variant = kPair;
-          best_n = tile_n;
-        }
+    // The kernel, tile and split of the least modelled time.
+    double best = 0;
+    uint32_t best_variant = 0;
+    auto consider = [&](uint32_t variant, uint32_t tile_n, uint32_t split) {
+      if ((p.variant && p.variant != variant) || (forced_tile && tile_n != forced_tile) ||
+          (forced_split && split != forced_split))
+        return;
+      const double t =
+          modelled_us(variant, tile_n, split, rows, cols, k_tiles, slots, guarded, sms);
+      if (best_variant == 0 || t < best) {
+        best = t;
+        best_variant = variant;
+        p.tile_n = tile_n;
+        p.split = split;
       }
-      if (p.variant == 0) {
-        for (uint32_t tile_n : {128u, 64u})
-          for (uint32_t split = 1; split <= max_split; split *= 2) {
-            const uint64_t ctas = static_cast<uint64_t>(ceil_div(rows, 128)) *
-                                  ceil_div(cols, tile_n) * split;
-            const uint64_t waves = (ctas + sms - 1) / sms;
-            const double t =
-                waves * (ceil_div(k_tiles, split) * (tile_n == 128 ? 300.0 : 220.0) +
-                         800.0) + 3000.0 + (split > 1 ? 1500.0 : 0.0);
-            if (t < best) {
-              best = t;
-              best_variant = kSingle;
-              best_n = tile_n;
-              best_split = split;
-            }
-          }
-      }
-      p.variant = best_variant;
-      p.tile_n = best_n;
-      p.split = best_split;
-    } else {
-      p.tile_n = 128;
-      const uint64_t tiles = static_cast<uint64_t>(ceil_div(rows, 128)) *
-                             ceil_div(cols, 128);
-      while (p.split < max_split && tiles * p.split * 2 <= sms)
-        p.split *= 2;
+    };
+    for (uint32_t tile_n : {256u, 128u})
+      consider(kPair, tile_n, 1);
+    const uint32_t single = p.variant == kGuardedLoads ? kGuardedLoads : kSingle;
+    for (uint32_t tile_n : {128u, 64u})
+      for (uint32_t split = 1; split <= 8; split *= 2)
+        if (split == 1 || split * 2 <= k_tiles || split == forced_split)
+          if (tile_n == 128 || single == kSingle)
+            consider(single, tile_n, split);
+    if (!best_variant) {
+      p.refusal = "CTA pairs do not split the sum";
+      return p;
     }
+    p.variant = best_variant;
     if (p.variant == kPair) {
       p.tiles_m = ceil_div(rows, 2 * HEXIR_PRODUCT_BM);
       p.tiles_n = ceil_div(cols, p.tile_n);
       p.smem = HEXIR_PAIR_SMEM_BYTES;
-      p.split = 1;
-      if (forced_split > 1)
-        p.refusal = "CTA pairs do not split the sum";
       return p;
     }
     p.tiles_m = ceil_div(rows, HEXIR_PRODUCT_BM);
@@ -551,14 +576,14 @@ hexir_status_t launch_product(Call &call, uint32_t op, uint32_t m, uint32_t n,
   const bool b_mn = op != HEXIR_PRODUCT_INPUT_GRAD;
   const bool aligned_a = rows16(args.a, args.lda, 2) && args.lda < 1ull << 39;
   const bool aligned_b = rows16(args.b, args.ldb, 2) && args.ldb < 1ull << 39;
-  const bool aligned = aligned_a && aligned_b;
   const uint32_t sms = static_cast<uint32_t>(std::max(call.dev->sm_count, 2));
   args.vec = rows16(args.out, args.ldo, 2) &&
              (!args.preact_out || rows16(args.preact_out, args.ldp, 2)) &&
              (!args.residual || rows16(args.residual, args.ldr, 2)) &&
              (!args.slope_at || rows16(args.slope_at, args.lds, 2));
   const bool slots = !args.vec || args.residual || args.slope_at;
-  const ProductPlan p = plan_product(op, m, n, k, aligned, slots, flags, sms);
+  const ProductPlan p = plan_product(
+      op, m, n, k, (aligned_a ? 0u : 1u) + (aligned_b ? 0u : 1u), slots, flags, sms);
   if (!p.refusal.empty())
     return fail(&call.error, "linear: " + p.refusal, HEXIR_ERROR_INVALID_ARGUMENT);
   const uint64_t tiles = static_cast<uint64_t>(p.tiles_m) * p.tiles_n;
@@ -652,7 +677,7 @@ extern "C" hexir_status_t hexir_cuda_linear_plan(
   // Without a GPU: B200's 148 SMs.
   std::string error;
   DeviceState *dev = device_state(ordinal, &error);
-  const ProductPlan p = plan_product(op, m, n, k, aligned != 0,
+  const ProductPlan p = plan_product(op, m, n, k, aligned ? 0u : 2u,
                                      op != HEXIR_PRODUCT_WEIGHT_GRAD, flags,
                                      dev ? std::max(dev->sm_count, 2) : 148);
   if (!p.refusal.empty())

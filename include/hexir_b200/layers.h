@@ -51,13 +51,15 @@ extern "C" {
 #define HEXIR_ACTIVATION_RELU 3u /* x > 0 ? x : 0 */
 
 /* flags of the linear calls, for tests: which kernel runs (the call is
- * refused where that kernel cannot run it), and over how many CTAs of a
- * cluster the sum is split (1, 2, 4 or 8; single, skinny, guarded). */
+ * refused where that kernel cannot run it), over how many CTAs of a cluster
+ * the sum is split (1, 2, 4 or 8; single, skinny, guarded), and the columns
+ * of a tile (256 or 128 of a pair, 128 or 64 of a single CTA). */
 #define HEXIR_LINEAR_FORCE_PAIR 0x100u    /* CTA pairs, 256-row tiles */
 #define HEXIR_LINEAR_FORCE_SINGLE 0x200u  /* one CTA, 128-row tiles */
 #define HEXIR_LINEAR_FORCE_SKINNY 0x400u  /* tokens as tile columns, m <= 64 */
 #define HEXIR_LINEAR_FORCE_GUARDED 0x800u /* bounds-checked loads */
 #define HEXIR_LINEAR_SPLIT(S) (((uint32_t)(S) & 0xFFu) << 16)
+#define HEXIR_LINEAR_TILE(N) (((uint32_t)(N) / 16u & 0xFFu) << 24)
 
 /* y = act(z) + residual with z = x . w + bias, for x [m][k], w [k][n],
  * bias [n], residual, preact and y [m][n], all of one type, bf16 or f16.

@@ -41,7 +41,8 @@ def test_linear_refusals():
     assert linear(flags=0x1) == BAD
     assert linear(flags=_ffi.LINEAR_FORCE_PAIR | _ffi.LINEAR_FORCE_SINGLE) == BAD
     assert linear(flags=_ffi.LINEAR_SPLIT(3)) == BAD
-    assert linear(flags=1 << 24) == BAD
+    assert linear(flags=1 << 24) == BAD                 # no tile of 16 columns
+    assert linear(flags=_ffi.LINEAR_FORCE_SINGLE | _ffi.LINEAR_TILE(256)) == BAD
     assert linear(m=0xFFFFFFFF) == BAD
     with pytest.raises(ValueError):
         hx.cuda_linear(0, P, P, P, 4, 8, 16, "bf16", "softmax")
