@@ -17,6 +17,7 @@
 #include "activation_f32.cuh"
 #include "common.cuh"
 #include "layers_abi.h"
+#include "two.cuh"
 
 using namespace hexir;
 
@@ -63,62 +64,6 @@ struct Pack {
   static constexpr int kN = 16 / sizeof(T);
   uint4 w;
 };
-
-// Two values that are computed side by side: sm_100 adds and multiplies two
-// f32 with one instruction.
-template <typename R>
-struct Two {
-  R x, y;
-};
-__device__ __forceinline__ uint64_t both(const Two<float> &a) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
-  return r;
-}
-__device__ __forceinline__ Two<float> apart(uint64_t r) {
-  Two<float> a;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(r));
-  return a;
-}
-__device__ __forceinline__ Two<float> add(const Two<float> &a, const Two<float> &b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(both(a)), "l"(both(b)));
-  return apart(r);
-}
-__device__ __forceinline__ Two<float> mul(const Two<float> &a, const Two<float> &b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(both(a)), "l"(both(b)));
-  return apart(r);
-}
-__device__ __forceinline__ Two<float> fma(const Two<float> &a, const Two<float> &b,
-                                          const Two<float> &c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(r)
-      : "l"(both(a)), "l"(both(b)), "l"(both(c)));
-  return apart(r);
-}
-__device__ __forceinline__ Two<double> add(const Two<double> &a,
-                                           const Two<double> &b) {
-  return {a.x + b.x, a.y + b.y};
-}
-__device__ __forceinline__ Two<double> mul(const Two<double> &a,
-                                           const Two<double> &b) {
-  return {a.x * b.x, a.y * b.y};
-}
-__device__ __forceinline__ Two<double> fma(const Two<double> &a,
-                                           const Two<double> &b,
-                                           const Two<double> &c) {
-  return {::fma(a.x, b.x, c.x), ::fma(a.y, b.y, c.y)};
-}
-template <typename R>
-__device__ __forceinline__ R half_of(const Two<R> &a, int j) {
-  return j % 2 ? a.y : a.x;
-}
-template <typename R>
-__device__ __forceinline__ Two<R> twice(R v) {
-  return {v, v};
-}
 
 __device__ __forceinline__ void widen_pack(const Pack<double> &p,
                                            Two<double> (&f)[1]) {
@@ -442,6 +387,8 @@ __device__ __forceinline__ void norm_rows(const hexir_layer_norm_args_t &p) {
   __shared__ R slots[2][kRows * TH / 32];
   extern __shared__ uint4 copies[];  // gamma and beta as this block's rows lie
   const uint32_t tid = threadIdx.x % TH, group = threadIdx.x / TH;
+  griddep_wait();  // nothing global is read or written before this
+  griddep_launch_dependents();
   const R n = static_cast<R>(p.cols), inv_n = R(1) / n;
   const T *x_rows = static_cast<const T *>(p.x);
   const T *gamma = static_cast<const T *>(p.gamma);
@@ -562,6 +509,8 @@ template <typename T>
 __device__ __forceinline__ void norm_rows_wide(const hexir_layer_norm_args_t &p) {
   typedef real_t<T> R;
   constexpr int TH = 512;
+  griddep_wait();
+  griddep_launch_dependents();
   __shared__ R slots[2][2 * TH / 32];
   const R n = static_cast<R>(p.cols), inv_n = R(1) / n;
   const T *gamma = static_cast<const T *>(p.gamma);
@@ -630,6 +579,8 @@ __device__ __forceinline__ void norm_grad_rows(
   __shared__ R slots[2][kRows * 2 * TH / 32];
   extern __shared__ uint4 ring[];  // [DEPTH][tensors][kPacks][kBlock]
   const uint32_t tid = threadIdx.x % TH, group = threadIdx.x / TH;
+  griddep_wait();  // nothing global is read or written before this
+  griddep_launch_dependents();
   const R inv_n = R(1) / static_cast<R>(p.cols);
   const T *x_rows = static_cast<const T *>(p.x);
   const T *dy_rows = static_cast<const T *>(p.dy);
@@ -846,6 +797,8 @@ __device__ __forceinline__ void norm_grad_rows_wide(
     const hexir_layer_norm_grad_args_t &p) {
   typedef real_t<T> R;
   constexpr int TH = 512;
+  griddep_wait();
+  griddep_launch_dependents();
   __shared__ R slots[2][2 * TH / 32];
   const R inv_n = R(1) / static_cast<R>(p.cols);
   const T *gamma = static_cast<const T *>(p.gamma);
@@ -882,6 +835,8 @@ __device__ __forceinline__ void norm_grad_columns(
     const hexir_layer_norm_grad_args_t &p) {
   typedef real_t<T> R;
   __shared__ R joined[8][32][2];
+  griddep_wait();
+  griddep_launch_dependents();
   const uint64_t c = (uint64_t)blockIdx.x * 32 + threadIdx.x % 32;
   const uint32_t lane = threadIdx.x / 32;
   R dgamma = 0, dbeta = 0;
@@ -940,6 +895,7 @@ __device__ __forceinline__ void norm_grad_join(
     const hexir_layer_norm_grad_args_t &p) {
   T *out = static_cast<T *>(blockIdx.y ? p.dbeta : p.dgamma);
   griddep_wait();
+  griddep_launch_dependents();
   if (out)
     column_sums<T>(static_cast<const real_t<T> *>(p.partials) +
                        (uint64_t)blockIdx.y * p.cols,
@@ -948,10 +904,14 @@ __device__ __forceinline__ void norm_grad_join(
 
 // dz = dy * act'(z) and the sums of dz over the rows of part blockIdx.y, for
 // 256 columns: a warp covers a row's 256 columns (8 per lane), the 8 warps
-// take the part's rows in turn.
+// take the part's rows in turn, 4 of them in flight at a time (with one, the
+// loads' latency left HBM at 0.4 of its rate).
 template <typename T>
 __device__ __forceinline__ void output_grad(const hexir_output_grad_args_t &p) {
+  constexpr uint32_t kRows = 4;
   __shared__ float joined[8][256];
+  griddep_wait();  // nothing global is read or written before this
+  griddep_launch_dependents();
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const uint32_t col = blockIdx.x * 256 + lane * 8;
   const uint32_t left = col < p.n ? p.n - col : 0;
@@ -963,46 +923,55 @@ __device__ __forceinline__ void output_grad(const hexir_output_grad_args_t &p) {
   const uint32_t rows = row0 < p.m ? min(p.rows_per_part, p.m - row0) : 0;
   Two<float> sum[4] = {{0, 0}, {0, 0}, {0, 0}, {0, 0}};
   if (left) {
-    for (uint32_t i = warp; i < rows; i += 8) {
-      const uint64_t row = row0 + i;
-      Pack<T> g, at;
-      if (whole) {
-        g.w = __ldcs(reinterpret_cast<const uint4 *>(dy + row * p.lddy));
-        if (p.activation)
-          at.w = __ldcs(reinterpret_cast<const uint4 *>(z + row * p.ldp));
-      } else {
-        T e[8], f[8];
+    for (uint32_t i = warp; i < rows; i += 8 * kRows) {
+      Pack<T> g[kRows], at[kRows];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool in = static_cast<uint32_t>(j) < left;
-          e[j] = in ? dy[row * p.lddy + j] : narrow<T>(0.0f);
-          f[j] = in && p.activation ? z[row * p.ldp + j] : narrow<T>(0.0f);
-        }
-        g.w = *reinterpret_cast<const uint4 *>(e);
-        at.w = *reinterpret_cast<const uint4 *>(f);
-      }
-      Two<float> v[4], s[4];
-      if (p.activation) {
-        widen_pack(g, v);
-        widen_pack(at, s);
-        slope_f32(p.activation, reinterpret_cast<const float(&)[8]>(s),
-                  reinterpret_cast<float(&)[8]>(v));
-        narrow_pack(v, g);
-      }
-      if (p.dz) {
+      for (uint32_t r = 0; r < kRows; ++r) {
+        // Rows past the part are read as its last and not used.
+        const uint64_t row = row0 + min(i + 8 * r, rows - 1);
         if (whole) {
-          *reinterpret_cast<uint4 *>(dz + row * p.lddz) = g.w;
+          g[r].w = __ldcs(reinterpret_cast<const uint4 *>(dy + row * p.lddy));
+          if (p.activation)
+            at[r].w = __ldcs(reinterpret_cast<const uint4 *>(z + row * p.ldp));
         } else {
+          T e[8], f[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (static_cast<uint32_t>(j) < left)
-              dz[row * p.lddz + j] = pack_get(g, j);
+          for (uint32_t j = 0; j < 8; ++j) {
+            e[j] = dy[row * p.lddy + min(j, left - 1)];
+            f[j] = p.activation ? z[row * p.ldp + min(j, left - 1)] : e[j];
+          }
+          g[r].w = *reinterpret_cast<const uint4 *>(e);
+          at[r].w = *reinterpret_cast<const uint4 *>(f);
         }
       }
-      widen_pack(g, v);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        sum[j] = add(sum[j], v[j]);
+      for (uint32_t r = 0; r < kRows; ++r) {
+        if (i + 8 * r >= rows)
+          break;
+        const uint64_t row = row0 + i + 8 * r;
+        Two<float> v[4], s[4];
+        if (p.activation) {
+          widen_pack(g[r], v);
+          widen_pack(at[r], s);
+          slope_f32(p.activation, reinterpret_cast<const float(&)[8]>(s),
+                    reinterpret_cast<float(&)[8]>(v));
+          narrow_pack(v, g[r]);
+        }
+        if (p.dz) {
+          if (whole) {
+            *reinterpret_cast<uint4 *>(dz + row * p.lddz) = g[r].w;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (static_cast<uint32_t>(j) < left)
+                dz[row * p.lddz + j] = pack_get(g[r], j);
+          }
+        }
+        widen_pack(g[r], v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          sum[j] = add(sum[j], v[j]);
+      }
     }
   }
   if (!p.partials)
@@ -1024,6 +993,7 @@ template <typename T>
 __device__ __forceinline__ void output_grad_join(
     const hexir_output_grad_args_t &p) {
   griddep_wait();
+  griddep_launch_dependents();
   column_sums<T>(p.partials, p.n, p.parts, static_cast<T *>(p.dbias), p.n);
 }
 

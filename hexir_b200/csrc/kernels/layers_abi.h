@@ -53,7 +53,7 @@ typedef struct {
   uint32_t rows, cols, depth;
   uint32_t activation;
   uint32_t is_f16;        /* f16, else bf16 */
-  uint32_t vec;           /* epilogue rows 32-byte aligned (8 per 16 bytes) */
+  uint32_t vec;           /* epilogue rows on 16- (1) or 32-byte (2) boundaries */
   uint32_t tiles_m, tiles_n, group_m;
   uint32_t tile_n;        /* columns of a tile */
   uint32_t k_tiles;       /* ceil(depth / BK) */

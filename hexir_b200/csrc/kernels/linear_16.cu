@@ -91,7 +91,8 @@ __device__ __forceinline__ uint4 pack8(const float *v, bool is_f16) {
 // tile 26 k cycles long.
 //
 // Rows on 16-byte boundaries (p.vec) are fetched and stored a lane's row at a
-// time, 16 bytes an access; any others by the whole warp, two rows of 16
+// time, 16 bytes an access (stored 32 where they are on 32-byte boundaries, so
+// that each access fills a sector); any others by the whole warp, two rows of 16
 // elements an access, through the slots.
 
 constexpr uint32_t kSlotBytes = 1024u;  // 32 rows x 32 bytes
@@ -200,6 +201,15 @@ __device__ __forceinline__ void store_block(const Args &p, void *base, uint64_t 
     if (row >= p.rows)
       return;
     dst += row * ld + col;
+    if (p.vec == 2 && col + 16 <= p.cols) {
+      const uint4 lo = pack8(v, f16), hi = pack8(v + 8, f16);
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(
+                       dst),
+                   "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w), "r"(hi.x),
+                   "r"(hi.y), "r"(hi.z), "r"(hi.w)
+                   : "memory");
+      return;
+    }
 #pragma unroll
     for (uint32_t h = 0; h < 2; ++h) {
       const uint32_t c = col + 8 * h;
@@ -441,6 +451,8 @@ __device__ __forceinline__ void product_pair(const CUtensorMap *map_a,
   cluster_sync();  // the peer's barriers exist before anything arrives there
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  griddep_wait();  // nothing global is read or written before this
+  griddep_launch_dependents();
 
   const uint32_t tiles = p.tiles_m * p.tiles_n;
   const uint32_t first = blockIdx.x / 2, step = gridDim.x / 2;
@@ -815,6 +827,8 @@ __device__ __forceinline__ void product_single(const CUtensorMap *map_a,
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  griddep_wait();  // nothing global is read or written before this
+  griddep_launch_dependents();
 
   // The tile, and this CTA's share of its sum.
   uint32_t tm, tn;

@@ -87,19 +87,27 @@ hexir_status_t launch(CUfunction fn, unsigned gx, unsigned gy, unsigned bx,
 // placed while that kernel's last CTAs run, and the kernel itself waits
 // (griddepcontrol.wait) for that kernel's completion before reading.  Hides
 // the launch gap between a GEMM and its split-K reduction or stream-K
-// fix-up.  A plain launch where the driver has no cuLaunchKernelEx.
+// fix-up, and between one layer kernel and the next.  A launch without it
+// where the driver has no cuLaunchKernelEx.
 hexir_status_t launch_after(CUfunction fn, unsigned gx, unsigned gy,
                             unsigned bx, CUstream stream, void **params,
-                            const char *what, std::string *error) {
+                            const char *what, std::string *error, unsigned smem,
+                            unsigned cluster) {
   const Driver &d = driver();
   if (!d.LaunchKernelEx)
-    return launch(fn, gx, gy, bx, 0, stream, params, what, error);
+    return cluster > 1 ? launch_cluster(fn, gx, cluster, bx, smem, stream, params,
+                                        what, error)
+                       : launch(fn, gx, gy, bx, smem, stream, params, what, error);
   if (fault_hit(FaultSite::Launch))
     return fail(error, std::string(what) + ": injected fault (HEXIR_FAULT)");
-  CUlaunchAttribute attr;
-  std::memset(&attr, 0, sizeof(attr));
-  attr.id = CU_LAUNCH_ATTRIBUTE_PROGRAMMATIC_STREAM_SERIALIZATION;
-  attr.value.programmaticStreamSerializationAllowed = 1;
+  CUlaunchAttribute attrs[2];
+  std::memset(attrs, 0, sizeof(attrs));
+  attrs[0].id = CU_LAUNCH_ATTRIBUTE_PROGRAMMATIC_STREAM_SERIALIZATION;
+  attrs[0].value.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = CU_LAUNCH_ATTRIBUTE_CLUSTER_DIMENSION;
+  attrs[1].value.clusterDim.x = cluster;
+  attrs[1].value.clusterDim.y = 1;
+  attrs[1].value.clusterDim.z = 1;
   CUlaunchConfig cfg;
   std::memset(&cfg, 0, sizeof(cfg));
   cfg.gridDimX = gx;
@@ -108,9 +116,10 @@ hexir_status_t launch_after(CUfunction fn, unsigned gx, unsigned gy,
   cfg.blockDimX = bx;
   cfg.blockDimY = 1;
   cfg.blockDimZ = 1;
+  cfg.sharedMemBytes = smem;
   cfg.hStream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   const CUresult r = d.LaunchKernelEx(&cfg, fn, params, nullptr);
   if (r != CUDA_SUCCESS)
     return fail(error, cuda_message(what, r));

@@ -161,7 +161,8 @@ hexir_status_t launch(CUfunction fn, unsigned gx, unsigned gy, unsigned bx,
                       const char *what, std::string *error);
 hexir_status_t launch_after(CUfunction fn, unsigned gx, unsigned gy,
                             unsigned bx, CUstream stream, void **params,
-                            const char *what, std::string *error);
+                            const char *what, std::string *error,
+                            unsigned smem = 0, unsigned cluster = 1);
 hexir_status_t launch_cluster(CUfunction fn, unsigned gx, unsigned cluster,
                               unsigned bx, unsigned smem, CUstream stream,
                               void **params, const char *what,

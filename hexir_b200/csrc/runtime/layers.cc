@@ -196,7 +196,8 @@ struct LayersLib {
   Sized norm[4][kMaxShapes] = {}, norm_grad[4][kMaxShapes] = {};
   CUfunction norm_wide[4] = {}, norm_grad_wide[4] = {},
              norm_grad_columns[4] = {}, norm_grad_join[4] = {};
-  CUfunction output_grad[4] = {}, output_grad_join[4] = {};
+  Sized output_grad[4] = {};
+  CUfunction output_grad_join[4] = {};
 };
 
 CUdeviceptr layers_error_word(const LayersLib *lib) { return lib->error_word; }
@@ -253,7 +254,7 @@ LayersLib *layers_library(DeviceState *dev, std::string *error) {
     get(&lib->norm_grad_join[t], grad + "_join");
     if (t >= static_cast<int>(HEXIR_DTYPE_BF16)) {
       const std::string out = std::string("hexir_linear_output_grad_") + kDtypeName[t];
-      get(&lib->output_grad[t], out);
+      get(&lib->output_grad[t].fn, out);
       get(&lib->output_grad_join[t], out + "_join");
     }
   }
@@ -274,6 +275,9 @@ LayersLib *layers_library(DeviceState *dev, std::string *error) {
     r = d.FuncSetAttribute(lib->skinny,
                            CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES,
                            kSmemLimit);
+  for (int t = HEXIR_DTYPE_BF16; t < 4 && r == CUDA_SUCCESS; ++t)
+    r = d.FuncGetAttribute(&lib->output_grad[t].registers, CU_FUNC_ATTRIBUTE_NUM_REGS,
+                           lib->output_grad[t].fn);
   for (int t = 0; t < 4; ++t)
     for (int s = 0; s < kMaxShapes; ++s)
       for (LayersLib::Sized *k : {&lib->norm[t][s], &lib->norm_grad[t][s]}) {
@@ -581,6 +585,9 @@ hexir_status_t launch_product(Call &call, uint32_t op, uint32_t m, uint32_t n,
              (!args.preact_out || rows16(args.preact_out, args.ldp, 2)) &&
              (!args.residual || rows16(args.residual, args.ldr, 2)) &&
              (!args.slope_at || rows16(args.slope_at, args.lds, 2));
+  if (args.vec && !off(args.out, 32) && args.ldo % 16 == 0 &&
+      (!args.preact_out || (!off(args.preact_out, 32) && args.ldp % 16 == 0)))
+    args.vec = 2;
   const bool slots = !args.vec || args.residual || args.slope_at;
   const ProductPlan p = plan_product(
       op, m, n, k, (aligned_a ? 0u : 1u) + (aligned_b ? 0u : 1u), slots, flags, sms);
@@ -629,9 +636,9 @@ hexir_status_t launch_product(Call &call, uint32_t op, uint32_t m, uint32_t n,
   void *params[] = {&map_a, &map_b, &args};
   if (p.variant == kPair) {
     const uint64_t pairs = std::min<uint64_t>(tiles, sms / 2);
-    return launch(call.lib->pair[op], static_cast<unsigned>(2 * pairs), 1,
-                  HEXIR_PAIR_THREADS, p.smem, stream, params,
-                  "launch hexir_linear_16 pair", &call.error);
+    return launch_after(call.lib->pair[op], static_cast<unsigned>(2 * pairs), 1,
+                        HEXIR_PAIR_THREADS, stream, params,
+                        "launch hexir_linear_16 pair", &call.error, p.smem);
   }
   CUfunction fn = p.variant == kSkinny         ? call.lib->skinny
                   : p.variant == kGuardedLoads ? call.lib->guarded[op]
@@ -639,10 +646,8 @@ hexir_status_t launch_product(Call &call, uint32_t op, uint32_t m, uint32_t n,
   const char *what = p.variant == kSkinny         ? "launch hexir_linear_16 skinny"
                      : p.variant == kGuardedLoads ? "launch hexir_linear_16 guarded"
                                                   : "launch hexir_linear_16 single";
-  return p.split > 1 ? launch_cluster(fn, grid, p.split, HEXIR_SINGLE_THREADS,
-                                      p.smem, stream, params, what, &call.error)
-                     : launch(fn, grid, 1, HEXIR_SINGLE_THREADS, p.smem, stream,
-                              params, what, &call.error);
+  return launch_after(fn, grid, 1, HEXIR_SINGLE_THREADS, stream, params, what,
+                      &call.error, p.smem, p.split);
 }
 
 // TMA coordinates are signed 32-bit numbers.
@@ -883,15 +888,18 @@ extern "C" hexir_status_t hexir_cuda_linear_output_grad(
   const uint32_t gx = ceil_div(c.n, 256);
   hexir_status_t st = HEXIR_OK;
   if (c.m) {
-    const uint64_t sms = static_cast<uint64_t>(std::max(call.dev->sm_count, 1));
-    const uint64_t want = std::max<uint64_t>(1, sms * 8 / gx);
+    // One wave of blocks where the rows allow it.
+    const LayersLib::Sized &kernel = call.lib->output_grad[c.dtype];
+    const uint64_t resident = static_cast<uint64_t>(std::max(call.dev->sm_count, 1)) *
+                              blocks_per_sm(kernel.registers, 256, 8192);
+    const uint64_t want = std::max<uint64_t>(1, resident / gx);
     args.parts = static_cast<uint32_t>(std::min<uint64_t>(
         {want, static_cast<uint64_t>(ceil_div(c.m, 32)), uint64_t(kSumsPerColumn)}));
     args.rows_per_part = ceil_div(c.m, args.parts);
     args.parts = ceil_div(c.m, args.rows_per_part);
     void *params[] = {&args};
-    st = launch(call.lib->output_grad[c.dtype], gx, args.parts, 256, 0, s, params,
-                "launch hexir_linear_output_grad", &call.error);
+    st = launch_after(kernel.fn, gx, args.parts, 256, s, params,
+                      "launch hexir_linear_output_grad", &call.error);
   }
   if (st == HEXIR_OK && c.dbias) {
     void *params[] = {&args};
@@ -955,10 +963,10 @@ extern "C" hexir_status_t hexir_cuda_layer_norm(int ordinal,
   const int kind = kind_of(c.dtype);
   const int at = norm_shape(kNorm[kind], c.cols, size, layout);
   if (at < 0)
-    return call.finish(launch(call.lib->norm_wide[c.dtype],
-                              static_cast<unsigned>(std::min<uint64_t>(c.rows, 1u << 24)),
-                              1, 512, 0, s, params, "launch hexir_layer_norm wide",
-                              &call.error));
+    return call.finish(
+        launch_after(call.lib->norm_wide[c.dtype],
+                     static_cast<unsigned>(std::min<uint64_t>(c.rows, 1u << 24)), 1, 512,
+                     s, params, "launch hexir_layer_norm wide", &call.error));
   const NormShape &shape = kNorm[kind][at];
   const LayersLib::Sized &kernel = call.lib->norm[c.dtype][at];
   // Shifted rows: gamma and beta as the rows lie.
@@ -967,10 +975,9 @@ extern "C" hexir_status_t hexir_cuda_layer_norm(int ordinal,
   const uint64_t resident =
       static_cast<uint64_t>(std::max(call.dev->sm_count, 1)) *
       blocks_per_sm(kernel.registers, shape.block(), copies);
-  return call.finish(
-      launch(kernel.fn,
-             static_cast<unsigned>(norm_blocks(shape, layout, c.rows, resident)), 1,
-             shape.block(), copies, s, params, "launch hexir_layer_norm", &call.error));
+  return call.finish(launch_after(
+      kernel.fn, static_cast<unsigned>(norm_blocks(shape, layout, c.rows, resident)), 1,
+      shape.block(), s, params, "launch hexir_layer_norm", &call.error, copies));
 }
 
 extern "C" hexir_status_t hexir_cuda_layer_norm_grad(
@@ -1050,21 +1057,22 @@ extern "C" hexir_status_t hexir_cuda_layer_norm_grad(
         sms * blocks_per_sm(kernel.registers, shape.block(), ring), kSumsPerColumn / 2);
     args.parts =
         static_cast<uint32_t>(norm_blocks(shape, layout, c.rows, resident));
-    st = launch(kernel.fn, args.parts, 1, shape.block(), ring, s, params,
-                "launch hexir_layer_norm_grad", &call.error);
+    st = launch_after(kernel.fn, args.parts, 1, shape.block(), s, params,
+                      "launch hexir_layer_norm_grad", &call.error, ring);
   } else if (c.rows) {
     // The column sums first: dx may be dy.
     if (sums) {
       args.parts = static_cast<uint32_t>(
           std::min<uint64_t>(kSumsPerColumn / 2, (c.rows + 63) / 64));
-      st = launch(call.lib->norm_grad_columns[c.dtype], ceil_div(c.cols, 32),
-                  args.parts, 256, 0, s, params,
-                  "launch hexir_layer_norm_grad columns", &call.error);
+      st = launch_after(call.lib->norm_grad_columns[c.dtype], ceil_div(c.cols, 32),
+                        args.parts, 256, s, params,
+                        "launch hexir_layer_norm_grad columns", &call.error);
     }
     if (st == HEXIR_OK && c.dx)
-      st = launch(call.lib->norm_grad_wide[c.dtype],
-                  static_cast<unsigned>(std::min<uint64_t>(c.rows, 1u << 24)), 1, 512,
-                  0, s, params, "launch hexir_layer_norm_grad wide", &call.error);
+      st = launch_after(call.lib->norm_grad_wide[c.dtype],
+                        static_cast<unsigned>(std::min<uint64_t>(c.rows, 1u << 24)), 1,
+                        512, s, params, "launch hexir_layer_norm_grad wide",
+                        &call.error);
   }
   if (st == HEXIR_OK && sums)
     st = launch_after(call.lib->norm_grad_join[c.dtype], ceil_div(c.cols, 32), 2,
