@@ -315,3 +315,447 @@ def test_linear_output_grad(m, n, dtype, act, pad, shift):
     assert bool((work[size:] == 0xA5).all()), "a write behind the workspace"
     assert_within(dz.numpy(), *ref.output_grad(dy.numpy(), z.numpy(), act, dtype), "dz")
     assert_within(dbias.numpy()[0], *ref.column_sums(dz.numpy(), dtype), "dbias")
+
+
+# ------------------------------------------------- forms, streams and captures
+
+def forced(m, n, k):
+    """Every kernel that can run the shape, by flags."""
+    out = [0, GUARDED | _ffi.LINEAR_SPLIT(1), GUARDED | _ffi.LINEAR_SPLIT(2)]
+    if aligned8(n, k):
+        out += [SINGLE | _ffi.LINEAR_TILE(64) | _ffi.LINEAR_SPLIT(1),
+                SINGLE | _ffi.LINEAR_TILE(64) | _ffi.LINEAR_SPLIT(4),
+                PAIR | _ffi.LINEAR_TILE(128), PAIR | _ffi.LINEAR_TILE(256)]
+        if m <= 64:
+            out += [SKINNY | _ffi.LINEAR_SPLIT(1), SKINNY | _ffi.LINEAR_SPLIT(4)]
+    return out
+
+
+@pytest.mark.parametrize("m,n,k", [(48, 200, 304), (300, 520, 136), (70, 99, 65)])
+def test_every_kernel_in_place_over_the_residual(m, n, k):
+    """y may be the residual's own buffer; every tile width too."""
+    rng = np.random.default_rng(k)
+    x = inputs(rng, m, k, "bf16")
+    w = inputs(rng, k, n, "bf16", scale=1 / np.sqrt(k))
+    start = normal(rng, (m, n))
+    for flags in forced(m, n, k):
+        y = Tensor(m, n, "bf16", data=start)
+        r = y.numpy()
+        hx.cuda_linear(0, x.ptr, w.ptr, y.ptr, m, n, k, "bf16", "gelu",
+                       residual=y.ptr, flags=flags, stream=stream())
+        sync()
+        y.check_frame()
+        want = ref.linear(x.numpy(), w.numpy(), None, "gelu", r, "bf16")
+        assert_within(y.numpy(), want[0], want[1], f"flags {flags:#x}")
+
+
+@pytest.mark.parametrize("ldx,ldw,ldy", [(136, 257, 256), (135, 256, 256),
+                                         (136, 256, 257), (129, 250, 249)])
+def test_operands_by_tma_and_by_guarded_loads_mix(ldx, ldw, ldy):
+    """One operand on 16-byte rows, the other (or the output) off them."""
+    m, n, k = 200, 249, 129
+    rng = np.random.default_rng(ldx + ldw)
+    x = Tensor(m, k, "f16", ldx - k, data=normal(rng, (m, k)))
+    w = Tensor(k, n, "f16", ldw - n, data=normal(rng, (k, n), 1 / np.sqrt(k)))
+    r = Tensor(m, n, "f16", ldy - n, data=normal(rng, (m, n)))
+    y = Tensor(m, n, "f16", ldy - n)
+    hx.cuda_linear(0, x.ptr, w.ptr, y.ptr, m, n, k, "f16", "swish", residual=r.ptr,
+                   ldx=ldx, ldw=ldw, ldy=ldy, ldr=ldy, stream=stream())
+    sync()
+    y.check_frame()
+    want = ref.linear(x.numpy(), w.numpy(), None, "swish", r.numpy(), "f16")
+    assert_within(y.numpy(), want[0], want[1], "y")
+
+
+def test_empty_sums_and_empty_outputs():
+    b, r = inputs(np.random.default_rng(1), 1, 40, "bf16"), \
+        inputs(np.random.default_rng(2), 7, 40, "bf16")
+    y, z = Tensor(7, 40, "bf16"), Tensor(7, 40, "bf16")
+    hx.cuda_linear(0, 0, 0, y.ptr, 7, 40, 0, "bf16", "tanh", bias=b.ptr,
+                   residual=r.ptr, preact=z.ptr, stream=stream())
+    sync()
+    want = ref.linear(np.zeros((7, 0)), np.zeros((0, 40)), b.numpy()[0], "tanh",
+                      r.numpy(), "bf16")
+    assert_within(y.numpy(), want[0], want[1], "y")
+    assert_within(z.numpy(), want[2], want[3], "z")
+    y.check_frame()
+    # No output, or none of it: nothing is written, nothing is needed.
+    for m, n in ((0, 40), (7, 0), (0, 0)):
+        hx.cuda_linear(0, 0, 0, 0, m, n, 16, stream=stream())
+        hx.cuda_linear_output_grad(0, 0, m, n, "bf16", "gelu", stream=stream())
+    hx.cuda_linear_input_grad(0, 0, 0, 0, 0, 8, 8, stream=stream())
+    # Sums over no rows are zeros.
+    dw, db = Tensor(24, 40, "f16"), Tensor(1, 40, "f16")
+    work = torch.empty(hx.grad_workspace_bytes(40, "f16"), device="cuda",
+                       dtype=torch.uint8)
+    hx.cuda_linear_weight_grad(0, 0, 0, dw.ptr, 0, 40, 24, "f16", stream=stream())
+    hx.cuda_linear_output_grad(0, 0, 0, 40, "f16", dbias=db.ptr,
+                               workspace=work.data_ptr(),
+                               workspace_bytes=work.numel(), stream=stream())
+    # dz . w^T over no columns of dz is the residual.
+    dx, res = Tensor(5, 24, "f16"), inputs(np.random.default_rng(3), 5, 24, "f16")
+    hx.cuda_linear_input_grad(0, 0, 0, dx.ptr, 5, 0, 24, "f16", residual=res.ptr,
+                              stream=stream())
+    dg, dbeta = Tensor(1, 40, "f64"), Tensor(1, 40, "f64")
+    work64 = torch.empty(hx.grad_workspace_bytes(40, "f64"), device="cuda",
+                         dtype=torch.uint8)
+    hx.cuda_layer_norm(0, 0, 0, 0, 40, "f32", stream=stream())
+    hx.cuda_layer_norm_grad(0, 0, 0, 0, 0, 0, 0, 40, "f64", dgamma=dg.ptr,
+                            dbeta=dbeta.ptr, workspace=work64.data_ptr(),
+                            workspace_bytes=work64.numel(), stream=stream())
+    sync()
+    for t in (dw, db, dg, dbeta):
+        t.check_frame()
+        assert not t.numpy().any()
+    assert np.array_equal(dx.numpy(), res.numpy())
+
+
+@pytest.mark.parametrize("dtype,cols", [("bf16", 768), ("bf16", 1001), ("f32", 4096),
+                                        ("f64", 1025), ("f16", 20000)])
+def test_layer_norm_grad_in_place(dtype, cols):
+    """dx may be dy, or the residual; sums alone and dx alone."""
+    rng = np.random.default_rng(cols)
+    rows, wide = 37, "f64" if dtype == "f64" else "f32"
+    x = inputs(rng, rows, cols, dtype)
+    mean = Tensor(1, rows, wide, data=x.numpy().mean(1))
+    rstd = Tensor(1, rows, wide, data=1 / np.sqrt(x.numpy().var(1) + 1e-3))
+    dy0, r0 = normal(rng, (rows, cols)), normal(rng, (rows, cols))
+    size = hx.grad_workspace_bytes(cols, dtype)
+    work = torch.empty(size, device="cuda", dtype=torch.uint8)
+    for place in ("dy", "residual", "sums"):
+        dy, r = Tensor(rows, cols, dtype, data=dy0), Tensor(rows, cols, dtype, data=r0)
+        want = ref.layer_norm_grad(dy.numpy(), x.numpy(), mean.numpy()[0],
+                                   rstd.numpy()[0], None, r.numpy(), dtype)
+        dx = {"dy": dy, "residual": r, "sums": None}[place]
+        dgamma, dbeta = Tensor(1, cols, dtype), Tensor(1, cols, dtype)
+        hx.cuda_layer_norm_grad(0, dy.ptr, x.ptr, mean.ptr, rstd.ptr,
+                                dx.ptr if dx else 0, rows, cols, dtype,
+                                dgamma=dgamma.ptr, dbeta=dbeta.ptr, residual=r.ptr,
+                                workspace=work.data_ptr(), workspace_bytes=size,
+                                stream=stream())
+        sync()
+        assert_within(dgamma.numpy()[0], *want[1], "dgamma")
+        assert_within(dbeta.numpy()[0], *want[2], "dbeta")
+        if dx:
+            assert_within(dx.numpy(), *want[0], "dx")
+        else:
+            dx = Tensor(rows, cols, dtype)
+            hx.cuda_layer_norm_grad(0, dy.ptr, x.ptr, mean.ptr, rstd.ptr, dx.ptr, rows,
+                                    cols, dtype, residual=r.ptr, stream=stream())
+            sync()
+            assert_within(dx.numpy(), *want[0], "dx")
+
+
+def test_output_grad_in_place_and_alone():
+    rng = np.random.default_rng(9)
+    z, dy = inputs(rng, 90, 72, "bf16"), inputs(rng, 90, 72, "bf16")
+    want = ref.output_grad(dy.numpy(), z.numpy(), "swish", "bf16")
+    hx.cuda_linear_output_grad(0, dy.ptr, 90, 72, "bf16", "swish", preact=z.ptr,
+                               dz=dy.ptr, stream=stream())
+    sync()
+    dy.check_frame()
+    assert_within(dy.numpy(), *want, "dz")
+
+
+@pytest.mark.parametrize("flags", [0, GUARDED, PAIR, SKINNY])
+def test_a_nan_stays_in_its_row_and_column(flags):
+    m, n, k = 40, 264, 200
+    rng = np.random.default_rng(4)
+    x = torch.tensor(normal(rng, (m, k)), device="cuda").bfloat16()
+    w = torch.tensor(normal(rng, (k, n)), device="cuda").bfloat16()
+    x[3, 7], x[20, k - 1] = float("nan"), float("inf")
+    w[k - 1, 100] = float("nan")
+    y = torch.empty(m, n, device="cuda", dtype=torch.bfloat16)
+    hx.cuda_linear(0, x.data_ptr(), w.data_ptr(), y.data_ptr(), m, n, k,
+                   flags=flags, stream=stream())
+    sync()
+    fine = torch.ones(m, n, dtype=torch.bool, device="cuda")
+    fine[3], fine[20], fine[:, 100] = False, False, False
+    assert bool(y[fine].isfinite().all())
+    assert bool(y[3].isnan().all()) and bool(y[:, 100].isnan().all())
+    assert not bool(y[20].isfinite().any())
+
+
+def test_offsets_beyond_32_bits():
+    """Row strides that put the last rows past 2^32 elements."""
+    rows, cols, ld = 4, 1000, 1_500_000_064
+    big = torch.empty(3 * ld + cols, device="cuda", dtype=torch.bfloat16)
+    x = big.as_strided((rows, cols), (ld, 1))
+    x.copy_(torch.randn(rows, cols, device="cuda"))
+    y = torch.empty(rows, cols, device="cuda", dtype=torch.bfloat16)
+    hx.cuda_layer_norm(0, x.data_ptr(), y.data_ptr(), rows, cols, "bf16", ldx=ld,
+                       stream=stream())
+    sync()
+    (want, bound), _, _ = ref.layer_norm(x.double().cpu().numpy(), None, None, 1e-5,
+                                         "bf16")
+    assert_within(y.double().cpu().numpy(), want, bound, "y")
+    w = torch.randn(cols, 64, device="cuda").bfloat16()
+    out = torch.empty(rows, 64, device="cuda", dtype=torch.bfloat16)
+    res = x[:, :64]
+    for flags in (0, GUARDED, SINGLE, PAIR):
+        hx.cuda_linear(0, x.data_ptr(), w.data_ptr(), out.data_ptr(), rows, 64, cols,
+                       "bf16", residual=res.data_ptr(), ldx=ld, ldr=ld, flags=flags,
+                       stream=stream())
+        sync()
+        want = ref.linear(x.double().cpu().numpy(), w.double().cpu().numpy(), None,
+                          "none", res.double().cpu().numpy(), "bf16")
+        assert_within(out.double().cpu().numpy(), want[0], want[1], f"y {flags:#x}")
+
+
+def feed_forward(rows, cols, hidden, dtype="bf16", seed=0):
+    """A pre-norm feed-forward block's tensors, as torch tensors."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    t = TORCH[dtype]
+
+    def normal_(*shape, std=1.0, mean=0.0):
+        return (torch.randn(*shape, generator=g, device="cuda") * std + mean).to(t)
+    return {"x": normal_(rows, cols), "gamma": normal_(cols, std=0.1, mean=1.0),
+            "beta": normal_(cols, std=0.1),
+            "w1": normal_(cols, hidden, std=cols ** -0.5), "b1": normal_(hidden, std=0.1),
+            "w2": normal_(hidden, cols, std=hidden ** -0.5), "b2": normal_(cols, std=0.1),
+            "dy": normal_(rows, cols)}
+
+
+class Block:
+    """y = x + w2 . gelu(w1 . norm(x) + b1) + b2 and all its gradients through the
+    layer calls, in buffers made once."""
+
+    def __init__(self, rows, cols, hidden, dtype="bf16"):
+        self.shape, self.dtype = (rows, cols, hidden), dtype
+        t = TORCH[dtype]
+
+        def empty(*shape, of=t):
+            return torch.empty(*shape, device="cuda", dtype=of)
+        self.h, self.dh, self.dx = (empty(rows, cols) for _ in range(3))
+        self.a, self.z, self.dz = (empty(rows, hidden) for _ in range(3))
+        self.y = empty(rows, cols)
+        self.mean, self.rstd = (empty(rows, of=torch.float32) for _ in range(2))
+        self.dw1, self.dw2 = empty(cols, hidden), empty(hidden, cols)
+        self.db1, self.db2 = empty(hidden), empty(cols)
+        self.dgamma, self.dbeta = empty(cols), empty(cols)
+        self.work = empty(hx.grad_workspace_bytes(max(cols, hidden), dtype),
+                          of=torch.uint8)
+
+    def forward(self, p, on):
+        r, c, f = self.shape
+        hx.cuda_layer_norm(0, p["x"].data_ptr(), self.h.data_ptr(), r, c, self.dtype,
+                           gamma=p["gamma"].data_ptr(), beta=p["beta"].data_ptr(),
+                           mean=self.mean.data_ptr(), rstd=self.rstd.data_ptr(),
+                           stream=on)
+        hx.cuda_linear(0, self.h.data_ptr(), p["w1"].data_ptr(), self.a.data_ptr(), r, f,
+                       c, self.dtype, "gelu", bias=p["b1"].data_ptr(),
+                       preact=self.z.data_ptr(), stream=on)
+        hx.cuda_linear(0, self.a.data_ptr(), p["w2"].data_ptr(), self.y.data_ptr(), r, c,
+                       f, self.dtype, bias=p["b2"].data_ptr(),
+                       residual=p["x"].data_ptr(), stream=on)
+
+    def backward(self, p, on):
+        r, c, f = self.shape
+        dt, work = self.dtype, self.work
+        dy = p["dy"].data_ptr()
+        hx.cuda_linear_output_grad(0, dy, r, c, dt, dbias=self.db2.data_ptr(),
+                                   workspace=work.data_ptr(),
+                                   workspace_bytes=work.numel(), stream=on)
+        hx.cuda_linear_weight_grad(0, self.a.data_ptr(), dy, self.dw2.data_ptr(), r, c,
+                                   f, dt, stream=on)
+        hx.cuda_linear_input_grad(0, dy, p["w2"].data_ptr(), self.dz.data_ptr(), r, c, f,
+                                  dt, "gelu", preact=self.z.data_ptr(), stream=on)
+        hx.cuda_linear_output_grad(0, self.dz.data_ptr(), r, f, dt,
+                                   dbias=self.db1.data_ptr(), workspace=work.data_ptr(),
+                                   workspace_bytes=work.numel(), stream=on)
+        hx.cuda_linear_weight_grad(0, self.h.data_ptr(), self.dz.data_ptr(),
+                                   self.dw1.data_ptr(), r, f, c, dt, stream=on)
+        hx.cuda_linear_input_grad(0, self.dz.data_ptr(), p["w1"].data_ptr(),
+                                  self.dh.data_ptr(), r, f, c, dt, stream=on)
+        hx.cuda_layer_norm_grad(0, self.dh.data_ptr(), p["x"].data_ptr(),
+                                self.mean.data_ptr(), self.rstd.data_ptr(),
+                                self.dx.data_ptr(), r, c, dt,
+                                gamma=p["gamma"].data_ptr(),
+                                dgamma=self.dgamma.data_ptr(),
+                                dbeta=self.dbeta.data_ptr(), residual=dy,
+                                workspace=work.data_ptr(),
+                                workspace_bytes=work.numel(), stream=on)
+
+    def outputs(self):
+        return {"y": self.y, "dx": self.dx, "dw1": self.dw1, "dw2": self.dw2,
+                "db1": self.db1, "db2": self.db2, "dgamma": self.dgamma,
+                "dbeta": self.dbeta}
+
+
+def block_in_64_bits(p):
+    q = {k: v.double().requires_grad_(k != "dy") for k, v in p.items()}
+    x = q["x"]
+    mean = x.mean(1, keepdim=True)
+    h = (x - mean) / torch.sqrt(((x - mean) ** 2).mean(1, keepdim=True) + 1e-5)
+    z = (h * q["gamma"] + q["beta"]) @ q["w1"] + q["b1"]
+    a = 0.5 * z * torch.erfc(-z * 0.5 ** 0.5)
+    y = x + a @ q["w2"] + q["b2"]
+    y.backward(q["dy"])
+    names = {"dx": "x", "dw1": "w1", "dw2": "w2", "db1": "b1", "db2": "b2",
+             "dgamma": "gamma", "dbeta": "beta"}
+    return {"y": y.detach(), **{k: q[v].grad for k, v in names.items()}}
+
+
+def worst(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("rows,cols,hidden", [(300, 256, 1024), (1, 512, 2048),
+                                              (77, 130, 515)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_a_feed_forward_block_forward_and_backward(rows, cols, hidden, dtype):
+    """The calls in a row, as a training step has them.  Every stage stores its
+    result in the type, off by a half step at most: the relative error of an
+    output is that of the 7 roundings before it, each carried on by products
+    whose norms the next stage's stay within, so 7 half steps and one for
+    their second order bound it in the 2-norm (the roundings are far from
+    aligned; the products' f32 sums are 2^-15 below them)."""
+    p = feed_forward(rows, cols, hidden, dtype)
+    block = Block(rows, cols, hidden, dtype)
+    block.forward(p, stream())
+    block.backward(p, stream())
+    sync()
+    want = block_in_64_bits(p)
+    for name, got in block.outputs().items():
+        assert worst(got, want[name]) <= 8 * ref.HALF[dtype], name
+
+
+def test_a_captured_training_step_replays():
+    """A block's step captured into a graph: replays follow its inputs, equal
+    the same calls made eagerly bit for bit, and two graphs with workspaces of
+    their own run side by side on two streams."""
+    shape = (260, 256, 1000)
+    eager = Block(*shape)
+    p = feed_forward(*shape, seed=1)
+    eager.forward(p, stream())       # also: the device code is loaded
+    eager.backward(p, stream())
+    sync()
+    steps = []
+    for seed in (1, 2):
+        mine, block, on = feed_forward(*shape, seed=seed), Block(*shape), torch.cuda.Stream()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=on):
+            s = torch.cuda.current_stream().cuda_stream
+            block.forward(mine, s)
+            block.backward(mine, s)
+        steps.append((mine, block, on, graph))
+    for seeds in ((1, 2), (5, 6), (7, 8)):
+        for (mine, block, on, graph), seed in zip(steps, seeds):
+            fresh = feed_forward(*shape, seed=seed)
+            torch.cuda.synchronize()
+            for k in mine:
+                mine[k].copy_(fresh[k])
+        torch.cuda.synchronize()
+        for mine, block, on, graph in steps:
+            with torch.cuda.stream(on):
+                graph.replay()
+                graph.replay()
+        sync()
+        for mine, block, on, graph in steps:
+            eager.forward(mine, stream())
+            eager.backward(mine, stream())
+            sync()
+            for (name, got), want in zip(block.outputs().items(),
+                                         eager.outputs().values()):
+                assert torch.equal(got, want), name
+
+
+def test_streams_and_threads_at_once():
+    """The same step from four threads, each on a stream of its own: every
+    result has the bits of the step made alone."""
+    import threading
+    shape = (200, 256, 600)
+    inputs_ = [feed_forward(*shape, seed=s) for s in range(4)]
+    alone = []
+    for p in inputs_:
+        b = Block(*shape)
+        b.forward(p, stream())
+        b.backward(p, stream())
+        sync()
+        alone.append(b)
+    blocks, streams = [Block(*shape) for _ in range(4)], [torch.cuda.Stream()
+                                                         for _ in range(4)]
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(i):
+        try:
+            for _ in range(10):
+                blocks[i].forward(inputs_[i], streams[i].cuda_stream)
+                blocks[i].backward(inputs_[i], streams[i].cuda_stream)
+        except Exception as err:  # noqa: BLE001 - reported below
+            errors.append(err)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    sync()
+    assert not errors
+    for a, b in zip(alone, blocks):
+        for (name, got), want in zip(b.outputs().items(), a.outputs().values()):
+            assert torch.equal(got, want), name
+
+
+def test_results_repeat_bit_for_bit():
+    """Sums have a fixed order: the same call twice, in between other work."""
+    p = feed_forward(513, 768, 1030, seed=3)
+    first, second = Block(513, 768, 1030), Block(513, 768, 1030)
+    for b in (first, second):
+        b.forward(p, stream())
+        b.backward(p, stream())
+        Block(5, 64, 64).forward(feed_forward(5, 64, 64), stream())
+    sync()
+    for (name, a), b in zip(first.outputs().items(), second.outputs().values()):
+        assert torch.equal(a, b), name
+
+
+def test_gradients_against_differences():
+    """The block's gradient along a direction, against a difference of its loss
+    sum(y dy) in 64 bits: the gradient is in f16 (2^-11 a rounding, 8 of them),
+    the difference is off by its step's square (1e-8 of the third derivative)."""
+    p = feed_forward(20, 64, 128, "f16", seed=4)
+    block = Block(20, 64, 128, "f16")
+    block.forward(p, stream())
+    block.backward(p, stream())
+    sync()
+
+    def loss(q):
+        x = q["x"]
+        mean = x.mean(1, keepdim=True)
+        h = (x - mean) / torch.sqrt(((x - mean) ** 2).mean(1, keepdim=True) + 1e-5)
+        z = (h * q["gamma"] + q["beta"]) @ q["w1"] + q["b1"]
+        return ((x + 0.5 * z * torch.erfc(-z * 0.5 ** 0.5) @ q["w2"] + q["b2"])
+                * q["dy"]).sum()
+    names = {"x": "dx", "w1": "dw1", "w2": "dw2", "b1": "db1", "b2": "db2",
+             "gamma": "dgamma", "beta": "dbeta"}
+    q = {k: v.double() for k, v in p.items()}
+    for name, grad in names.items():
+        g = getattr(block, grad).double()
+        along = g / g.norm()  # the gradient's own direction: no cancellation
+        step = 1e-4
+        up, down = dict(q), dict(q)
+        up[name], down[name] = q[name] + step * along, q[name] - step * along
+        slope = float((loss(up) - loss(down)) / (2 * step))
+        assert abs(slope - float(g.norm())) <= (8 * ref.HALF["f16"] + 1e-6) * abs(slope)
+
+
+def test_launch_faults_are_reported_and_leave_nothing_behind():
+    x = torch.randn(64, 64, device="cuda").bfloat16()
+    y = torch.empty_like(x)
+    before = hx.launch_count()
+    hx.fault_configure("launch:1")
+    try:
+        with pytest.raises(_ffi.HexirError) as err:
+            hx.cuda_linear(0, x.data_ptr(), x.data_ptr(), y.data_ptr(), 64, 64, 64,
+                           stream=stream())
+        assert err.value.status == _ffi.ERROR_DEVICE
+    finally:
+        hx.fault_configure("")
+    hx.cuda_linear(0, x.data_ptr(), x.data_ptr(), y.data_ptr(), 64, 64, 64,
+                   stream=stream())
+    sync()
+    assert hx.launch_count() == before + 1
+    with pytest.raises(_ffi.HexirError) as err:
+        hx.cuda_layer_norm(99, x.data_ptr(), y.data_ptr(), 64, 64, "bf16")
+    assert err.value.status == _ffi.ERROR_DEVICE

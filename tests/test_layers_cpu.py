@@ -155,3 +155,17 @@ def test_plans():
     with pytest.raises(_ffi.HexirError):
         hx.linear_plan("forward", 5, 8, 8, aligned=False,
                        flags=_ffi.LINEAR_FORCE_PAIR)
+
+
+def test_the_reference_slopes_are_the_activations_derivatives():
+    """The formulas the GPU tests use, against central differences in 64 bits
+    (off by the step's square, 1e-10, times a third derivative below 3, and by
+    rounding, 1e-16 / 1e-5); corners, where the slope jumps, left out."""
+    import numpy as np
+    from tests import layers_reference as ref
+    z = np.linspace(-9, 9, 2001)
+    z = z[np.abs(z) > 1e-4]
+    h = 1e-5
+    for name in ref.ACTS:
+        diff = (ref.act(name, z + h) - ref.act(name, z - h)) / (2 * h)
+        assert np.abs(diff - ref.slope(name, z)).max() < 1e-9, name
