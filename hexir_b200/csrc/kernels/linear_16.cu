@@ -628,95 +628,87 @@ __device__ __forceinline__ uint4 load_now(uintptr_t at) {
 }
 
 // One thread's chunks of an operand's 128 x 64 tiles: chunk i is 8 elements of
-// 128-byte row (i * 32 + tid / 8) of the stage.  A thread's chunks, in every
-// tile, start at the same byte of a 16-byte block: they are 32 rows, 64
-// elements or 64 values of the sum apart, and each of these is a multiple of 16
-// bytes whatever the stride.
+// 128-byte row (i * 32 + lane / 8 * 8 + warp) of the stage.  The chunks of a
+// warp, in every tile, start at the same byte of a 16-byte block: their rows are
+// 8 apart (and 64 elements or 64 values of the sum), and each of these is a
+// multiple of 16 bytes whatever the stride.  So the words to shift by are the
+// warp's, taken by a branch, and only halves are shifted by instructions.
 //
 // A k tile wholly inside the operand along the sum, whose blocks lie wholly
 // inside the tensor's memory (from its first element to its last, gaps between
-// rows included), needs no checks but those along the side, which stay the
-// same for the whole launch: 25 instructions a chunk.  In the others (the last
-// k tile, and the first at the tensor's start) every chunk is checked, and the
-// few whose blocks reach outside the memory are taken element by element.  With
-// all checks on every chunk (126 instructions, few of them independent) a stage
-// took 3.6 us instead of 1.4.
+// rows included), needs no checks: chunks beyond the operand's side read the
+// side's first instead, and what they leave in the sums is never stored.  In
+// the others (the last k tile, and the first at the tensor's start) every chunk
+// is checked, and the few whose blocks reach outside the memory are taken
+// element by element.
 template <bool MN>
 struct GuardedOperand {
-  uintptr_t at0;                // chunk 0 of k tile 0
-  uintptr_t low, high;          // the whole tile's first element and last
+  uintptr_t block[kChunks];     // of k tile 0
   uintptr_t first, last, safe;  // the tensor; its first whole block
-  uint64_t step, row32;         // bytes to the next k tile, and 32 rows on
-  uint32_t sides, depth;        // extents along the tile's side and the sum
-  uint32_t side0, tid;
-  bool whole;                   // the tile lies inside the operand's side
+  uint64_t step;                // bytes to the next k tile
+  uint32_t depth;
+  uint32_t shift;               // bytes into a block
+  uint32_t inner0, inner1;      // the k tiles that need no checks
   uint32_t side_counts;         // 4 bits a chunk: elements inside the side
+  uint32_t k0, dst0;            // chunk 0: of the sum; byte in the stage
 
   __device__ __forceinline__ GuardedOperand(const void *p, uint64_t ld,
-                                            uint32_t side_extent, uint32_t depth_,
-                                            uint32_t side0_, uint32_t tid_)
-      : sides(side_extent), depth(depth_), side0(side0_), tid(tid_) {
+                                            uint32_t sides, uint32_t depth_,
+                                            uint32_t side0, uint32_t warp,
+                                            uint32_t lane)
+      : depth(depth_) {
     const uint32_t majors = MN ? depth : sides, minors = MN ? sides : depth;
+    const uint32_t row0 = lane / 8 * 8 + warp, column = lane % 8 * 8;
     first = reinterpret_cast<uintptr_t>(p);
     last = majors ? first + ((majors - 1) * ld + minors) * 2 : first;
     safe = (first + 15) & ~static_cast<uintptr_t>(15);
     step = MN ? ld * (2 * kBK) : 2 * kBK;
-    row32 = ld * 64;
-    at0 = address(side_of(0), k_of(0), ld);
-    low = address(side0, 0, ld);
-    whole = side0 + kBM <= sides;
-    high = address(whole ? side0 + kBM - 1 : sides - 1, kBK - 1, ld);
+    k0 = MN ? row0 : column;
+    dst0 = row0 * 128 + ((lane % 8 ^ warp) << 4);
+    // Within a warp the major index is the same but for multiples of 8.
+    shift = static_cast<uint32_t>(
+                first + ((MN ? 0 : side0) + static_cast<uint64_t>(warp)) * ld * 2) & 15u;
     side_counts = 0;
 #pragma unroll
     for (uint32_t i = 0; i < kChunks; ++i) {
-      const uint32_t s = side_of(i);
+      const uint32_t row = i * 32 + row0;
+      uint32_t s = side0 + (MN ? row / 64 * 64 + column : row);
       const uint32_t n = s >= sides ? 0u : (MN ? min(8u, sides - s) : 8u);
       side_counts |= n << 4 * i;
+      s = n ? s : side0;
+      block[i] = address(s, MN ? row % 64 : column, ld) & ~static_cast<uintptr_t>(15);
     }
+    // Blocks from the tile's first to 32 bytes past the start of its last
+    // element's lie in the memory.
+    const uintptr_t low = address(side0, 0, ld) & ~static_cast<uintptr_t>(15);
+    const uintptr_t high = address(min(side0 + kBM, sides) - 1, kBK - 1, ld) + 32;
+    inner0 = low >= first ? 0 : 1;
+    inner1 = depth / kBK;
+    while (inner1 > inner0 && high + (inner1 - 1) * step > last)
+      --inner1;
   }
   __device__ __forceinline__ uintptr_t address(uint32_t s, uint32_t k,
                                                uint64_t ld) const {
     return first + (MN ? k * ld + s : s * ld + k) * 2;
   }
-  // Stage row of chunk i; its first element along the side and along the sum
-  // (of k tile 0); its address.
-  __device__ __forceinline__ uint32_t row(uint32_t i) const {
-    return (i * kLoaders + tid) / 8;
-  }
-  __device__ __forceinline__ uint32_t side_of(uint32_t i) const {
-    return side0 + (MN ? row(i) / 64 * 64 + tid % 8 * 8 : row(i));
-  }
-  __device__ __forceinline__ uint32_t k_of(uint32_t i) const {
-    return MN ? row(i) % 64 : tid % 8 * 8;
-  }
-  __device__ __forceinline__ uintptr_t where(uint32_t i, uint32_t kt) const {
-    return at0 + kt * step + (MN ? i % 2 * row32 + i / 2 * 128 : i * row32);
-  }
-  // Whether a k tile needs no checks (the same for the whole block).
   __device__ __forceinline__ bool interior(uint32_t kt) const {
-    const uintptr_t lo = low + kt * step, hi = high + kt * step;
-    return (kt + 1) * kBK <= depth &&
-           (lo & ~static_cast<uintptr_t>(15)) >= first && hi + 32 <= last;
-  }
-  __device__ __forceinline__ uint32_t side_count(uint32_t i) const {
-    return side_counts >> 4 * i & 15u;
+    return kt >= inner0 && kt < inner1;
   }
   // Elements of chunk i that the operand has.
   __device__ __forceinline__ uint32_t count(uint32_t i, uint32_t kt) const {
-    const uint32_t k = kt * kBK + k_of(i), n = side_count(i);
+    const uint32_t k = kt * kBK + k0 + (MN ? i % 2 * 32 : 0);
+    const uint32_t n = side_counts >> 4 * i & 15u;
     return k >= depth ? 0u : (MN ? n : min(n, depth - k));
   }
 
   __device__ __forceinline__ void load(uint32_t kt, Blocks &b) const {
     b.apart = 0;
+    const uint64_t offset = kt * step;
     if (interior(kt)) {
 #pragma unroll
       for (uint32_t i = 0; i < kChunks; ++i) {
-        uintptr_t block = where(i, kt) & ~static_cast<uintptr_t>(15);
-        if (!whole)
-          block = side_count(i) ? block : safe;
-        b.lo[i] = load_now(block);
-        b.hi[i] = load_now(block + 16);
+        b.lo[i] = load_now(block[i] + offset);
+        b.hi[i] = load_now(block[i] + offset + 16);
       }
       return;
     }
@@ -724,25 +716,53 @@ struct GuardedOperand {
 #pragma unroll
     for (uint32_t i = 0; i < kChunks; ++i) {
       const uint32_t n = count(i, kt);
-      const uintptr_t block = where(i, kt) & ~static_cast<uintptr_t>(15);
-      const bool two = (static_cast<uint32_t>(where(i, kt)) & 15u) + 2 * n > 16;
-      const bool inside = block >= first && block + (two ? 32 : 16) <= last;
+      const uintptr_t at = block[i] + offset;
+      const bool two = shift + 2 * n > 16;
+      const bool inside = at >= first && at + (two ? 32 : 16) <= last;
       b.apart |= static_cast<uint32_t>(n && !inside) << i;
       const bool use = n && inside;
       if (any) {
-        b.lo[i] = load_now(use ? block : safe);
-        b.hi[i] = load_now(use && two ? block + 16 : safe);
+        b.lo[i] = load_now(use ? at : safe);
+        b.hi[i] = load_now(use && two ? at + 16 : safe);
       }
     }
   }
+  // The chunks, WORDS 32-bit words and possibly a half into their blocks.
+  template <int WORDS>
+  __device__ __forceinline__ void store_inner(const Blocks &b, uint8_t *dst) const {
+    const uint32_t half = (shift & 2u) * 8u;
+#pragma unroll
+    for (uint32_t i = 0; i < kChunks; ++i) {
+      const uint32_t w[9] = {b.lo[i].x, b.lo[i].y, b.lo[i].z, b.lo[i].w, b.hi[i].x,
+                             b.hi[i].y, b.hi[i].z, b.hi[i].w, 0};
+      uint4 out;
+      out.x = __funnelshift_r(w[WORDS], w[WORDS + 1], half);
+      out.y = __funnelshift_r(w[WORDS + 1], w[WORDS + 2], half);
+      out.z = __funnelshift_r(w[WORDS + 2], w[WORDS + 3], half);
+      out.w = __funnelshift_r(w[WORDS + 3], w[WORDS + 4], half);
+      *reinterpret_cast<uint4 *>(dst + i * (kLoaders * 16)) = out;
+    }
+  }
   // Into the stage, as TMA's 128-byte swizzle would have it; elements beyond
-  // the operand are 0.
+  // the sum are 0.
   __device__ __forceinline__ void store(uint32_t kt, const Blocks &b,
                                         uint8_t *dst) const {
-    const uint32_t shift = static_cast<uint32_t>(at0) & 15u;
-    const bool inner = interior(kt);
     // The rows of a thread's chunks are 32 apart, so they swizzle alike.
-    dst += row(0) * 128 + ((tid % 8 ^ (row(0) & 7u)) << 4);
+    dst += dst0;
+    const uint32_t words = __shfl_sync(0xFFFFFFFFu, shift / 4, 0);
+    if (interior(kt)) {
+      if (words < 2) {
+        if (words == 0)
+          store_inner<0>(b, dst);
+        else
+          store_inner<1>(b, dst);
+      } else if (words == 2) {
+        store_inner<2>(b, dst);
+      } else {
+        store_inner<3>(b, dst);
+      }
+      return;
+    }
 #pragma unroll
     for (uint32_t i = 0; i < kChunks; ++i) {
       uint32_t w[8] = {b.lo[i].x, b.lo[i].y, b.lo[i].z, b.lo[i].w,
@@ -756,28 +776,21 @@ struct GuardedOperand {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         w[j] = __funnelshift_r(w[j], w[j + 1], (shift & 2u) * 8u);
-      if (!inner || !whole) {
-        const uint32_t n = inner ? side_count(i) : count(i, kt);
-        if (b.apart >> i & 1u) {
-          const uint16_t *src = reinterpret_cast<const uint16_t *>(where(i, kt));
-          uint32_t e[8];
+      const uint32_t n = count(i, kt);
+      if (b.apart >> i & 1u) {
+        const uint16_t *src =
+            reinterpret_cast<const uint16_t *>(block[i] + kt * step + shift);
+        uint32_t e[8];
 #pragma unroll
-          for (uint32_t j = 0; j < 8; ++j)
-            e[j] = src[min(j, n - 1)];
+        for (uint32_t j = 0; j < 8; ++j)
+          e[j] = src[min(j, n - 1)];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            w[j] = e[2 * j] | e[2 * j + 1] << 16;
-        }
-        if (MN || !inner) {
-#pragma unroll
-          for (uint32_t j = 0; j < 4; ++j)
-            w[j] = n >= 2 * j + 2 ? w[j] : (n == 2 * j + 1 ? w[j] & 0xFFFFu : 0u);
-        } else {
-#pragma unroll
-          for (uint32_t j = 0; j < 4; ++j)
-            w[j] = n ? w[j] : 0u;
-        }
+        for (int j = 0; j < 4; ++j)
+          w[j] = e[2 * j] | e[2 * j + 1] << 16;
       }
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j)
+        w[j] = n >= 2 * j + 2 ? w[j] : (n == 2 * j + 1 ? w[j] & 0xFFFFu : 0u);
       *reinterpret_cast<uint4 *>(dst + i * (kLoaders * 16)) =
           make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -930,9 +943,8 @@ __device__ __forceinline__ void product_single(const CUtensorMap *map_a,
     if (GUARDED) {
       // The loads of one stage are in flight while the last one's are shifted
       // into place and stored.
-      const uint32_t tid = threadIdx.x - 64;
-      const GuardedOperand<A_MN> a(p.a, p.lda, p.rows, p.depth, lane0, tid);
-      const GuardedOperand<B_MN> b(p.b, p.ldb, p.cols, p.depth, col0, tid);
+      const GuardedOperand<A_MN> a(p.a, p.lda, p.rows, p.depth, lane0, warp - 2, lane);
+      const GuardedOperand<B_MN> b(p.b, p.ldb, p.cols, p.depth, col0, warp - 2, lane);
       Blocks ra[2], rb[2];
       RingPlace at;
       auto load = [&](uint32_t kt, Blocks &xa, Blocks &xb) {
