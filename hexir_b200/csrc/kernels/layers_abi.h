@@ -35,10 +35,12 @@ extern "C" {
 #define HEXIR_PAIR_SMEM_BYTES                           \
   (HEXIR_PAIR_STAGES * HEXIR_PAIR_STAGE_BYTES + 1024 + \
    HEXIR_EPILOGUE_BYTES(8))
-/* Single CTAs: a load warp, an MMA warp and 8 epilogue (or guarded load)
- * warps. */
+/* Single CTAs: a load warp, an MMA warp and 8 epilogue warps, which are the
+ * first of the 16 that load where loads are guarded. */
 #define HEXIR_SINGLE_EPILOGUE_WARPS 8
 #define HEXIR_SINGLE_THREADS (64 + HEXIR_SINGLE_EPILOGUE_WARPS * 32)
+#define HEXIR_GUARDED_LOAD_WARPS 16
+#define HEXIR_GUARDED_THREADS (64 + HEXIR_GUARDED_LOAD_WARPS * 32)
 #define HEXIR_SINGLE_MAX_STAGES 12
 
 typedef struct {

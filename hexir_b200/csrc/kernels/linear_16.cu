@@ -607,7 +607,7 @@ __device__ __forceinline__ void product_pair(const CUtensorMap *map_a,
 // TMA would have written, and become the epilogue afterwards.  An operand
 // that TMA can describe still comes by TMA.
 
-constexpr uint32_t kLoaders = 256;                // threads
+constexpr uint32_t kLoaders = HEXIR_GUARDED_LOAD_WARPS * 32;  // threads
 constexpr uint32_t kChunks = kBM * 8 / kLoaders;  // of an operand's tile, a thread
 
 // The two 16-byte blocks of memory that each of a stage's chunks (8 elements of
@@ -628,8 +628,8 @@ __device__ __forceinline__ uint4 load_now(uintptr_t at) {
 }
 
 // One thread's chunks of an operand's 128 x 64 tiles: chunk i is 8 elements of
-// 128-byte row (i * 32 + lane / 8 * 8 + warp) of the stage.  The chunks of a
-// warp, in every tile, start at the same byte of a 16-byte block: their rows are
+// 128-byte row (i * 64 + warp / 8 * 32 + lane / 8 * 8 + warp % 8) of the stage.
+// The chunks of a warp, in every tile, start at the same byte of a 16-byte block: their rows are
 // 8 apart (and 64 elements or 64 values of the sum), and each of these is a
 // multiple of 16 bytes whatever the stride.  So the words to shift by are the
 // warp's, taken by a branch, and only halves are shifted by instructions.
@@ -658,25 +658,25 @@ struct GuardedOperand {
                                             uint32_t lane)
       : depth(depth_) {
     const uint32_t majors = MN ? depth : sides, minors = MN ? sides : depth;
-    const uint32_t row0 = lane / 8 * 8 + warp, column = lane % 8 * 8;
+    const uint32_t row0 = warp / 8 * 32 + lane / 8 * 8 + warp % 8, column = lane % 8 * 8;
     first = reinterpret_cast<uintptr_t>(p);
     last = majors ? first + ((majors - 1) * ld + minors) * 2 : first;
     safe = (first + 15) & ~static_cast<uintptr_t>(15);
     step = MN ? ld * (2 * kBK) : 2 * kBK;
     k0 = MN ? row0 : column;
-    dst0 = row0 * 128 + ((lane % 8 ^ warp) << 4);
+    dst0 = row0 * 128 + ((lane % 8 ^ warp % 8) << 4);
     // Within a warp the major index is the same but for multiples of 8.
     shift = static_cast<uint32_t>(
-                first + ((MN ? 0 : side0) + static_cast<uint64_t>(warp)) * ld * 2) & 15u;
+                first + ((MN ? 0 : side0) + static_cast<uint64_t>(warp % 8)) * ld * 2) & 15u;
     side_counts = 0;
 #pragma unroll
     for (uint32_t i = 0; i < kChunks; ++i) {
-      const uint32_t row = i * 32 + row0;
-      uint32_t s = side0 + (MN ? row / 64 * 64 + column : row);
+      const uint32_t row = i * 64 + row0;
+      uint32_t s = side0 + (MN ? i * 64 + column : row);
       const uint32_t n = s >= sides ? 0u : (MN ? min(8u, sides - s) : 8u);
       side_counts |= n << 4 * i;
       s = n ? s : side0;
-      block[i] = address(s, MN ? row % 64 : column, ld) & ~static_cast<uintptr_t>(15);
+      block[i] = address(s, MN ? row0 : column, ld) & ~static_cast<uintptr_t>(15);
     }
     // Blocks from the tile's first to 32 bytes past the start of its last
     // element's lie in the memory.
@@ -696,7 +696,7 @@ struct GuardedOperand {
   }
   // Elements of chunk i that the operand has.
   __device__ __forceinline__ uint32_t count(uint32_t i, uint32_t kt) const {
-    const uint32_t k = kt * kBK + k0 + (MN ? i % 2 * 32 : 0);
+    const uint32_t k = kt * kBK + k0;
     const uint32_t n = side_counts >> 4 * i & 15u;
     return k >= depth ? 0u : (MN ? n : min(n, depth - k));
   }
@@ -747,7 +747,7 @@ struct GuardedOperand {
   // the sum are 0.
   __device__ __forceinline__ void store(uint32_t kt, const Blocks &b,
                                         uint8_t *dst) const {
-    // The rows of a thread's chunks are 32 apart, so they swizzle alike.
+    // The rows of a thread's chunks are 64 apart, so they swizzle alike.
     dst += dst0;
     const uint32_t words = __shfl_sync(0xFFFFFFFFu, shift / 4, 0);
     if (interior(kt)) {
@@ -924,7 +924,7 @@ __device__ __forceinline__ void product_single(const CUtensorMap *map_a,
     if (leader)
       mma_commit(&done);  // also after a wait that ran out: nothing in flight
   } else {
-    if (!SWAP) {
+    if (!SWAP && warp < 2 + kWarps) {
       for (uint32_t i = 0; i < ahead.depth; ++i)
         fetch_next();
       if (FORM == HEXIR_PRODUCT_FORWARD && p.bias) {
@@ -982,6 +982,10 @@ __device__ __forceinline__ void product_single(const CUtensorMap *map_a,
       }
       __syncwarp();
     }
+  }
+
+  const bool finishes = warp >= 2 && warp < 2 + kWarps;
+  if (finishes) {
     ok = __all_sync(0xFFFFFFFFu,
                     mbar_wait_pipeline(&done, 0, 4 * p.timeout_ns));
     tc_fence_after();
@@ -1021,7 +1025,7 @@ __device__ __forceinline__ void product_single(const CUtensorMap *map_a,
   if (p.split > 1) {
     __syncwarp();
     cluster_sync();
-    if (warp >= 2 && ok) {
+    if (finishes && ok) {
       const uint32_t my = quarter * 32 + lane;
       const float4 *sums = reinterpret_cast<const float4 *>(ring);
       uint32_t nth = 0;
@@ -1059,7 +1063,7 @@ __device__ __forceinline__ void product_single(const CUtensorMap *map_a,
     __syncwarp();
     cluster_sync();  // the peers have read this CTA's sums
   }
-  if (warp >= 2)
+  if (finishes)
     copies_wait<0>();
   tc_fence_before();
   __syncthreads();
@@ -1086,7 +1090,7 @@ __device__ __forceinline__ void product_single(const CUtensorMap *map_a,
     product_single<FORM, false, SWAP>(&map_a, &map_b, args);                  \
   }
 #define PRODUCT_GUARDED(NAME, FORM)                                           \
-  extern "C" __global__ void __launch_bounds__(HEXIR_SINGLE_THREADS)          \
+  extern "C" __global__ void __launch_bounds__(HEXIR_GUARDED_THREADS)         \
       NAME(const __grid_constant__ CUtensorMap map_a,                         \
            const __grid_constant__ CUtensorMap map_b, const Args args) {      \
     product_single<FORM, true, false>(&map_a, &map_b, args);                  \

@@ -646,7 +646,10 @@ hexir_status_t launch_product(Call &call, uint32_t op, uint32_t m, uint32_t n,
   const char *what = p.variant == kSkinny         ? "launch hexir_linear_16 skinny"
                      : p.variant == kGuardedLoads ? "launch hexir_linear_16 guarded"
                                                   : "launch hexir_linear_16 single";
-  return launch_after(fn, grid, 1, HEXIR_SINGLE_THREADS, stream, params, what,
+  return launch_after(fn, grid, 1,
+                      p.variant == kGuardedLoads ? HEXIR_GUARDED_THREADS
+                                                    : HEXIR_SINGLE_THREADS,
+                      stream, params, what,
                       &call.error, p.smem, p.split);
 }
 
