@@ -638,9 +638,42 @@ __device__ __forceinline__ uint4 load_now(uintptr_t at) {
 // inside the tensor's memory (from its first element to its last, gaps between
 // rows included), needs no checks: chunks beyond the operand's side read the
 // side's first instead, and what they leave in the sums is never stored.  In
-// the others (the last k tile, and the first at the tensor's start) every chunk
-// is checked, and the few whose blocks reach outside the memory are taken
+// the others (the last k tiles, and the first at the tensor's start) every
+// chunk is checked, and the few whose blocks reach outside the memory are taken
 // element by element.
+
+__device__ __forceinline__ uintptr_t element_at(const void *p, uint64_t ld, bool mn,
+                                                uint32_t s, uint32_t k) {
+  return reinterpret_cast<uintptr_t>(p) + (mn ? k * ld + s : s * ld + k) * 2;
+}
+
+// One past an operand's last element.
+__device__ __forceinline__ uintptr_t memory_end(const void *p, uint64_t ld, bool mn,
+                                                uint32_t sides, uint32_t depth) {
+  return depth ? element_at(p, ld, mn, sides - 1, depth - 1) + 2
+               : reinterpret_cast<uintptr_t>(p);
+}
+
+// Leaves of the k tiles [inner0, inner1) those that need no checks of a tile
+// that starts at side0: blocks from the one of its first element to 32 bytes
+// past the start of its last lie in the memory.
+__device__ __forceinline__ void keep_inner(const void *p, uint64_t ld, bool mn,
+                                           uint32_t sides, uint32_t depth,
+                                           uint32_t side0, uint32_t &inner0,
+                                           uint32_t &inner1) {
+  const uint64_t step = mn ? ld * (2 * kBK) : 2 * kBK;
+  const uintptr_t low =
+      element_at(p, ld, mn, side0, 0) & ~static_cast<uintptr_t>(15);
+  const uintptr_t high =
+      element_at(p, ld, mn, min(side0 + kBM, sides) - 1, kBK - 1) + 32;
+  const uintptr_t end = memory_end(p, ld, mn, sides, depth);
+  if (low < reinterpret_cast<uintptr_t>(p))
+    inner0 = max(inner0, 1u);
+  inner1 = min(inner1, depth / kBK);
+  while (inner1 > inner0 && high + (inner1 - 1) * step > end)
+    --inner1;
+}
+
 template <bool MN>
 struct GuardedOperand {
   uintptr_t block[kChunks];     // of k tile 0
@@ -648,7 +681,6 @@ struct GuardedOperand {
   uint64_t step;                // bytes to the next k tile
   uint32_t depth;
   uint32_t shift;               // bytes into a block
-  uint32_t inner0, inner1;      // the k tiles that need no checks
   uint32_t side_counts;         // 4 bits a chunk: elements inside the side
   uint32_t k0, dst0;            // chunk 0: of the sum; byte in the stage
 
@@ -657,10 +689,10 @@ struct GuardedOperand {
                                             uint32_t side0, uint32_t warp,
                                             uint32_t lane)
       : depth(depth_) {
-    const uint32_t majors = MN ? depth : sides, minors = MN ? sides : depth;
-    const uint32_t row0 = warp / 8 * 32 + lane / 8 * 8 + warp % 8, column = lane % 8 * 8;
+    const uint32_t row0 = warp / 8 * 32 + lane / 8 * 8 + warp % 8;
+    const uint32_t column = lane % 8 * 8;
     first = reinterpret_cast<uintptr_t>(p);
-    last = majors ? first + ((majors - 1) * ld + minors) * 2 : first;
+    last = memory_end(p, ld, MN, sides, depth);
     safe = (first + 15) & ~static_cast<uintptr_t>(15);
     step = MN ? ld * (2 * kBK) : 2 * kBK;
     k0 = MN ? row0 : column;
@@ -676,23 +708,9 @@ struct GuardedOperand {
       const uint32_t n = s >= sides ? 0u : (MN ? min(8u, sides - s) : 8u);
       side_counts |= n << 4 * i;
       s = n ? s : side0;
-      block[i] = address(s, MN ? row0 : column, ld) & ~static_cast<uintptr_t>(15);
+      block[i] = element_at(p, ld, MN, s, MN ? row0 : column) &
+                 ~static_cast<uintptr_t>(15);
     }
-    // Blocks from the tile's first to 32 bytes past the start of its last
-    // element's lie in the memory.
-    const uintptr_t low = address(side0, 0, ld) & ~static_cast<uintptr_t>(15);
-    const uintptr_t high = address(min(side0 + kBM, sides) - 1, kBK - 1, ld) + 32;
-    inner0 = low >= first ? 0 : 1;
-    inner1 = depth / kBK;
-    while (inner1 > inner0 && high + (inner1 - 1) * step > last)
-      --inner1;
-  }
-  __device__ __forceinline__ uintptr_t address(uint32_t s, uint32_t k,
-                                               uint64_t ld) const {
-    return first + (MN ? k * ld + s : s * ld + k) * 2;
-  }
-  __device__ __forceinline__ bool interior(uint32_t kt) const {
-    return kt >= inner0 && kt < inner1;
   }
   // Elements of chunk i that the operand has.
   __device__ __forceinline__ uint32_t count(uint32_t i, uint32_t kt) const {
@@ -701,22 +719,22 @@ struct GuardedOperand {
     return k >= depth ? 0u : (MN ? n : min(n, depth - k));
   }
 
-  __device__ __forceinline__ void load(uint32_t kt, Blocks &b) const {
-    b.apart = 0;
-    const uint64_t offset = kt * step;
-    if (interior(kt)) {
+  // A k tile without checks: the blocks at `block`, which is on the tile.
+  __device__ __forceinline__ void load_inner(Blocks &b) {
 #pragma unroll
-      for (uint32_t i = 0; i < kChunks; ++i) {
-        b.lo[i] = load_now(block[i] + offset);
-        b.hi[i] = load_now(block[i] + offset + 16);
-      }
-      return;
+    for (uint32_t i = 0; i < kChunks; ++i) {
+      b.lo[i] = load_now(block[i]);
+      b.hi[i] = load_now(block[i] + 16);
+      block[i] += step;
     }
+  }
+  __device__ __forceinline__ void load_checked(uint32_t kt, Blocks &b) const {
+    b.apart = 0;
     const bool any = safe + 16 <= last;
 #pragma unroll
     for (uint32_t i = 0; i < kChunks; ++i) {
       const uint32_t n = count(i, kt);
-      const uintptr_t at = block[i] + offset;
+      const uintptr_t at = block[i] + kt * step;
       const bool two = shift + 2 * n > 16;
       const bool inside = at >= first && at + (two ? 32 : 16) <= last;
       b.apart |= static_cast<uint32_t>(n && !inside) << i;
@@ -729,7 +747,7 @@ struct GuardedOperand {
   }
   // The chunks, WORDS 32-bit words and possibly a half into their blocks.
   template <int WORDS>
-  __device__ __forceinline__ void store_inner(const Blocks &b, uint8_t *dst) const {
+  __device__ __forceinline__ void store_shifted(const Blocks &b, uint8_t *dst) const {
     const uint32_t half = (shift & 2u) * 8u;
 #pragma unroll
     for (uint32_t i = 0; i < kChunks; ++i) {
@@ -743,26 +761,26 @@ struct GuardedOperand {
       *reinterpret_cast<uint4 *>(dst + i * (kLoaders * 16)) = out;
     }
   }
-  // Into the stage, as TMA's 128-byte swizzle would have it; elements beyond
-  // the sum are 0.
-  __device__ __forceinline__ void store(uint32_t kt, const Blocks &b,
-                                        uint8_t *dst) const {
+  // Into the stage, as TMA's 128-byte swizzle would have it.
+  __device__ __forceinline__ void store_inner(const Blocks &b, uint8_t *stage,
+                                              uint32_t words) const {
     // The rows of a thread's chunks are 64 apart, so they swizzle alike.
-    dst += dst0;
-    const uint32_t words = __shfl_sync(0xFFFFFFFFu, shift / 4, 0);
-    if (interior(kt)) {
-      if (words < 2) {
-        if (words == 0)
-          store_inner<0>(b, dst);
-        else
-          store_inner<1>(b, dst);
-      } else if (words == 2) {
-        store_inner<2>(b, dst);
-      } else {
-        store_inner<3>(b, dst);
-      }
-      return;
+    uint8_t *dst = stage + dst0;
+    if (words < 2) {
+      if (words == 0)
+        store_shifted<0>(b, dst);
+      else
+        store_shifted<1>(b, dst);
+    } else if (words == 2) {
+      store_shifted<2>(b, dst);
+    } else {
+      store_shifted<3>(b, dst);
     }
+  }
+  // Elements beyond the sum are 0.
+  __device__ __forceinline__ void store_checked(uint32_t kt, const Blocks &b,
+                                                uint8_t *stage) const {
+    uint8_t *dst = stage + dst0;
 #pragma unroll
     for (uint32_t i = 0; i < kChunks; ++i) {
       uint32_t w[8] = {b.lo[i].x, b.lo[i].y, b.lo[i].z, b.lo[i].w,
@@ -851,6 +869,23 @@ __device__ __forceinline__ void product_single(const CUtensorMap *map_a,
   const uint32_t kt1 = static_cast<uint32_t>(
       static_cast<uint64_t>(p.k_tiles) * (rank + 1) / p.split);
   const uint32_t lane0 = tm * kBM, col0 = tn * p.tile_n;
+  // GUARDED: of these, [inner0, inner1) need no checks.  The others come first,
+  // so that what checking needs is no longer there in the loop without checks.
+  uint32_t inner0 = kt0, inner1 = kt1;
+  if (GUARDED) {
+    if (!tma_a)
+      keep_inner(p.a, p.lda, A_MN, p.rows, p.depth, lane0, inner0, inner1);
+    if (!tma_b)
+      keep_inner(p.b, p.ldb, B_MN, p.cols, p.depth, col0, inner0, inner1);
+    if (inner0 >= inner1)
+      inner0 = inner1 = kt1;
+  }
+  const uint32_t head = inner0 - kt0, checked = head + (kt1 - inner1);
+  auto nth_tile = [&](uint32_t i) {
+    return !GUARDED || i < head ? kt0 + i
+           : i < checked        ? inner1 + (i - head)
+                                : inner0 + (i - checked);
+  };
   // The epilogue warps: 32 lanes' rows, and every other block of 16 columns
   // (of the cluster's share of them, once the sums are joined).
   const uint32_t quarter = warp & 3u, side = warp >= 2 ? (warp - 2) / 4 : 0;
@@ -871,7 +906,8 @@ __device__ __forceinline__ void product_single(const CUtensorMap *map_a,
       const bool leader = elect_one();
       RingPlace at;
       uint32_t fills = 0;
-      for (uint32_t kt = kt0; kt < kt1; ++kt, ++fills, at.next(stages)) {
+      for (; fills < kt1 - kt0; ++fills, at.next(stages)) {
+        const uint32_t kt = nth_tile(fills);
         ok = __all_sync(0xFFFFFFFFu, mbar_wait_pipeline(&empty[at.stage],
                                                         at.parity ^ 1u, p.timeout_ns));
         if (!ok)
@@ -941,44 +977,78 @@ __device__ __forceinline__ void product_single(const CUtensorMap *map_a,
       }
     }
     if (GUARDED) {
-      // The loads of one stage are in flight while the last one's are shifted
-      // into place and stored.
-      const GuardedOperand<A_MN> a(p.a, p.lda, p.rows, p.depth, lane0, warp - 2, lane);
-      const GuardedOperand<B_MN> b(p.b, p.ldb, p.cols, p.depth, col0, warp - 2, lane);
-      Blocks ra[2], rb[2];
+      GuardedOperand<A_MN> a(p.a, p.lda, p.rows, p.depth, lane0, warp - 2, lane);
+      GuardedOperand<B_MN> b(p.b, p.ldb, p.cols, p.depth, col0, warp - 2, lane);
       RingPlace at;
-      auto load = [&](uint32_t kt, Blocks &xa, Blocks &xb) {
-        if (kt < kt1) {
-          if (!tma_a)
-            a.load(kt, xa);
-          if (!tma_b)
-            b.load(kt, xb);
-        }
+      const uint32_t words_a = __shfl_sync(0xFFFFFFFFu, a.shift / 4, 0);
+      const uint32_t words_b = __shfl_sync(0xFFFFFFFFu, b.shift / 4, 0);
+      bool going = true;
+      auto empty_stage = [&] {
+        going = __all_sync(0xFFFFFFFFu, mbar_wait_pipeline(&empty[at.stage],
+                                                           at.parity ^ 1u, p.timeout_ns));
+        return ring + at.stage * stage_bytes;
       };
-      auto settle = [&](uint32_t kt, const Blocks &xa, const Blocks &xb) {
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait_pipeline(&empty[at.stage],
-                                                        at.parity ^ 1u, p.timeout_ns)))
-          return false;
-        uint8_t *dst = ring + at.stage * stage_bytes;
-        if (!tma_a)
-          a.store(kt, xa, dst);
-        if (!tma_b)
-          b.store(kt, xb, dst + kABytes);
+      auto filled = [&] {
         fence_async_smem();
         __syncwarp();
         if (lane == 0)
           mbar_arrive(&full[at.stage]);
         at.next(stages);
-        return true;
       };
-      load(kt0, ra[0], rb[0]);
-      for (uint32_t kt = kt0; kt < kt1; kt += 2) {
-        load(kt + 1, ra[1], rb[1]);
-        if (!settle(kt, ra[0], rb[0]))
+      Blocks ra[2], rb[2];
+#pragma unroll 1
+      for (uint32_t i = 0; i < checked && going; ++i) {
+        const uint32_t kt = nth_tile(i);
+        if (!tma_a)
+          a.load_checked(kt, ra[0]);
+        if (!tma_b)
+          b.load_checked(kt, rb[0]);
+        uint8_t *dst = empty_stage();
+        if (going) {
+          if (!tma_a)
+            a.store_checked(kt, ra[0], dst);
+          if (!tma_b)
+            b.store_checked(kt, rb[0], dst + kABytes);
+          filled();
+        }
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < kChunks; ++i) {
+        a.block[i] += inner0 * a.step;
+        b.block[i] += inner0 * b.step;
+      }
+      // The loads of one stage are in flight while the last one's are shifted
+      // into place and stored.
+      auto load = [&](Blocks &xa, Blocks &xb) {
+        if (!tma_a)
+          a.load_inner(xa);
+        if (!tma_b)
+          b.load_inner(xb);
+      };
+      auto settle = [&](const Blocks &xa, const Blocks &xb) {
+        uint8_t *dst = empty_stage();
+        if (going) {
+          if (!tma_a)
+            a.store_inner(xa, dst, words_a);
+          if (!tma_b)
+            b.store_inner(xb, dst + kABytes, words_b);
+          filled();
+        }
+      };
+      uint32_t left = inner1 - inner0;
+      if (left)
+        load(ra[0], rb[0]);
+#pragma unroll 1
+      while (left && going) {
+        if (left > 1)
+          load(ra[1], rb[1]);
+        settle(ra[0], rb[0]);
+        if (left == 1 || !going)
           break;
-        load(kt + 2, ra[0], rb[0]);
-        if (kt + 1 < kt1 && !settle(kt + 1, ra[1], rb[1]))
-          break;
+        if (left > 2)
+          load(ra[0], rb[0]);
+        settle(ra[1], rb[1]);
+        left -= 2;
       }
       __syncwarp();
     }

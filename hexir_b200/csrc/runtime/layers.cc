@@ -440,7 +440,7 @@ double modelled_us(uint32_t variant, uint32_t tile_n, uint32_t split, uint32_t r
   // Clusters are placed inside a GPC: 32 of 4 CTAs and 16 of 8 are resident.
   const uint64_t resident = split >= 4 ? sms * 7 / 8 / split * split : sms;
   const uint64_t waves = (ctas + resident - 1) / std::max<uint64_t>(resident, 1);
-  const double k_tile = c.k_tile + 0.8 * guarded;  // operands of guarded loads
+  const double k_tile = c.k_tile + 0.23 * guarded;  // operands of guarded loads
   return c.base + waves * (ceil_div(k_tiles, split) * k_tile + c.wave);
 }
 
