@@ -135,10 +135,9 @@ __device__ __forceinline__ T pack_get(const Pack<T> &p, int j) {
 //             16-byte boundaries;
 //   kShifted  the same packs of memory, but the row starts `phase` elements
 //             after a boundary: its first pack is filled from element `phase`
-//             on (16-bit types; every tensor of the call has the same phase,
-//             and a thread's rows are a multiple of 8 apart so that they
-//             share it).  f32 and f64 gain nothing by it: their single
-//             elements make loads that are wide enough;
+//             on (16-bit types and long f32 rows; every tensor of the call has
+//             the same phase, and a thread's rows are a multiple of 8 apart so
+//             that they share it);
 //   kAny      single elements tid, tid + TH, ..., so that a warp's accesses
 //             stay consecutive.
 enum Layout { kWhole, kShifted, kAny };
@@ -1048,13 +1047,12 @@ __device__ __forceinline__ void output_grad_join(
   NORM(SUFFIX, T, 512, 32, w, kWhole, 1)                                       \
   NORM(SUFFIX, T, 32, 8, h, kShifted, 5)                                       \
   NORM(SUFFIX, T, 32, 16, h, kShifted, 3)                                      \
-  NORM(SUFFIX, T, 32, 24, h, kShifted, 2)                                      \
-  NORM(SUFFIX, T, 32, 32, h, kShifted, 2)                                      \
+  NORM(SUFFIX, T, 64, 16, h, kShifted, 3)                                      \
   NORM(SUFFIX, T, 128, 16, h, kShifted, 4)                                     \
-  NORM(SUFFIX, T, 256, 16, h, kShifted, 4)                                     \
-  NORM(SUFFIX, T, 256, 24, h, kShifted, 2)                                     \
-  NORM(SUFFIX, T, 256, 32, h, kShifted, 2)                                     \
-  NORM(SUFFIX, T, 512, 32, h, kShifted, 1)                                     \
+  NORM(SUFFIX, T, 256, 16, h, kShifted, 3)                                     \
+  NORM(SUFFIX, T, 320, 16, h, kShifted, 2)                                     \
+  NORM(SUFFIX, T, 512, 16, h, kShifted, 2)                                     \
+  NORM(SUFFIX, T, 1024, 16, h, kShifted, 1)                                    \
   NORM(SUFFIX, T, 32, 32, s, kAny, 2)                                          \
   NORM(SUFFIX, T, 256, 16, s, kAny, 3)                                         \
   NORM(SUFFIX, T, 512, 32, s, kAny, 1)                                         \
@@ -1088,6 +1086,12 @@ NORM(f32, float, 128, 16, w, kWhole, 3)
 NORM(f32, float, 256, 16, w, kWhole, 3)
 NORM(f32, float, 512, 16, w, kWhole, 2)
 NORM(f32, float, 1024, 16, w, kWhole, 1)
+NORM(f32, float, 256, 8, h, kShifted, 4)
+NORM(f32, float, 320, 8, h, kShifted, 3)
+NORM(f32, float, 512, 8, h, kShifted, 2)
+NORM(f32, float, 640, 8, h, kShifted, 1)
+NORM(f32, float, 512, 16, h, kShifted, 1)
+NORM(f32, float, 1024, 16, h, kShifted, 1)
 NORM(f32, float, 32, 8, s, kAny, 5)
 NORM(f32, float, 32, 16, s, kAny, 3)
 NORM(f32, float, 128, 8, s, kAny, 4)
@@ -1101,6 +1105,11 @@ NORM_GRAD(f32, float, 128, 8, w, kWhole, 2, 4)
 NORM_GRAD(f32, float, 256, 8, w, kWhole, 2, 4)
 NORM_GRAD(f32, float, 512, 8, w, kWhole, 1, 3)
 NORM_GRAD(f32, float, 512, 16, w, kWhole, 1, 2)
+NORM_GRAD(f32, float, 256, 8, h, kShifted, 2, 4)
+NORM_GRAD(f32, float, 320, 8, h, kShifted, 1, 4)
+NORM_GRAD(f32, float, 512, 8, h, kShifted, 1, 3)
+NORM_GRAD(f32, float, 640, 8, h, kShifted, 1, 2)
+NORM_GRAD(f32, float, 512, 16, h, kShifted, 1, 2)
 NORM_GRAD(f32, float, 64, 8, s, kAny, 2, 4)
 NORM_GRAD(f32, float, 128, 8, s, kAny, 2, 4)
 NORM_GRAD(f32, float, 320, 8, s, kAny, 1, 4)
