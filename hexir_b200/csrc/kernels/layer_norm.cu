@@ -749,7 +749,34 @@ __device__ __forceinline__ void norm_grad_rows(
   if (!p.partials)
     return;
   R *part = static_cast<R *>(p.partials) + (uint64_t)blockIdx.x * 2 * p.cols;
-  if (kRows == 1) {
+  // Whole rows in 16-byte stores (a warp's 4-byte stores would each touch 32
+  // sectors); single elements lie next to each other across a warp.
+  if (kRows == 1 && LAYOUT == kWhole) {
+    constexpr int kV = 16 / sizeof(R);
+#pragma unroll
+    for (int i = 0; i < kPacks; ++i) {
+      if (!lay.some(i))
+        continue;
+#pragma unroll
+      for (int j = 0; j < kN; j += kV) {
+        R *at = part + lay.column(i, j);
+        Pack<R> v;
+        Two<R> f[kV / 2];
+#pragma unroll
+        for (int e = 0; e < kV / 2; ++e)
+          f[e] = dgamma[(i * kN + j) / 2 + e];
+        narrow_pack(f, v);
+        *reinterpret_cast<uint4 *>(at) = v.w;
+#pragma unroll
+        for (int e = 0; e < kV / 2; ++e)
+          f[e] = dbeta[(i * kN + j) / 2 + e];
+        narrow_pack(f, v);
+        *reinterpret_cast<uint4 *>(at + p.cols) = v.w;
+      }
+    }
+    return;
+  }
+  if (kRows == 1 && LAYOUT == kAny) {
 #pragma unroll
     for (int i = 0; i < kPacks; ++i)
 #pragma unroll
@@ -762,31 +789,54 @@ __device__ __forceinline__ void norm_grad_rows(
       }
     return;
   }
-  // The block's rows may differ in phase: their sums meet by column, in the
-  // ring's place.
-  R(*joined)[TH * NE] = reinterpret_cast<R(*)[TH * NE]>(ring);
+  // The block's rows may differ in phase, and a shifted row's packs are not
+  // whole 16 bytes of sums: the sums meet in the ring's place, by their place
+  // in the row's packs.
+  static_assert(DEPTH * sizeof(T) >= sizeof(R), "the ring holds the sums");
+  R(*joined)[2][TH * NE] = reinterpret_cast<R(*)[2][TH * NE]>(ring);
+  __shared__ uint32_t phases[kRows];
   __syncthreads();
+  if (tid == 0)
+    phases[group] = lay.phase;
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-#pragma unroll
-    for (int i = 0; i < kPacks; ++i)
+  for (int i = 0; i < kPacks; ++i) {
+    if (LAYOUT == kAny) {
 #pragma unroll
       for (int j = 0; j < kN; ++j) {
-        const uint32_t c = lay.column(i, j);
-        if (c < p.cols)
-          joined[group][c] =
-              half_of(which ? dbeta[(i * kN + j) / 2] : dgamma[(i * kN + j) / 2], j);
+        const uint32_t at = (i * kN + j) * TH + tid;
+        joined[group][0][at] = half_of(dgamma[(i * kN + j) / 2], j);
+        joined[group][1][at] = half_of(dbeta[(i * kN + j) / 2], j);
       }
-    __syncthreads();
-    for (uint32_t c = threadIdx.x; c < p.cols; c += 256) {
+    } else {
+      constexpr int kV = 16 / sizeof(R);
+#pragma unroll
+      for (int j = 0; j < kN; j += kV) {
+        const uint32_t at = (i * TH + tid) * kN + j;
+        Pack<R> v;
+        Two<R> f[kV / 2];
+#pragma unroll
+        for (int e = 0; e < kV / 2; ++e)
+          f[e] = dgamma[(i * kN + j) / 2 + e];
+        narrow_pack(f, v);
+        *reinterpret_cast<uint4 *>(&joined[group][0][at]) = v.w;
+#pragma unroll
+        for (int e = 0; e < kV / 2; ++e)
+          f[e] = dbeta[(i * kN + j) / 2 + e];
+        narrow_pack(f, v);
+        *reinterpret_cast<uint4 *>(&joined[group][1][at]) = v.w;
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int which = 0; which < 2; ++which)
+    for (uint32_t c = threadIdx.x; c < p.cols; c += kBlock) {
       R s = 0;
 #pragma unroll
       for (uint32_t w = 0; w < kRows; ++w)
-        s += joined[w][c];
+        s += joined[w][which][c + phases[w]];
       part[(uint64_t)which * p.cols + c] = s;
     }
-    __syncthreads();
-  }
 }
 
 // Longer rows: dx in three passes (the later two from L2); dgamma and dbeta
@@ -1051,6 +1101,7 @@ __device__ __forceinline__ void output_grad_join(
   NORM(SUFFIX, T, 128, 16, h, kShifted, 4)                                     \
   NORM(SUFFIX, T, 256, 16, h, kShifted, 3)                                     \
   NORM(SUFFIX, T, 320, 16, h, kShifted, 2)                                     \
+  NORM(SUFFIX, T, 384, 16, h, kShifted, 2)                                     \
   NORM(SUFFIX, T, 512, 16, h, kShifted, 2)                                     \
   NORM(SUFFIX, T, 1024, 16, h, kShifted, 1)                                    \
   NORM(SUFFIX, T, 32, 32, s, kAny, 2)                                          \
@@ -1106,13 +1157,13 @@ NORM_GRAD(f32, float, 256, 8, w, kWhole, 2, 4)
 NORM_GRAD(f32, float, 512, 8, w, kWhole, 1, 3)
 NORM_GRAD(f32, float, 512, 16, w, kWhole, 1, 2)
 NORM_GRAD(f32, float, 256, 8, h, kShifted, 2, 4)
-NORM_GRAD(f32, float, 320, 8, h, kShifted, 1, 4)
+NORM_GRAD(f32, float, 320, 8, h, kShifted, 2, 4)
 NORM_GRAD(f32, float, 512, 8, h, kShifted, 1, 3)
 NORM_GRAD(f32, float, 640, 8, h, kShifted, 1, 2)
 NORM_GRAD(f32, float, 512, 16, h, kShifted, 1, 2)
 NORM_GRAD(f32, float, 64, 8, s, kAny, 2, 4)
 NORM_GRAD(f32, float, 128, 8, s, kAny, 2, 4)
-NORM_GRAD(f32, float, 320, 8, s, kAny, 1, 4)
+NORM_GRAD(f32, float, 320, 8, s, kAny, 2, 4)
 NORM_GRAD(f32, float, 512, 8, s, kAny, 1, 3)
 NORM_GRAD(f32, float, 512, 16, s, kAny, 1, 2)
 

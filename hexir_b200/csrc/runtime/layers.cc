@@ -37,7 +37,7 @@ struct NormShape {
   uint32_t rows() const { return threads < 256 ? 256 / threads : 1; }
   uint32_t block() const { return rows() * threads; }
 };
-constexpr int kMaxShapes = 20;
+constexpr int kMaxShapes = 21;
 // By the kind of type: 16-bit, f32, f64.
 constexpr NormShape kNorm[3][kMaxShapes] = {
     {{"w32x8", 32, 8, kWhole, 0},
@@ -55,6 +55,7 @@ constexpr NormShape kNorm[3][kMaxShapes] = {
      {"h128x16", 128, 16, kShifted, 0},
      {"h256x16", 256, 16, kShifted, 0},
      {"h320x16", 320, 16, kShifted, 0},
+     {"h384x16", 384, 16, kShifted, 0},
      {"h512x16", 512, 16, kShifted, 0},
      {"h1024x16", 1024, 16, kShifted, 0},
      {"s32x32", 32, 32, kAny, 0},
@@ -1064,11 +1065,9 @@ extern "C" hexir_status_t hexir_cuda_layer_norm_grad(
   if (c.rows && at >= 0) {
     const NormShape &shape = kNormGrad[kind][at];
     const LayersLib::Sized &kernel = call.lib->norm_grad[c.dtype][at];
-    // The ring of rows; then the column sums of a block's rows.
-    const uint32_t row = shape.block() * shape.elements;
-    const uint32_t ring =
-        std::max<uint32_t>(shape.depth * (c.residual && c.dx ? 3 : 2) * row * size,
-                           shape.rows() > 1 ? row * real : 0);
+    // The ring of rows; its place then holds the column sums of a block's rows.
+    const uint32_t ring = shape.depth * (c.residual && c.dx ? 3 : 2) * shape.block() *
+                          shape.elements * size;
     const uint64_t resident = std::min<uint64_t>(
         sms * blocks_per_sm(kernel.registers, shape.block(), ring), kSumsPerColumn / 2);
     args.parts =
