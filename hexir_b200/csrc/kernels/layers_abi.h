@@ -57,9 +57,10 @@ typedef struct {
   uint32_t is_f16;        /* f16, else bf16 */
   uint32_t vec;           /* epilogue rows on 16- (1) or 32-byte (2) boundaries */
   uint32_t tiles_m, tiles_n, group_m;
+  uint32_t full_tiles;    /* pair: those not cut in two */
   uint32_t tile_n;        /* columns of a tile */
   uint32_t k_tiles;       /* ceil(depth / BK) */
-  uint32_t split, k_tiles_per_split;
+  uint32_t split;
   uint32_t stages;        /* single: pipeline stages */
   uint32_t tmem_cols;     /* single: TMEM columns (a power of two >= 32) */
   uint32_t ring_bytes;    /* single: the stages, or the sums of a split tile */

@@ -388,6 +388,18 @@ __device__ __forceinline__ void load_operand(uint8_t *dst, uint32_t size,
     load(dst, static_cast<int32_t>(k), static_cast<int32_t>(side));
   }
 }
+// A pair's part of B: boxes of 64 in either layout, for tiles of two widths.
+template <bool MN, typename Load>
+__device__ __forceinline__ void load_boxes(uint8_t *dst, uint32_t size, uint32_t side,
+                                           uint32_t k, Load load) {
+  for (uint32_t b = 0; b < size / 64; ++b) {
+    const int32_t at = static_cast<int32_t>(side + b * 64);
+    if (MN)
+      load(dst + b * kBox, at, static_cast<int32_t>(k));
+    else
+      load(dst + b * kBox, static_cast<int32_t>(k), at);
+  }
+}
 
 // The four K = 16 steps of one stage.
 template <int CG, bool A_MN, bool B_MN>
@@ -410,7 +422,8 @@ __device__ __forceinline__ uint8_t *align1024(uint8_t *p) {
 // of A, half of the columns of B and its own rows' sums in TMEM, so a stage
 // costs half the shared-memory traffic per product of a single CTA's.  Two
 // sets of sums alternate: the epilogue of one tile runs under the MMAs of the
-// next.
+// next.  Where the tiles of the last turn would leave half of the pairs or more
+// without work, they are cut in two (a half costs about 0.7 of a tile).
 template <int FORM>
 __device__ __forceinline__ void product_pair(const CUtensorMap *map_a,
                                              const CUtensorMap *map_b,
@@ -428,8 +441,6 @@ __device__ __forceinline__ void product_pair(const CUtensorMap *map_a,
   const uint32_t warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x / 32, 0);
   const uint32_t lane = threadIdx.x % 32;
   const uint32_t rank = cluster_ctarank();
-  const uint32_t half_n = p.tile_n / 2;
-  const uint32_t stage_bytes = kABytes + half_n * 128u;
 
   if (threadIdx.x == 0) {
     prefetch_tensormap(map_a);
@@ -454,7 +465,19 @@ __device__ __forceinline__ void product_pair(const CUtensorMap *map_a,
   griddep_wait();  // nothing global is read or written before this
   griddep_launch_dependents();
 
-  const uint32_t tiles = p.tiles_m * p.tiles_n;
+  // The work: full_tiles tiles, then the halves (along the columns) of the rest.
+  struct Item {
+    uint32_t row0, col0, half_n;  // half_n: columns of B a CTA holds
+  };
+  const uint32_t items = 2 * p.tiles_m * p.tiles_n - p.full_tiles;
+  auto item_of = [&](uint32_t i) {
+    const uint32_t over = i < p.full_tiles ? 0 : i - p.full_tiles;
+    uint32_t tm, tn;
+    tile_of(i < p.full_tiles ? i : p.full_tiles + over / 2, p.tiles_m, p.tiles_n,
+            p.group_m, tm, tn);
+    const uint32_t half_n = p.tile_n / (i < p.full_tiles ? 2u : 4u);
+    return Item{tm * 2 * kBM, tn * p.tile_n + (over & 1u) * (p.tile_n / 2), half_n};
+  };
   const uint32_t first = blockIdx.x / 2, step = gridDim.x / 2;
 
   if (warp == 0) {
@@ -462,11 +485,10 @@ __device__ __forceinline__ void product_pair(const CUtensorMap *map_a,
     RingPlace at;
     uint32_t fills = 0;
     bool ok = true;
-    for (uint32_t tile = first; tile < tiles && ok; tile += step) {
-      uint32_t tm, tn;
-      tile_of(tile, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
-      const uint32_t row0 = tm * 2 * kBM + rank * kBM;
-      const uint32_t col0 = tn * p.tile_n + rank * half_n;
+    for (uint32_t i = first; i < items && ok; i += step) {
+      const Item item = item_of(i);
+      const uint32_t row0 = item.row0 + rank * kBM;
+      const uint32_t col0 = item.col0 + rank * item.half_n;
       for (uint32_t kt = 0; kt < p.k_tiles; ++kt, ++fills, at.next(kStages)) {
         ok = __all_sync(0xFFFFFFFFu, mbar_wait_pipeline(&empty[at.stage],
                                                         at.parity ^ 1u, p.timeout_ns));
@@ -474,17 +496,18 @@ __device__ __forceinline__ void product_pair(const CUtensorMap *map_a,
           break;
         if (leader) {
           if (rank == 0)
-            mbar_arrive_expect_tx(&full[at.stage], 2 * stage_bytes);
+            mbar_arrive_expect_tx(&full[at.stage],
+                                  2 * (kABytes + item.half_n * 128u));
           uint8_t *dst = ring + at.stage * HEXIR_PAIR_STAGE_BYTES;
           const uint32_t bar = cluster_addr(&full[at.stage], 0);
           load_operand<A_MN>(dst, kBM, row0, kt * kBK,
                              [&](uint8_t *d, int32_t x, int32_t y) {
                                tma_load_2d_pair(d, map_a, x, y, bar);
                              });
-          load_operand<B_MN>(dst + kABytes, half_n, col0, kt * kBK,
-                             [&](uint8_t *d, int32_t x, int32_t y) {
-                               tma_load_2d_pair(d, map_b, x, y, bar);
-                             });
+          load_boxes<B_MN>(dst + kABytes, item.half_n, col0, kt * kBK,
+                           [&](uint8_t *d, int32_t x, int32_t y) {
+                             tma_load_2d_pair(d, map_b, x, y, bar);
+                           });
         }
         __syncwarp();
       }
@@ -495,13 +518,15 @@ __device__ __forceinline__ void product_pair(const CUtensorMap *map_a,
         mbar_wait_pipeline(&full[i % kStages], i / kStages & 1u, p.timeout_ns);
   } else if (warp == 1 && rank == 0) {
     const bool leader = elect_one();
-    const uint32_t desc = mma_desc<A_MN, B_MN>(2 * kBM, p.tile_n, p.is_f16 != 0);
+    const uint32_t whole = mma_desc<A_MN, B_MN>(2 * kBM, p.tile_n, p.is_f16 != 0);
+    const uint32_t part = mma_desc<A_MN, B_MN>(2 * kBM, p.tile_n / 2, p.is_f16 != 0);
     const uint32_t ring_addr = smem_addr(ring);
     RingPlace at;
     uint32_t t = 0;
     bool ok = true, ready = false;
-    for (uint32_t tile = first; tile < tiles && ok; tile += step, ++t) {
+    for (uint32_t i = first; i < items && ok; i += step, ++t) {
       const uint32_t set = t & 1u;
+      const uint32_t desc = i < p.full_tiles ? whole : part;
       ok = __all_sync(0xFFFFFFFFu, mbar_wait_pipeline(&sums_empty[set],
                                                       (t >> 1 & 1u) ^ 1u,
                                                       p.timeout_ns));
@@ -530,31 +555,30 @@ __device__ __forceinline__ void product_pair(const CUtensorMap *map_a,
     }
   } else if (warp >= 4) {
     const uint32_t quarter = warp & 3u, side = (warp - 4) / 4;
-    const uint32_t blocks = half_n / 16;  // of this warp in a tile
     const uint32_t row_in = rank * kBM + quarter * 32;
     Ahead<FORM> ahead(p, slots + (warp - 4) * (kAhead1 + 1) * kSlotBytes, lane);
-    uint32_t next_tile = first, next_block = 0;
+    // A warp takes its half of a tile's columns in blocks of 16.
+    uint32_t next_item = first, next_block = 0;
     auto fetch_next = [&] {
-      uint32_t tm = 0, tn = 0;
-      if (next_tile < tiles)
-        tile_of(next_tile, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
-      ahead.fetch(tm * 2 * kBM + row_in,
-                  tn * p.tile_n + side * half_n + next_block * 16, next_tile < tiles);
-      if (++next_block == blocks) {
+      Item next = {0, 0, 16};
+      if (next_item < items)
+        next = item_of(next_item);
+      ahead.fetch(next.row0 + row_in, next.col0 + side * next.half_n + next_block * 16,
+                  next_item < items);
+      if (++next_block >= next.half_n / 16) {
         next_block = 0;
-        next_tile += step;
+        next_item += step;
       }
     };
     for (uint32_t i = 0; i < ahead.depth; ++i)
       fetch_next();
     uint32_t t = 0;
-    for (uint32_t tile = first; tile < tiles; tile += step, ++t) {
-      uint32_t tm, tn;
-      tile_of(tile, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
-      const uint32_t row0 = tm * 2 * kBM + row_in;
+    for (uint32_t item_at = first; item_at < items; item_at += step, ++t) {
+      const Item item = item_of(item_at);
+      const uint32_t row0 = item.row0 + row_in, blocks = item.half_n / 16;
       const uint32_t set = t & 1u;
       if (FORM == HEXIR_PRODUCT_FORWARD && p.bias)
-        stage_bias(p, bias[warp - 4], tn * p.tile_n + side * half_n, half_n, lane);
+        stage_bias(p, bias[warp - 4], item.col0 + side * item.half_n, item.half_n, lane);
       // The whole warp leaves together: its TMEM loads are warp-wide.
       if (!__all_sync(0xFFFFFFFFu,
                       mbar_wait_pipeline(&sums_full[set], t >> 1 & 1u,
@@ -563,7 +587,7 @@ __device__ __forceinline__ void product_pair(const CUtensorMap *map_a,
       tc_fence_after();
       const uint32_t src = tmem + (quarter * 32u << 16) + set * 256u;
       for (uint32_t i = 0; i < blocks; ++i) {
-        const uint32_t c = side * half_n + i * 16;
+        const uint32_t c = side * item.half_n + i * 16;
         float v[16];
         __syncwarp();
         tmem_load16(src + c, v);
@@ -576,7 +600,7 @@ __device__ __forceinline__ void product_pair(const CUtensorMap *map_a,
         }
         uint8_t *slot = ahead.arrived();
         finish_block<FORM>(p, v, bias[warp - 4] + i * 16, slot, ahead.out(), row0,
-                           tn * p.tile_n + c, lane);
+                           item.col0 + c, lane);
         __syncwarp();
         fetch_next();
       }

@@ -413,13 +413,20 @@ enum ProductVariant { kPair = 1, kSingle = 2, kSkinny = 3, kGuardedLoads = 4 };
 struct ProductPlan {
   uint32_t variant = 0;
   uint32_t tile_n = 0, split = 1, stages = 0;
-  uint32_t tiles_m = 0, tiles_n = 0;
+  uint32_t tiles_m = 0, tiles_n = 0, full_tiles = 0;
   uint32_t tmem_cols = 0, ring = 0, smem = 0;
   std::string refusal;  // a forced kernel that cannot run this
 };
 
 uint32_t stage_bytes(uint32_t tile_n) {
   return HEXIR_PRODUCT_BM * 128u + tile_n * 128u;
+}
+
+// Tiles that CTA pairs take whole.  Those of a last turn that fills at most half
+// of the pairs are cut into halves of 128 columns, which take 0.7 of its time.
+uint64_t pair_full_tiles(uint64_t tiles, uint32_t tile_n, uint64_t pairs) {
+  const uint64_t over = tiles % pairs;
+  return tile_n == 256 && tiles > pairs && 2 * over <= pairs ? tiles - over : tiles;
 }
 
 // Modelled microseconds of a product: a base, and per wave of tiles (of pairs,
@@ -445,8 +452,10 @@ double modelled_us(uint32_t variant, uint32_t tile_n, uint32_t split, uint32_t r
     const Cost &c = kPairCost[slots][wide];
     const uint64_t tiles =
         static_cast<uint64_t>(ceil_div(rows, 256)) * ceil_div(cols, tile_n);
-    const uint64_t waves = (tiles + sms / 2 - 1) / (sms / 2);
-    return c.base + waves * (k_tiles * c.k_tile + c.wave);
+    const uint64_t pairs = sms / 2, whole = pair_full_tiles(tiles, tile_n, pairs);
+    const Cost &half = kPairCost[slots][0];
+    return c.base + (whole + pairs - 1) / pairs * (k_tiles * c.k_tile + c.wave) +
+           (whole < tiles ? k_tiles * half.k_tile + half.wave : 0.0);
   }
   const Cost &c = kSingleCost[wide][split >= 8 ? 3 : split / 2];
   const uint64_t ctas =
@@ -535,6 +544,8 @@ ProductPlan plan_product(uint32_t op, uint32_t m, uint32_t n, uint32_t k,
     if (p.variant == kPair) {
       p.tiles_m = ceil_div(rows, 2 * HEXIR_PRODUCT_BM);
       p.tiles_n = ceil_div(cols, p.tile_n);
+      p.full_tiles = static_cast<uint32_t>(pair_full_tiles(
+          static_cast<uint64_t>(p.tiles_m) * p.tiles_n, p.tile_n, sms / 2));
       p.smem = HEXIR_PAIR_SMEM_BYTES;
       return p;
     }
@@ -614,6 +625,7 @@ hexir_status_t launch_product(Call &call, uint32_t op, uint32_t m, uint32_t n,
   args.tiles_m = p.tiles_m;
   args.tiles_n = p.tiles_n;
   args.group_m = std::min<uint32_t>(8, p.tiles_m);
+  args.full_tiles = p.full_tiles;
   args.tile_n = p.tile_n;
   args.k_tiles = ceil_div(args.depth, HEXIR_PRODUCT_BK);
   args.split = p.split;
@@ -625,7 +637,7 @@ hexir_status_t launch_product(Call &call, uint32_t op, uint32_t m, uint32_t n,
   const unsigned grid = static_cast<unsigned>(tiles * p.split);
   Operand a = {args.a, args.lda, a_mn, args.rows, HEXIR_PRODUCT_BM};
   Operand b = {args.b, args.ldb, b_mn, args.cols,
-               p.variant == kPair ? p.tile_n / 2 : p.tile_n};
+               p.variant == kPair ? 64u : p.tile_n};
   if (p.variant == kSkinny) {
     // The transposed product: the weight's columns are the tile's rows.
     const Operand x = {args.a, args.lda, false, args.rows, p.tile_n};

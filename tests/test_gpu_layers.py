@@ -759,3 +759,33 @@ def test_launch_faults_are_reported_and_leave_nothing_behind():
     with pytest.raises(_ffi.HexirError) as err:
         hx.cuda_layer_norm(99, x.data_ptr(), y.data_ptr(), 64, 64, "bf16")
     assert err.value.status == _ffi.ERROR_DEVICE
+
+
+@pytest.mark.parametrize("rows,cols", [(2200, 2296), (2560, 1928), (1000, 5136)])
+def test_pairs_that_cut_the_last_tiles_in_two(rows, cols):
+    """More 256 x 256 tiles than CTA pairs by a few: the last ones are halves,
+    one of them possibly beyond the columns."""
+    depth, flags = 136, PAIR | _ffi.LINEAR_TILE(256)
+    rng = np.random.default_rng(cols)
+    a, b = inputs(rng, rows, depth, "bf16"), inputs(rng, depth, cols, "bf16", scale=0.1)
+    bt, at = Tensor(cols, depth, "bf16", data=b.numpy().T), \
+        Tensor(depth, rows, "bf16", data=a.numpy().T)
+    r, z = inputs(rng, rows, cols, "bf16"), Tensor(rows, cols, "bf16")
+    bias = inputs(rng, 1, cols, "bf16")
+    y, dx, dw = (Tensor(rows, cols, "bf16") for _ in range(3))
+    on = stream()
+    hx.cuda_linear(0, a.ptr, b.ptr, y.ptr, rows, cols, depth, "bf16", "tanh",
+                   bias=bias.ptr, residual=r.ptr, preact=z.ptr, flags=flags, stream=on)
+    hx.cuda_linear_input_grad(0, a.ptr, bt.ptr, dx.ptr, rows, depth, cols, "bf16",
+                              "swish", preact=r.ptr, flags=flags, stream=on)
+    hx.cuda_linear_weight_grad(0, at.ptr, b.ptr, dw.ptr, depth, cols, rows, "bf16",
+                               flags=flags, stream=on)
+    sync()
+    for t in (y, z, dx, dw):
+        t.check_frame()
+    want = ref.linear(a.numpy(), b.numpy(), bias.numpy()[0], "tanh", r.numpy(), "bf16")
+    assert_within(y.numpy(), want[0], want[1], "y")
+    assert_within(z.numpy(), want[2], want[3], "z")
+    assert_within(dx.numpy(), *ref.product(a.numpy(), b.numpy(), "bf16", "swish",
+                                           r.numpy()), "dx")
+    assert_within(dw.numpy(), *ref.product(a.numpy(), b.numpy(), "bf16"), "dw")
