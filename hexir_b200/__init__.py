@@ -5,7 +5,9 @@ epilogue) and the elementwise hexir.relu / hexir.add (plus, on request, the
 dialect's declared activations leaky_relu ... mish), behind the reference's
 surface: the .hxb module format, the HAL / module / VM C ABI
 (include/hexir_runtime), the hexir-run tool, and the -placement= syntax
-(extended with cuda:N and row-sharded cuda:F-L).  See include/ for the C ABI;
+(extended with cuda:N and row-sharded cuda:F-L).  Beside it, on device
+pointers: the bf16 / f16 linear with bias, activation and residual, its
+gradients, and layer norm with its gradient.  See include/ for the C ABI;
 this package is a thin Python face over it.
 """
 

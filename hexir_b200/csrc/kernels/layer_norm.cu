@@ -1110,8 +1110,8 @@ __device__ __forceinline__ void output_grad_join(
   NORM_GRAD(SUFFIX, T, 32, 8, w, kWhole, 2, 6)                                 \
   NORM_GRAD(SUFFIX, T, 32, 16, w, kWhole, 2, 4)                                \
   NORM_GRAD(SUFFIX, T, 64, 16, w, kWhole, 2, 4)                                \
-  NORM_GRAD(SUFFIX, T, 128, 16, w, kWhole, 2, 4)                               \
-  NORM_GRAD(SUFFIX, T, 256, 16, w, kWhole, 2, 4)                               \
+  NORM_GRAD(SUFFIX, T, 128, 16, w, kWhole, 2, 3)                               \
+  NORM_GRAD(SUFFIX, T, 256, 16, w, kWhole, 2, 3)                               \
   NORM_GRAD(SUFFIX, T, 384, 16, w, kWhole, 1, 4)                               \
   NORM_GRAD(SUFFIX, T, 512, 16, w, kWhole, 1, 3)                               \
   NORM_GRAD(SUFFIX, T, 1024, 16, w, kWhole, 1, 2)                              \

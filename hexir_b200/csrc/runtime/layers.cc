@@ -97,8 +97,8 @@ constexpr NormShape kNormGrad[3][kMaxShapes] = {
     {{"w32x8", 32, 8, kWhole, 6},
      {"w32x16", 32, 16, kWhole, 4},
      {"w64x16", 64, 16, kWhole, 4},
-     {"w128x16", 128, 16, kWhole, 4},
-     {"w256x16", 256, 16, kWhole, 4},
+     {"w128x16", 128, 16, kWhole, 3},
+     {"w256x16", 256, 16, kWhole, 3},
      {"w384x16", 384, 16, kWhole, 4},
      {"w512x16", 512, 16, kWhole, 3},
      {"w1024x16", 1024, 16, kWhole, 2},

@@ -21,9 +21,14 @@
  * the caller passes it, and calls that may overlap pass different scratch.
  * Results do not depend on timing: every sum has a fixed order.
  *
- * An output may not overlap an input or another output, except that y (dx)
- * and residual may be the same tensor (same pointer and stride), and that dz
- * may be dy.
+ * An output may not overlap an input or another output, except that two may
+ * be the same tensor (same pointer and stride) where one takes the other's
+ * place row by row: y (dx) and residual, dz and dy, a norm's y and x, a
+ * norm's dx and dy.  Inputs may overlap each other.
+ *
+ * The first of these calls on a device loads their device code, which a
+ * stream capture does not allow: make one (of any size, an empty one will do)
+ * before capturing.
  */
 #ifndef HEXIR_B200_LAYERS_H
 #define HEXIR_B200_LAYERS_H
