@@ -478,6 +478,13 @@ def _activation(act) -> int:
     return _ffi.LINEAR_ACTIVATIONS[act]
 
 
+def _counts(together: int) -> None:
+    """Refuses counts that the calls' 32-bit fields would cut off: `together`
+    is all of them or-ed."""
+    if together >> 32:
+        raise ValueError("a negative size or flag, or one of 2**32 or more")
+
+
 def cuda_linear(ordinal: int, x: int, w: int, y: int, m: int, n: int, k: int,
                 dtype: str = "bf16", activation: str = "none", *, bias: int = 0,
                 residual: int = 0, preact: int = 0, ldx: int = 0, ldw: int = 0,
@@ -485,6 +492,7 @@ def cuda_linear(ordinal: int, x: int, w: int, y: int, m: int, n: int, k: int,
                 stream: int = 0) -> None:
     """y = activation(x . w + bias) + residual for x [m][k], w [k][n], bf16 or
     f16; preact (optional) receives x . w + bias (hexir_cuda_linear)."""
+    _counts(m | n | k | flags)
     call = _ffi.LinearCall(_dtype(dtype), _activation(activation), m, n, k, flags,
                            x, w, bias, residual, preact, y, ldx, ldw, ldr, ldp, ldy)
     check(lib().hexir_cuda_linear(ordinal, C.byref(call), stream or None),
@@ -500,6 +508,7 @@ def cuda_linear_output_grad(ordinal: int, dy: int, m: int, n: int,
     """dz = dy * activation'(preact) and dbias = the column sums of dz
     (hexir_cuda_linear_output_grad); dbias needs a workspace of
     grad_workspace_bytes(n, dtype)."""
+    _counts(m | n)
     call = _ffi.LinearOutputGradCall(_dtype(dtype), _activation(activation), m, n,
                                      dy, preact, dz, dbias, workspace,
                                      workspace_bytes, lddy, ldp, lddz)
@@ -516,6 +525,7 @@ def cuda_linear_input_grad(ordinal: int, dz: int, w: int, dx: int, m: int, n: in
     """dx = (dz . w^T) * activation'(preact) + residual, with the activation
     and preactivations of the layer whose output this layer's input was
     (hexir_cuda_linear_input_grad)."""
+    _counts(m | n | k | flags)
     call = _ffi.LinearInputGradCall(_dtype(dtype), _activation(activation), m, n, k,
                                     flags, dz, w, preact, residual, dx, lddz, ldw,
                                     ldp, ldr, lddx)
@@ -528,6 +538,7 @@ def cuda_linear_weight_grad(ordinal: int, x: int, dz: int, dw: int, m: int, n: i
                             lddz: int = 0, lddw: int = 0, flags: int = 0,
                             stream: int = 0) -> None:
     """dw = x^T . dz, [k][n] (hexir_cuda_linear_weight_grad)."""
+    _counts(m | n | k | flags)
     call = _ffi.LinearWeightGradCall(_dtype(dtype), 0, m, n, k, flags, x, dz, dw,
                                      ldx, lddz, lddw)
     check(lib().hexir_cuda_linear_weight_grad(ordinal, C.byref(call),
@@ -560,6 +571,7 @@ def cuda_layer_norm(ordinal: int, x: int, y: int, rows: int, cols: int,
                     ldy: int = 0, stream: int = 0) -> None:
     """y = (x - mean) * rstd * gamma + beta along each row; mean and rstd
     (optional outputs, [rows]) are f32, f64 for f64 (hexir_cuda_layer_norm)."""
+    _counts(cols | (rows if rows < 0 else 0))
     call = _ffi.LayerNormCall(_dtype(dtype), cols, rows, eps, x, gamma, beta, y,
                               mean, rstd, ldx, ldy)
     check(lib().hexir_cuda_layer_norm(ordinal, C.byref(call), stream or None),
@@ -575,6 +587,7 @@ def cuda_layer_norm_grad(ordinal: int, dy: int, x: int, mean: int, rstd: int,
     """Layer norm's gradient: dx (+ residual), dgamma and dbeta
     (hexir_cuda_layer_norm_grad); dgamma and dbeta need a workspace of
     grad_workspace_bytes(cols, dtype)."""
+    _counts(cols | (rows if rows < 0 else 0))
     call = _ffi.LayerNormGradCall(_dtype(dtype), cols, rows, dy, x, mean, rstd,
                                   gamma, residual, dx, dgamma, dbeta, workspace,
                                   workspace_bytes, lddy, ldx, ldr, lddx)

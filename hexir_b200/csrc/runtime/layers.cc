@@ -28,7 +28,8 @@ enum Layout { kWhole, kShifted, kAny };
 
 // The norm kernels: the name's end in layer_norm.cu, threads per row (blocks
 // have 256 at least, several rows where a row has less), elements per thread,
-// layout, and the gradient's rows of the ring.  A row runs the first kernel of its layout that holds it.
+// layout, and the gradient's rows of the ring.  A row runs the first kernel of
+// its layout that holds it.
 struct NormShape {
   const char *name;
   uint32_t threads, elements;

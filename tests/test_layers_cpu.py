@@ -169,3 +169,20 @@ def test_the_reference_slopes_are_the_activations_derivatives():
     for name in ref.ACTS:
         diff = (ref.act(name, z + h) - ref.act(name, z - h)) / (2 * h)
         assert np.abs(diff - ref.slope(name, z)).max() < 1e-9, name
+
+
+def test_counts_beyond_32_bits_are_refused_in_python():
+    """The calls' fields would cut them off without a word."""
+    for bad in (1 << 32, (1 << 32) + 5, -1):
+        for call in (lambda: hx.cuda_linear(0, 16, 16, 16, bad, 8, 8),
+                     lambda: hx.cuda_linear(0, 16, 16, 16, 8, 8, bad),
+                     lambda: hx.cuda_linear(0, 16, 16, 16, 8, 8, 8, flags=bad),
+                     lambda: hx.cuda_linear_output_grad(0, 16, bad, 8),
+                     lambda: hx.cuda_linear_input_grad(0, 16, 16, 16, 8, bad, 8),
+                     lambda: hx.cuda_linear_weight_grad(0, 16, 16, 16, 8, 8, bad),
+                     lambda: hx.cuda_layer_norm(0, 16, 16, 8, bad),
+                     lambda: hx.cuda_layer_norm_grad(0, 16, 16, 16, 16, 16, 8, bad)):
+            with pytest.raises(ValueError):
+                call()
+    with pytest.raises(ValueError):
+        hx.cuda_layer_norm(0, 16, 16, -1, 8)
