@@ -789,3 +789,76 @@ def test_pairs_that_cut_the_last_tiles_in_two(rows, cols):
     assert_within(dx.numpy(), *ref.product(a.numpy(), b.numpy(), "bf16", "swish",
                                            r.numpy()), "dx")
     assert_within(dw.numpy(), *ref.product(a.numpy(), b.numpy(), "bf16"), "dw")
+
+
+@pytest.mark.parametrize("dtype,rows,cols,pad,shift", [
+    ("f32", 1500, 1025, 0, 0), ("f32", 700, 2600, 1, 3), ("f32", 640, 4097, 2, 1),
+    ("f32", 330, 5003, 0, 2), ("f32", 310, 8190, 1, 1), ("f32", 300, 9001, 0, 0),
+    ("bf16", 1500, 1001, 0, 5), ("f16", 900, 2049, 2, 1), ("bf16", 620, 4097, 0, 7),
+    ("bf16", 500, 5999, 4, 3), ("f16", 320, 8001, 0, 1), ("f64", 1300, 1025, 0, 1)])
+def test_norms_of_many_rows_off_16_bytes(dtype, rows, cols, pad, shift):
+    """Blocks that take several rows each, all cut at the same place, up to the
+    tensor's last; the gradient in place of dy."""
+    rng = np.random.default_rng(rows)
+    x = inputs(rng, rows, cols, dtype, pad, shift, mean=2.0)
+    dy = inputs(rng, rows, cols, dtype, pad, shift)
+    g, b = inputs(rng, 1, cols, dtype), inputs(rng, 1, cols, dtype)
+    wide = "f64" if dtype == "f64" else "f32"
+    mean, rstd = Tensor(1, rows, wide), Tensor(1, rows, wide)
+    y = Tensor(rows, cols, dtype, pad, shift)
+    hx.cuda_layer_norm(0, x.ptr, y.ptr, rows, cols, dtype, gamma=g.ptr, beta=b.ptr,
+                       mean=mean.ptr, rstd=rstd.ptr, ldx=x.ld, ldy=y.ld,
+                       stream=stream())
+    sync()
+    y.check_frame()
+    want = ref.layer_norm(x.numpy(), g.numpy()[0], b.numpy()[0], 1e-5, dtype)
+    for got, (w, bound), what in ((y.numpy(), want[0], "y"),
+                                  (mean.numpy()[0], want[1], "mean"),
+                                  (rstd.numpy()[0], want[2], "rstd")):
+        assert_within(got, w, bound, what)
+    want = ref.layer_norm_grad(dy.numpy(), x.numpy(), mean.numpy()[0], rstd.numpy()[0],
+                               g.numpy()[0], None, dtype)
+    dgamma, dbeta = Tensor(1, cols, dtype), Tensor(1, cols, dtype)
+    work = torch.empty(hx.grad_workspace_bytes(cols, dtype), device="cuda",
+                       dtype=torch.uint8)
+    hx.cuda_layer_norm_grad(0, dy.ptr, x.ptr, mean.ptr, rstd.ptr, dy.ptr, rows, cols,
+                            dtype, gamma=g.ptr, dgamma=dgamma.ptr, dbeta=dbeta.ptr,
+                            workspace=work.data_ptr(), workspace_bytes=work.numel(),
+                            lddy=dy.ld, ldx=x.ld, lddx=dy.ld, stream=stream())
+    sync()
+    dy.check_frame()
+    assert_within(dy.numpy(), *want[0], "dx")
+    assert_within(dgamma.numpy()[0], *want[1], "dgamma")
+    assert_within(dbeta.numpy()[0], *want[2], "dbeta")
+
+
+@pytest.mark.parametrize("flags", [0, GUARDED | _ffi.LINEAR_SPLIT(1),
+                                   GUARDED | _ffi.LINEAR_SPLIT(4)])
+@pytest.mark.parametrize("shift", [0, 1, 6])
+def test_guarded_loads_at_the_ends_of_their_memory(flags, shift):
+    """Operands that begin and end exactly where their buffers do (the first
+    and last blocks reach outside them), at every phase of a row."""
+    for m, n, k in ((129, 131, 193), (7, 9, 64), (130, 3, 129), (1, 1, 1)):
+        rng = np.random.default_rng(m + shift)
+
+        def exact(rows, cols):
+            flat = torch.empty(shift + rows * cols, device="cuda", dtype=torch.bfloat16)
+            t = flat[shift:].view(rows, cols)
+            t.copy_(torch.as_tensor(normal(rng, (rows, cols))))
+            return t
+        x, w, wt, xt = exact(m, k), exact(k, n), exact(n, k), exact(k, m)
+        outs = [Tensor(m, n, "bf16") for _ in range(3)]
+        on = stream()
+        hx.cuda_linear(0, x.data_ptr(), w.data_ptr(), outs[0].ptr, m, n, k, flags=flags,
+                       stream=on)
+        hx.cuda_linear_input_grad(0, x.data_ptr(), wt.data_ptr(), outs[1].ptr, m, k, n,
+                                  flags=flags, stream=on)
+        hx.cuda_linear_weight_grad(0, xt.data_ptr(), w.data_ptr(), outs[2].ptr, k, n, m,
+                                   flags=flags, stream=on)
+        sync()
+        a = {id(t): t.double().cpu().numpy() for t in (x, w, wt, xt)}
+        for out, left, right in ((outs[0], a[id(x)], a[id(w)]),
+                                 (outs[1], a[id(x)], a[id(wt)].T),
+                                 (outs[2], a[id(xt)].T, a[id(w)])):
+            out.check_frame()
+            assert_within(out.numpy(), *ref.product(left, right, "bf16"), "product")
