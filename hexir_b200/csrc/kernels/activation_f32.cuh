@@ -15,7 +15,6 @@
 
 namespace hexir {
 
-constexpr uint32_t kActNone = 0u;
 constexpr uint32_t kActRelu = 3u;
 
 // 2^x, and e^x; subnormal results are kept.

@@ -659,10 +659,11 @@ __device__ __forceinline__ uint4 load_now(uintptr_t at) {
 
 // One thread's chunks of an operand's 128 x 64 tiles: chunk i is 8 elements of
 // 128-byte row (i * 64 + warp / 8 * 32 + lane / 8 * 8 + warp % 8) of the stage.
-// The chunks of a warp, in every tile, start at the same byte of a 16-byte block: their rows are
-// 8 apart (and 64 elements or 64 values of the sum), and each of these is a
-// multiple of 16 bytes whatever the stride.  So the words to shift by are the
-// warp's, taken by a branch, and only halves are shifted by instructions.
+// The chunks of a warp, in every tile, start at the same byte of a 16-byte
+// block: their rows are 8 apart (and 64 elements or 64 values of the sum), and
+// each of these is a multiple of 16 bytes whatever the stride.  So the words to
+// shift by are the warp's, taken by a branch, and only halves are shifted by
+// instructions.
 //
 // A k tile wholly inside the operand along the sum, whose blocks lie wholly
 // inside the tensor's memory (from its first element to its last, gaps between
@@ -734,8 +735,8 @@ struct GuardedOperand {
     k0 = MN ? row0 : column;
     dst0 = row0 * 128 + ((lane % 8 ^ warp % 8) << 4);
     // Within a warp the major index is the same but for multiples of 8.
-    shift = static_cast<uint32_t>(
-                first + ((MN ? 0 : side0) + static_cast<uint64_t>(warp % 8)) * ld * 2) & 15u;
+    const uint64_t major = (MN ? 0 : side0) + warp % 8;
+    shift = static_cast<uint32_t>(first + major * ld * 2) & 15u;
     side_counts = 0;
 #pragma unroll
     for (uint32_t i = 0; i < kChunks; ++i) {
