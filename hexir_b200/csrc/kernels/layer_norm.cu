@@ -21,6 +21,7 @@
 #include "activation_f32.cuh"
 #include "common.cuh"
 #include "layers_abi.h"
+#include "norm_ring.h"
 #include "two.cuh"
 
 using namespace hexir;
@@ -566,10 +567,11 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void *src) {
 // its sums of dy * xhat and dy in partial row b.
 //
 // The rows to come (x, dy and the residual) are copied into a ring of DEPTH
-// rows in shared memory.  Every thread copies and reads its own packs alone,
-// so the ring needs no barrier, and the registers hold the column sums
-// instead of rows in flight (with one row ahead in registers, two blocks fit
-// an SM and the loads' latency was 5 of 9 cycles between instructions).
+// rows in shared memory.  Every thread zeroes, copies and reads its own places
+// alone (norm_ring.h), so the ring needs no barrier, and the registers hold the
+// column sums instead of rows in flight (with one row ahead in registers, two
+// blocks fit an SM and the loads' latency was 5 of 9 cycles between
+// instructions).
 template <typename T, int TH, int NE, int LAYOUT, int DEPTH>
 __device__ __forceinline__ void norm_grad_rows(
     const hexir_layer_norm_grad_args_t &p) {
@@ -594,11 +596,14 @@ __device__ __forceinline__ void norm_grad_rows(
   uint64_t row = (uint64_t)blockIdx.x * kRows + group;
   const Lay lay(tid, p.cols, x_rows + row * p.ldx);
   const uint32_t tensors = res_rows ? 3 : 2;
-  uint4 *mine = ring + threadIdx.x;
-  // Rows of single elements: the ring holds them one by one, so that a warp's
-  // accesses fall into different banks.
+  // Rows of single elements: the ring holds them one by one.
   constexpr bool kSingles = LAYOUT == kAny && sizeof(T) >= 4;
-  T *singles = reinterpret_cast<T *>(ring) + threadIdx.x;
+  // Element j of this thread's pack `pack` of the ring; with j = 0, the pack
+  // itself where the ring holds packs.
+  auto ring_at = [&](uint32_t pack, uint32_t j) {
+    return reinterpret_cast<T *>(ring) +
+           NormRing<kN, kBlock, kSingles>::at(pack, j, threadIdx.x);
+  };
   const uint64_t last = p.rows - 1;
 
   Two<R> dgamma[NE / 2], dbeta[NE / 2];
@@ -618,9 +623,23 @@ __device__ __forceinline__ void norm_grad_rows(
       g[i] = lay.parameter(static_cast<const T *>(p.gamma), i);
     }
   }
-  // Places that no copy fills stay 0.
-  for (uint32_t i = 0; i < DEPTH * tensors * kPacks; ++i)
-    mine[i * kBlock] = make_uint4(0, 0, 0, 0);
+  // The places that no copy fills are 0, and those alone are zeroed: nothing
+  // orders a plain store before a copy to the same place.  (16-bit single
+  // elements are stored as whole packs, zeros included.)
+  for (uint32_t s = 0; s < DEPTH * tensors; ++s) {
+#pragma unroll
+    for (int i = 0; i < kPacks; ++i) {
+      const uint32_t pack = s * kPacks + i;
+      if (kSingles) {
+#pragma unroll
+        for (int j = 0; j < kN; ++j)
+          if (lay.column(i, j) >= p.cols)
+            *ring_at(pack, j) = narrow<T>(R(0));
+      } else if (LAYOUT != kAny && !lay.some(i)) {
+        *reinterpret_cast<uint4 *>(ring_at(pack, 0)) = make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
 
   auto fetch = [&](uint64_t at, uint32_t stage) {
     if (at < p.rows) {
@@ -636,14 +655,14 @@ __device__ __forceinline__ void norm_grad_rows(
 #pragma unroll
         for (int i = 0; i < kPacks; ++i) {
           const uint32_t at_pack = (stage * tensors + t) * kPacks + i;
-          uint4 *dst = mine + at_pack * kBlock;
+          uint4 *dst = reinterpret_cast<uint4 *>(ring_at(at_pack, 0));
           if (kSingles) {
 #pragma unroll
             for (int j = 0; j < kN; ++j) {
               const uint32_t c = lay.column(i, j);
               if (c < p.cols)
                 copy_async<sizeof(T) >= 4 ? sizeof(T) : 4>(
-                    smem_addr(singles + (at_pack * kN + j) * kBlock), src[t] + c);
+                    smem_addr(ring_at(at_pack, j)), src[t] + c);
             }
           } else if (LAYOUT == kAny) {
             *dst = lay.template load_pack<true>(src[t], i, spans[t], false).w;
@@ -670,10 +689,10 @@ __device__ __forceinline__ void norm_grad_rows(
       T e[kN];
 #pragma unroll
       for (int j = 0; j < kN; ++j)
-        e[j] = singles[(at_pack * kN + j) * kBlock];
+        e[j] = *ring_at(at_pack, j);
       v.w = *reinterpret_cast<const uint4 *>(e);
     } else {
-      v.w = mine[at_pack * kBlock];
+      v.w = *reinterpret_cast<const uint4 *>(ring_at(at_pack, 0));
     }
     if (lay.warp_cut(i))
       v.w = lay.inside(v.w, i);

@@ -862,3 +862,62 @@ def test_guarded_loads_at_the_ends_of_their_memory(flags, shift):
                                  (outs[2], a[id(xt)].T, a[id(w)])):
             out.check_frame()
             assert_within(out.numpy(), *ref.product(left, right, "bf16"), "product")
+
+
+# Rows whose tensors lie differently over 16 bytes, element by element: every
+# length of such kernels, below its limit.
+SINGLES = [("f32", 257, 0), ("f32", 1001, 0), ("f32", 511, 2), ("f32", 1500, 2),
+           ("f32", 2049, 2), ("f32", 4095, 2), ("f32", 8000, 2), ("f64", 255, 0),
+           ("f64", 511, 0), ("f64", 1025, 0), ("f64", 2047, 0), ("f64", 4095, 1)]
+
+
+@pytest.mark.parametrize("dtype,cols,apart", SINGLES)
+def test_gradients_of_single_elements_repeat(dtype, cols, apart):
+    """The ring of rows of single elements: repeated with the inputs in turn in
+    L2 and out of it, after NaNs have gone through the same shared memory, with
+    and without dx and the residual, the gradients keep their bits, and they
+    are right."""
+    rng = np.random.default_rng(cols)
+    rows, wide = 600, "f64" if dtype == "f64" else "f32"
+    dy = inputs(rng, rows, cols, dtype, 1, 1)
+    x = inputs(rng, rows, cols, dtype, 1, 1 + apart, 2.0, 1.0)
+    residual = inputs(rng, rows, cols, dtype, 1, 1)
+    gamma = inputs(rng, 1, cols, dtype, scale=0.2, mean=1.0)
+    xd = x.numpy()
+    mean = Tensor(1, rows, wide, data=xd.mean(1))
+    rstd = Tensor(1, rows, wide, data=1 / np.sqrt(xd.var(1) + 1e-3))
+    nans = Tensor(rows, cols + 1, dtype, data=np.full((rows, cols + 1), np.nan))
+    nan_out = Tensor(rows, cols + 1, dtype, 0, 1)
+    dx = Tensor(rows, cols, dtype, 1, 1)
+    dgamma, dbeta = Tensor(1, cols, dtype), Tensor(1, cols, dtype)
+    size = hx.grad_workspace_bytes(cols, dtype)
+    work = torch.empty(size, device="cuda", dtype=torch.uint8)
+    flush = torch.empty(1 << 28, device="cuda", dtype=torch.uint8)
+    first = {}
+    for turn in range(24):
+        if turn % 4 < 2:
+            flush.fill_(turn)
+        if turn % 3 == 0:   # leaves NaN in the ring's memory
+            hx.cuda_layer_norm_grad(0, nans.ptr, nans.ptr, mean.ptr, rstd.ptr,
+                                    nan_out.ptr, rows, cols + 1, dtype,
+                                    residual=nans.ptr, stream=stream())
+        form = turn % 2     # with all of dx and the residual, or the sums alone
+        dx.view.fill_(FILL)
+        hx.cuda_layer_norm_grad(0, dy.ptr, x.ptr, mean.ptr, rstd.ptr,
+                                0 if form else dx.ptr, rows, cols, dtype,
+                                gamma=gamma.ptr, dgamma=dgamma.ptr, dbeta=dbeta.ptr,
+                                residual=0 if form else residual.ptr,
+                                workspace=work.data_ptr(), workspace_bytes=size,
+                                lddy=dy.ld, ldx=x.ld, lddx=dx.ld, ldr=residual.ld,
+                                stream=stream())
+        sync()
+        got = [t.view.clone() for t in (dgamma, dbeta, dx)]
+        for name, a, b in zip(("dgamma", "dbeta", "dx"), got,
+                              first.setdefault(form, got)):
+            assert torch.equal(a, b), f"{name}, turn {turn}"
+    want = ref.layer_norm_grad(dy.numpy(), xd, mean.numpy()[0], rstd.numpy()[0],
+                               gamma.numpy()[0], residual.numpy(), dtype)
+    assert_within(first[0][2].double().cpu().numpy(), *want[0], "dx")
+    for form in (0, 1):
+        for (w, bound), got, what in zip(want[1:], first[form], ("dgamma", "dbeta")):
+            assert_within(got.double().cpu().numpy()[0], w, bound, what)

@@ -186,3 +186,30 @@ def test_counts_beyond_32_bits_are_refused_in_python():
                 call()
     with pytest.raises(ValueError):
         hx.cuda_layer_norm(0, 16, 16, -1, 8)
+
+
+def host_program(name, where):
+    """A C++ test program that includes the kernels' own headers, built for
+    this host."""
+    import os
+    import shutil
+    import subprocess
+    here = os.path.dirname(os.path.abspath(__file__))
+    cc = shutil.which("g++") or shutil.which("c++")
+    if cc is None:
+        pytest.skip("no C++ compiler")
+    exe = str(where / name)
+    subprocess.run([cc, "-O1", "-std=c++17", "-Wall", "-o", exe,
+                    "-I", os.path.join(here, "..", "hexir_b200", "csrc"),
+                    os.path.join(here, name + ".cc")], check=True)
+    return subprocess.run([exe], check=True, capture_output=True,
+                          text=True).stdout.split()
+
+
+def test_every_place_of_the_norm_gradients_ring_is_one_threads(tmp_path):
+    """No barrier orders one thread's use of the ring against another's, so no
+    place may be two threads'; zeroed as packs, a ring of single elements has
+    places of other threads almost everywhere."""
+    bad, mixed4, mixed2 = map(int, host_program("norm_places", tmp_path))
+    assert bad == 0
+    assert mixed4 > 4000 and mixed2 > 1200   # of 4096 and of 1536 elements
