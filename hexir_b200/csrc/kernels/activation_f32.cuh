@@ -161,6 +161,18 @@ __device__ __forceinline__ void act_f32(uint32_t act, float (&v)[N]) {
   }
 }
 
+// z with magnitudes above 128 made 128, as a factor of something that is 0 to f32
+// from |z| = 105 on (and NaN for NaN).  An infinity, which a z beyond its type's
+// range is stored as, would make that product NaN.  One instruction: bounded by
+// a minimum and a maximum, the elementwise gradient took 6 to 14 % longer (gelu
+// 8192 x 8192 88 us before, 93 with two, 91 with one; the products' epilogues
+// are not slowed down by it).
+__device__ __forceinline__ float factor_near(float z) {
+  float r;
+  asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(z), "f"(128.0f));
+  return r;
+}
+
 // g[i] *= act'(z[i]).
 template <int N>
 __device__ __forceinline__ void slope_f32(uint32_t act, const float (&z)[N],
@@ -201,8 +213,9 @@ __device__ __forceinline__ void slope_f32(uint32_t act, const float (&z)[N],
         const Two<float> at = {z[i], z[i + 1]};
         Two<float> phi, e;
         normal_cdf(at, phi, e);
+        const Two<float> factor = {factor_near(z[i]), factor_near(z[i + 1])};
         const Two<float> s =
-            fma(mul(at, e), twice(0.39894228040143268f), phi);
+            fma(mul(factor, e), twice(0.39894228040143268f), phi);
         g[i] *= s.x;
         g[i + 1] *= s.y;
       }
@@ -212,7 +225,7 @@ __device__ __forceinline__ void slope_f32(uint32_t act, const float (&z)[N],
       for (int i = 0; i < N; ++i) {
         const float u = exp_near(-fabsf(z[i])), r = inverse_near(1.0f + u);
         const float s = z[i] > 0.0f ? r : u * r, c = z[i] > 0.0f ? u * r : r;
-        g[i] *= s * ::fmaf(z[i], c, 1.0f);
+        g[i] *= s * ::fmaf(factor_near(z[i]), c, 1.0f);
       }
       break;
     case HEXIR_ACT_MISH:
@@ -224,7 +237,7 @@ __device__ __forceinline__ void slope_f32(uint32_t act, const float (&z)[N],
         mish_parts(z[i], u, w, d);
         const float r = inverse_near(d);
         const float c = 4.0f * u * (1.0f + u) * (z[i] > 0.0f ? u : 1.0f);
-        g[i] *= ::fmaf(z[i] * c * r, r, w * r);
+        g[i] *= ::fmaf(factor_near(z[i]) * c * r, r, w * r);
       }
       break;
     default:

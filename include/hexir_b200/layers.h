@@ -91,7 +91,8 @@ hexir_status_t hexir_cuda_linear(int ordinal, const hexir_linear_call_t *call,
  * f32.  dy, preact and dz are [m][n] (bf16 or f16).  With
  * HEXIR_ACTIVATION_NONE preact is not read and dz may be NULL (dz is dy);
  * dbias may be NULL.  m == 0 gives a zero dbias.  act' at a corner is the
- * slope from the left (relu'(0) = 0).
+ * slope from the left (relu'(0) = 0), and at an infinity, which preact holds
+ * where z is beyond the type's range, its limit.
  * workspace: hexir_cuda_grad_workspace(n, dtype) bytes, 16-byte aligned,
  * when dbias is wanted; its contents need no initial value. */
 typedef struct {

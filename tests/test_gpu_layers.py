@@ -921,3 +921,64 @@ def test_gradients_of_single_elements_repeat(dtype, cols, apart):
     for form in (0, 1):
         for (w, bound), got, what in zip(want[1:], first[form], ("dgamma", "dbeta")):
             assert_within(got.double().cpu().numpy()[0], w, bound, what)
+
+
+LIMITS = {"none": (1, 1), "relu": (0, 1), "leaky_relu": (0.01, 1), "elu": (0, 1),
+          "sigmoid": (0, 0), "tanh": (0, 0), "gelu": (0, 1), "swish": (0, 1),
+          "mish": (0, 1)}
+
+
+@pytest.mark.parametrize("act", ref.ACTS)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_slopes_far_out_and_at_infinity_are_their_limits(act, dtype):
+    """From |z| = 128 on every slope is its limit to f32 (e^-128 is below its
+    smallest number), at the infinities too, where a type's largest value ends;
+    a NaN stays one.  dy times 0, 1 or 0.01 is rounded once."""
+    far = [128.0, 1e3, 1e4, 65504.0, float("inf")]
+    z = torch.tensor([[-v for v in far] + far + [float("nan")]], device="cuda")
+    z = z.repeat(40, 1).to(TORCH[dtype])
+    dy = torch.randn(z.shape, device="cuda").to(TORCH[dtype])
+    low, high = LIMITS[act]
+    slopes = torch.tensor([low] * 5 + [high] * 5, device="cuda")
+    want = (dy[:, :10].float() * slopes).to(TORCH[dtype])
+    m, n = z.shape
+    dz = torch.empty_like(dy)
+    hx.cuda_linear_output_grad(0, dy.data_ptr(), m, n, dtype, act, preact=z.data_ptr(),
+                               dz=dz.data_ptr(), stream=stream())
+    # The same through a product: dx = (dy . 1) act'(z).
+    one = torch.eye(n, device="cuda", dtype=TORCH[dtype])
+    clean = torch.where(torch.isnan(z), torch.zeros_like(z), z)
+    dx = torch.empty_like(dy)
+    hx.cuda_linear_input_grad(0, dy.data_ptr(), one.data_ptr(), dx.data_ptr(), m, n, n,
+                              dtype, act, preact=clean.data_ptr(), stream=stream())
+    sync()
+    assert bool((dz[:, :10] == want).all())
+    assert bool((dx[:, :10] == want).all())
+    assert bool(dx.isfinite().all())
+    if act not in ("none", "relu", "leaky_relu"):
+        assert bool(dz[:, 10].isnan().all())
+
+
+@pytest.mark.parametrize("act", ["gelu", "swish", "mish"])
+def test_preactivations_beyond_f16_have_finite_gradients(act):
+    """z = -102400 and 102400: y has its value (0, or beyond f16), z is stored
+    as an infinity, and the slope there is 0 or 1."""
+    m, n, k = 20, 16, 64
+    x = torch.full((m, k), 40.0, device="cuda", dtype=torch.float16)
+    w = torch.full((k, n), 40.0, device="cuda", dtype=torch.float16)
+    w[:, ::2] = -40.0
+    y, z, dz = (torch.empty(m, n, device="cuda", dtype=torch.float16) for _ in range(3))
+    dy = torch.randn(m, n, device="cuda").half()
+    db = torch.empty(n, device="cuda", dtype=torch.float16)
+    work = torch.empty(hx.grad_workspace_bytes(n, "f16"), device="cuda",
+                       dtype=torch.uint8)
+    hx.cuda_linear(0, x.data_ptr(), w.data_ptr(), y.data_ptr(), m, n, k, "f16", act,
+                   preact=z.data_ptr(), stream=stream())
+    hx.cuda_linear_output_grad(0, dy.data_ptr(), m, n, "f16", act, preact=z.data_ptr(),
+                               dz=dz.data_ptr(), dbias=db.data_ptr(),
+                               workspace=work.data_ptr(), workspace_bytes=work.numel(),
+                               stream=stream())
+    sync()
+    assert bool((y[:, ::2] == 0).all()) and bool(z.isinf().all())
+    assert bool((dz[:, ::2] == 0).all()) and bool((dz[:, 1::2] == dy[:, 1::2]).all())
+    assert bool(db.isfinite().all())
