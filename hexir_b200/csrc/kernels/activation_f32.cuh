@@ -26,7 +26,7 @@ __device__ __forceinline__ float exp2_near(float x) {
 __device__ __forceinline__ float exp_near(float x) {
   return exp2_near(1.4426950408889634f * x);
 }
-// 1 / x for x in [1, 5].
+// 1 / x for x >= 1 (0 from 2^126 on).
 __device__ __forceinline__ float inverse_near(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -73,7 +73,9 @@ __device__ __forceinline__ float sigmoid_near(float z) {
 // t P(t) e^(-u^2) with t = 1 / (1 + u / 2): P is smooth on the whole half
 // line, and its polynomial of degree 8 (least maximal relative error on
 // t in [1/6, 1], by reweighted least squares in extended precision) is within
-// 4.3e-8 of it.  Above 0, Phi(z) = 1 - Phi(-z).
+// 4.3e-8 of it.  Where t is below 1/6 (|z| > 14.1, without bound), e^(-z^2 / 2)
+// is below 2^-144, the last bits of f32's smallest numbers, or 0, and P, which
+// stays near 0.14, does not matter.  Above 0, Phi(z) = 1 - Phi(-z).
 __device__ __forceinline__ void normal_cdf(const Two<float> &z, Two<float> &phi,
                                            Two<float> &e) {
   const Two<float> t = {

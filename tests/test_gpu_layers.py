@@ -982,3 +982,30 @@ def test_preactivations_beyond_f16_have_finite_gradients(act):
     assert bool((y[:, ::2] == 0).all()) and bool(z.isinf().all())
     assert bool((dz[:, ::2] == 0).all()) and bool((dz[:, 1::2] == dy[:, 1::2]).all())
     assert bool(db.isfinite().all())
+
+
+@pytest.mark.parametrize("act", ref.ACTS)
+def test_activations_of_large_finite_sums(act):
+    """act(z) for z far beyond the fitted range of the normal distribution's
+    polynomial: to f32's precision z or its limit, so y has the rounded value."""
+    zs = torch.tensor([14.0, 14.5, 20.0, 40.0, 90.0, 128.0, 1e3, 1e10, 3e38],
+                      device="cuda")
+    zs = torch.cat([-zs, zs]).bfloat16()
+    n = zs.numel()
+    x = torch.ones(3, 1, device="cuda", dtype=torch.bfloat16)
+    y = torch.empty(3, n, device="cuda", dtype=torch.bfloat16)
+    hx.cuda_linear(0, x.data_ptr(), zs.data_ptr(), y.data_ptr(), 3, n, 1, "bf16", act,
+                   stream=stream())
+    sync()
+    z = zs.double().cpu().numpy()
+    want = np.where(z > 0, z, 0.0) if act in ("gelu", "swish", "mish") else ref.act(act, z)
+    if act in ("swish", "mish"):   # z e^z below, above z within its rounding
+        want = np.where(z < 0, z * np.exp(z.clip(-700, 0)), z)
+    # Below -87 exponentials are subnormal in f32: 2^-149 of absolute error,
+    # times z.  gelu at -14 is below 1e-43, the subnormals' last digits.
+    bound = np.abs(want) * (ref.HALF["bf16"] * 2 + (16 + 4 * np.abs(z).clip(0, 200))
+                            * ref.U32) + 2.0 ** -133 + 2.0 ** -149 * np.abs(z).clip(0, 128)
+    if act == "gelu":
+        bound = bound + 1e-43
+    for row in y.double().cpu().numpy():
+        assert_within(row, want, bound, act)
