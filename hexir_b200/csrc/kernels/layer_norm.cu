@@ -244,8 +244,8 @@ struct Row {
     return make_uint4(w.x & m[0], w.y & m[1], w.z & m[2], w.w & m[3]);
   }
   // The row's packs; a cut one may carry its neighbours' elements until
-  // clean() (which a load must not wait for).  `edge`: the tensor's first or
-  // last row, where such a pack may reach outside it.
+  // clean() (which a load must not wait for).  `edge`: such a pack may reach
+  // outside the tensor (norm_row_at_edge).
   __device__ __forceinline__ void load(const T *row, const Span &span, bool edge,
                                        Pack<T> (&v)[kPacks]) const {
 #pragma unroll
@@ -402,10 +402,9 @@ __device__ __forceinline__ void norm_rows(const hexir_layer_norm_args_t &p) {
   if (row >= p.rows)
     return;
   const Lay lay(tid, p.cols, x_rows + row * p.ldx);
-  const uint64_t last = p.rows - 1;
   const Span span = span_of(x_rows, p.ldx, p.rows, p.cols);
   Pack<T> x[kPacks], next[kPacks];
-  lay.load(x_rows + row * p.ldx, span, row == 0 || row == last, x);
+  lay.load(x_rows + row * p.ldx, span, norm_row_at_edge<kN>(row, p.rows, p.cols), x);
   // Shifted rows: gamma and beta as this row's packs lie, in shared memory.
   // Each thread reads back only what it writes here.
   uint4 *gamma_copy = copies + group * (2 * TH * kPacks);
@@ -423,7 +422,8 @@ __device__ __forceinline__ void norm_rows(const hexir_layer_norm_args_t &p) {
     const bool more = row + step < p.rows;
     lay.clean(x);
     if (more)
-      lay.load(x_rows + (row + step) * p.ldx, span, row + step == last, next);
+      lay.load(x_rows + (row + step) * p.ldx, span,
+               norm_row_at_edge<kN>(row + step, p.rows, p.cols), next);
     Two<R> sum2 = twice(R(0));
 #pragma unroll
     for (int i = 0; i < kPacks; ++i) {
@@ -604,7 +604,6 @@ __device__ __forceinline__ void norm_grad_rows(
     return reinterpret_cast<T *>(ring) +
            NormRing<kN, kBlock, kSingles>::at(pack, j, threadIdx.x);
   };
-  const uint64_t last = p.rows - 1;
 
   Two<R> dgamma[NE / 2], dbeta[NE / 2];
 #pragma unroll
@@ -643,6 +642,7 @@ __device__ __forceinline__ void norm_grad_rows(
 
   auto fetch = [&](uint64_t at, uint32_t stage) {
     if (at < p.rows) {
+      const bool edge = LAYOUT == kShifted && norm_row_at_edge<kN>(at, p.rows, p.cols);
       const T *src[3] = {x_rows + at * p.ldx, dy_rows + at * p.lddy,
                          res_rows ? res_rows + at * p.ldr : nullptr};
       const Span spans[3] = {span_of(x_rows, p.ldx, p.rows, p.cols),
@@ -668,7 +668,7 @@ __device__ __forceinline__ void norm_grad_rows(
             *dst = lay.template load_pack<true>(src[t], i, spans[t], false).w;
           } else {
             const T *from = src[t] + static_cast<int32_t>(lay.column(i, 0));
-            if (LAYOUT == kShifted && (at == 0 || at == last) && lay.warp_cut(i)) {
+            if (edge && lay.warp_cut(i)) {
               if (lay.apart(src[t], i, spans[t]))
                 *dst = gather_pack(src[t], lay.column(i, 0), p.cols);
               else if (lay.some(i))

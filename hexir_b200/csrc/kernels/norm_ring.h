@@ -1,7 +1,7 @@
 /*
  * norm_ring.h -- where the layer norm gradient's ring of rows (layer_norm.cu)
- * keeps each thread's elements in shared memory; also compiled for the host by
- * the tests.
+ * keeps each thread's elements in shared memory, and which rows' packs may reach
+ * outside their tensor; also compiled for the host by the tests.
  */
 #ifndef HEXIR_B200_NORM_RING_H
 #define HEXIR_B200_NORM_RING_H
@@ -34,6 +34,17 @@ struct NormRing {
                    : (pack * THREADS + thread) * PER + element;
   }
 };
+
+// Whether a pack of row `row` of `rows` may hold elements outside the tensor's
+// memory, for rows of `cols` elements that start anywhere and are at least that
+// far apart.  A pack reaches PER - 1 elements beyond its row at most.  Of rows as
+// long as that, the next one holds them; of shorter ones it takes up to PER
+// rows.
+template <uint32_t PER>
+HEXIR_HOST_DEVICE bool norm_row_at_edge(uint64_t row, uint64_t rows, uint32_t cols) {
+  const uint32_t near = cols >= PER ? 1u : PER;
+  return row < near || row + near >= rows;
+}
 
 }  // namespace hexir
 

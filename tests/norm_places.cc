@@ -1,5 +1,6 @@
-// The places of the layer norm gradient's ring (kernels/norm_ring.h), for every
-// thread: each is one thread's alone, and together they are the ring.
+// The rules of kernels/norm_ring.h: every place of the gradient's ring is one
+// thread's alone, and together they are the ring; a row whose 16-byte blocks
+// reach outside its tensor is an edge.
 #include <cstdint>
 #include <cstdio>
 #include <vector>
@@ -46,6 +47,27 @@ int mixed(uint32_t packs) {
   return other;
 }
 
+// Rows with a block outside the tensor's memory that no edge guards, and, of rows
+// of a pack or more, edges beside the first and the last row.
+template <uint32_t PER>
+int outside(int *needless) {
+  int bad = 0;
+  for (uint64_t offset = 0; offset < PER; ++offset)
+    for (uint64_t cols = 1; cols < 3 * PER; ++cols)
+      for (uint64_t ld = cols; ld < cols + PER + 2; ++ld)
+        for (uint64_t rows = 1; rows < 3 * PER; ++rows) {
+          const uint64_t first = 8 * PER + offset, last = first + (rows - 1) * ld + cols;
+          for (uint64_t row = 0; row < rows; ++row) {
+            const uint64_t begin = first + row * ld, end = begin + cols;
+            const uint64_t low = begin / PER * PER, high = (end + PER - 1) / PER * PER;
+            const bool edge = hexir::norm_row_at_edge<PER>(row, rows, cols);
+            bad += !edge && (low < first || high > last);
+            *needless += cols >= PER && edge && row != 0 && row != rows - 1;
+          }
+        }
+  return bad;
+}
+
 int main() {
   int bad = 0;
   for (uint32_t packs : {1u, 2u, 4u, 12u, 24u}) {
@@ -54,6 +76,9 @@ int main() {
            shared_or_missing<2, 512, true>(packs) + shared_or_missing<4, 512, false>(packs) +
            shared_or_missing<8, 256, false>(packs) + shared_or_missing<8, 1024, false>(packs);
   }
-  std::printf("%d %d %d\n", bad, mixed<4, 512>(2), mixed<2, 192>(4));
+  int needless = 0;
+  const int reach = outside<8>(&needless) + outside<4>(&needless);
+  std::printf("%d %d %d %d %d\n", bad, mixed<4, 512>(2), mixed<2, 192>(4), reach,
+              needless);
   return 0;
 }

@@ -1009,3 +1009,41 @@ def test_activations_of_large_finite_sums(act):
         bound = bound + 1e-43
     for row in y.double().cpu().numpy():
         assert_within(row, want, bound, act)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32", "f64"])
+@pytest.mark.parametrize("cols,pad", [(1, 0), (1, 1), (2, 0), (3, 0), (5, 1), (7, 0),
+                                      (8, 1)])
+def test_norms_of_rows_shorter_than_16_bytes(dtype, cols, pad):
+    """Several rows share a 16-byte block, at every offset of the tensor into
+    one; what lies around the tensors is NaN and does not reach the results."""
+    rows, per = 41, 16 // torch.empty(0, dtype=TORCH[dtype]).element_size()
+    wide = "f64" if dtype == "f64" else "f32"
+    rng = np.random.default_rng(cols)
+    for shift in range(per):
+        x, dy = (inputs(rng, rows, cols, dtype, pad, shift) for _ in range(2))
+        for t in (x, dy):
+            t.flat[:t.start] = float("nan")
+            t.flat[t.start + (rows - 1) * t.ld + cols:] = float("nan")
+        y, dx = (Tensor(rows, cols, dtype, pad, shift) for _ in range(2))
+        mean, rstd = Tensor(1, rows, wide), Tensor(1, rows, wide)
+        dgamma, dbeta = Tensor(1, cols, dtype), Tensor(1, cols, dtype)
+        size = hx.grad_workspace_bytes(cols, dtype)
+        work = torch.empty(size, device="cuda", dtype=torch.uint8)
+        hx.cuda_layer_norm(0, x.ptr, y.ptr, rows, cols, dtype, mean=mean.ptr,
+                           rstd=rstd.ptr, eps=0.5, ldx=x.ld, ldy=y.ld, stream=stream())
+        hx.cuda_layer_norm_grad(0, dy.ptr, x.ptr, mean.ptr, rstd.ptr, dx.ptr, rows,
+                                cols, dtype, dgamma=dgamma.ptr, dbeta=dbeta.ptr,
+                                workspace=work.data_ptr(), workspace_bytes=size,
+                                lddy=dy.ld, ldx=x.ld, lddx=dx.ld, stream=stream())
+        sync()
+        for t in (y, dx):
+            t.check_frame()
+        (want, bound), _, _ = ref.layer_norm(x.numpy(), None, None, 0.5, dtype)
+        assert_within(y.numpy(), want, bound, f"y, shift {shift}")
+        want = ref.layer_norm_grad(dy.numpy(), x.numpy(), mean.numpy()[0],
+                                   rstd.numpy()[0], None, None, dtype)
+        for got, (w, bound), what in ((dx.numpy(), want[0], "dx"),
+                                      (dgamma.numpy()[0], want[1], "dgamma"),
+                                      (dbeta.numpy()[0], want[2], "dbeta")):
+            assert_within(got, w, bound, f"{what}, shift {shift}")

@@ -210,6 +210,14 @@ def test_every_place_of_the_norm_gradients_ring_is_one_threads(tmp_path):
     """No barrier orders one thread's use of the ring against another's, so no
     place may be two threads'; zeroed as packs, a ring of single elements has
     places of other threads almost everywhere."""
-    bad, mixed4, mixed2 = map(int, host_program("norm_places", tmp_path))
+    bad, mixed4, mixed2 = map(int, host_program("norm_places", tmp_path)[:3])
     assert bad == 0
     assert mixed4 > 4000 and mixed2 > 1200   # of 4096 and of 1536 elements
+
+
+def test_rows_whose_blocks_reach_outside_their_tensor_are_edges(tmp_path):
+    """Every offset, row length, stride and count around a pack's: rows shorter
+    than a pack share the tensor's first and last block among several; of
+    longer ones only the first and the last row are edges."""
+    reach, needless = map(int, host_program("norm_places", tmp_path)[3:])
+    assert reach == 0 and needless == 0
