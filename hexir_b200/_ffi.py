@@ -53,6 +53,11 @@ LINEAR_FORCE_PAIR = 0x100
 LINEAR_FORCE_SINGLE = 0x200
 LINEAR_FORCE_SKINNY = 0x400
 LINEAR_FORCE_GUARDED = 0x800
+LINEAR_ALIGNED_ALL = 1
+LINEAR_ALIGNED_FIRST = 2
+LINEAR_ALIGNED_SECOND = 4
+LINEAR_ALIGNED_REST = 8
+LINEAR_PLAN_PLAIN = 0x1
 
 
 def LINEAR_SPLIT(s: int) -> int:

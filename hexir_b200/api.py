@@ -546,11 +546,17 @@ def cuda_linear_weight_grad(ordinal: int, x: int, dz: int, dw: int, m: int, n: i
           "hexir_cuda_linear_weight_grad")
 
 
-def linear_plan(op: str, m: int, n: int, k: int, aligned: bool = True,
-                flags: int = 0, ordinal: int = 0) -> tuple:
+def linear_plan(op: str, m: int, n: int, k: int, aligned: int = True,
+                flags: int = 0, ordinal: int = 0, *, plain: bool = False) -> tuple:
     """(variant, tile_n, split) a product would run with: op is "forward",
     "input_grad" or "weight_grad"; variant 1 = CTA pairs, 2 = single CTAs,
-    3 = skinny, 4 = guarded loads (hexir_cuda_linear_plan)."""
+    3 = skinny, 4 = guarded loads, 0 = none, for an empty output
+    (hexir_cuda_linear_plan).  aligned: whether all rows, of every tensor,
+    start on 16-byte boundaries, or those of the tensors of
+    _ffi.LINEAR_ALIGNED_*; plain: a call without residual and preact whose
+    slope it takes."""
+    if plain:
+        flags |= _ffi.LINEAR_PLAN_PLAIN
     ops = ("forward", "input_grad", "weight_grad")
     out = [C.c_uint32() for _ in range(3)]
     check(lib().hexir_cuda_linear_plan(ordinal, ops.index(op), m, n, k,

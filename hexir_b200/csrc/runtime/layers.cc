@@ -706,15 +706,30 @@ extern "C" hexir_status_t hexir_cuda_linear_plan(
     uint32_t flags, uint32_t *variant, uint32_t *tile_n, uint32_t *split) {
   Call call;
   hexir_status_t status;
+  const bool reads =
+      op != HEXIR_PRODUCT_WEIGHT_GRAD && !(flags & HEXIR_LINEAR_PLAN_PLAIN);
+  flags &= ~HEXIR_LINEAR_PLAN_PLAIN;
   std::string bad = check_linear("linear_plan", HEXIR_DTYPE_BF16, 0, flags, &status);
   if (op > HEXIR_PRODUCT_WEIGHT_GRAD || !bad.empty())
     return call.refuse(bad.empty() ? "linear_plan: op is 0, 1 or 2" : bad);
+  if (!extents_ok(m, n, k))
+    return call.refuse("linear_plan: m, n or k is too large");
+  if (aligned & ~15)
+    return call.refuse("linear_plan: unknown bits in aligned");
+  auto is_aligned = [&](int part) {
+    return (aligned & (HEXIR_LINEAR_ALIGNED_ALL | part)) != 0;
+  };
   // Without a GPU: B200's 148 SMs.
   std::string error;
   DeviceState *dev = device_state(ordinal, &error);
-  const ProductPlan p = plan_product(op, m, n, k, aligned ? 0u : 2u,
-                                     op != HEXIR_PRODUCT_WEIGHT_GRAD, flags,
-                                     dev ? std::max(dev->sm_count, 2) : 148);
+  ProductPlan p;
+  if ((op == HEXIR_PRODUCT_WEIGHT_GRAD ? k : m) &&
+      (op == HEXIR_PRODUCT_INPUT_GRAD ? k : n))
+    p = plan_product(op, m, n, k,
+                     (is_aligned(HEXIR_LINEAR_ALIGNED_FIRST) ? 0u : 1u) +
+                         (is_aligned(HEXIR_LINEAR_ALIGNED_SECOND) ? 0u : 1u),
+                     reads || !is_aligned(HEXIR_LINEAR_ALIGNED_REST), flags,
+                     dev ? std::max(dev->sm_count, 2) : 148);
   if (!p.refusal.empty())
     return call.refuse("linear_plan: " + p.refusal);
   if (variant)
@@ -722,7 +737,7 @@ extern "C" hexir_status_t hexir_cuda_linear_plan(
   if (tile_n)
     *tile_n = p.tile_n;
   if (split)
-    *split = p.split;
+    *split = p.variant ? p.split : 0;
   return HEXIR_OK;
 }
 

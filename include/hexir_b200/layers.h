@@ -133,11 +133,21 @@ typedef struct {
 hexir_status_t hexir_cuda_linear_weight_grad(
     int ordinal, const hexir_linear_weight_grad_call_t *call, void *stream);
 
-/* Which kernel the three products would run on: *variant 1 = CTA pairs,
- * 2 = single CTAs, 3 = skinny, 4 = guarded; *tile_n its tile's columns,
- * *split the CTAs that share one tile's sum.  op 0 = hexir_cuda_linear,
- * 1 = input_grad, 2 = weight_grad; m, n, k as that call has them; aligned:
- * whether every row starts on a 16-byte boundary. */
+/* Which kernel a product would run on: *variant 1 = CTA pairs, 2 = single
+ * CTAs, 3 = skinny, 4 = guarded, 0 = none (an empty output); *tile_n its tile's
+ * columns, *split the CTAs that share one tile's sum.  op 0 = hexir_cuda_linear,
+ * 1 = input_grad, 2 = weight_grad; m, n, k and flags as that call has them.
+ * What else the choice depends on:
+ *   aligned  the tensors all of whose rows start on 16-byte boundaries:
+ *            HEXIR_LINEAR_ALIGNED_*, 1 for all and 0 for none;
+ *   flags    with HEXIR_LINEAR_PLAN_PLAIN the answer is for a call without
+ *            residual and without preactivations whose slope it takes;
+ *            without it, for one that has either (weight_grad has none). */
+#define HEXIR_LINEAR_ALIGNED_ALL 1
+#define HEXIR_LINEAR_ALIGNED_FIRST 2  /* x; dz; x (in the order of op) */
+#define HEXIR_LINEAR_ALIGNED_SECOND 4 /* w; w; dz */
+#define HEXIR_LINEAR_ALIGNED_REST 8   /* outputs, residual, preactivations */
+#define HEXIR_LINEAR_PLAN_PLAIN 0x1u
 hexir_status_t hexir_cuda_linear_plan(int ordinal, uint32_t op, uint32_t m,
                                       uint32_t n, uint32_t k, int aligned,
                                       uint32_t flags, uint32_t *variant,

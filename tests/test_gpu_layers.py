@@ -1047,3 +1047,50 @@ def test_norms_of_rows_shorter_than_16_bytes(dtype, cols, pad):
                                       (dgamma.numpy()[0], want[1], "dgamma"),
                                       (dbeta.numpy()[0], want[2], "dbeta")):
             assert_within(got, w, bound, f"{what}, shift {shift}")
+
+
+PLANNED = [("forward", 136, 5960, 8), ("forward", 300, 520, 1000), ("forward", 48, 512, 512),
+           ("forward", 777, 1001, 153), ("input_grad", 280, 8, 3416),
+           ("input_grad", 300, 520, 1000), ("weight_grad", 8, 4832, 144),
+           ("weight_grad", 513, 72, 2056)]
+
+
+@pytest.mark.parametrize("op,m,n,k", PLANNED)
+def test_the_plan_is_what_runs(op, m, n, k):
+    """The kernel a call would launch (an injected launch fault names it),
+    against linear_plan for the same facts: with and without what the epilogue
+    reads, with each tensor on 16-byte rows and off them."""
+    names = {1: "pair", 2: "single", 3: "skinny", 4: "guarded"}
+    shapes = {"forward": ((m, k), (k, n), (m, n)),
+              "input_grad": ((m, n), (k, n), (m, k)),
+              "weight_grad": ((m, k), (m, n), (k, n))}[op]
+
+    def tensor(shape, aligned):
+        rows, cols = shape
+        ld = -(-cols // 8) * 8 + (0 if aligned else 1)
+        return torch.zeros(rows, ld, device="cuda", dtype=torch.bfloat16)
+    for aligned in (14, 2, 4, 6, 12, 0):
+        a, b, out = (tensor(s, aligned >> 1 + i & 1) for i, s in enumerate(shapes))
+        for reads in (False, True):
+            if reads and op == "weight_grad":
+                continue
+            args = (0, a.data_ptr(), b.data_ptr(), out.data_ptr(), m, n, k)
+            r = out.data_ptr() if reads else 0
+            la, lb, lo = a.stride(0), b.stride(0), out.stride(0)
+            hx.fault_configure("launch:1")
+            try:
+                with pytest.raises(_ffi.HexirError) as err:
+                    if op == "forward":
+                        hx.cuda_linear(*args, residual=r, ldx=la, ldw=lb, ldy=lo,
+                                       ldr=lo, stream=stream())
+                    elif op == "input_grad":
+                        hx.cuda_linear_input_grad(*args, residual=r, lddz=la, ldw=lb,
+                                                  lddx=lo, ldr=lo, stream=stream())
+                    else:
+                        hx.cuda_linear_weight_grad(*args, ldx=la, lddz=lb, lddw=lo,
+                                                   stream=stream())
+            finally:
+                hx.fault_configure("")
+            plan = hx.linear_plan(op, m, n, k, aligned, plain=not reads)
+            assert f"hexir_linear_16 {names[plan[0]]}:" in str(err.value), \
+                (aligned, reads, plan, str(err.value))

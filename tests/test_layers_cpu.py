@@ -221,3 +221,33 @@ def test_rows_whose_blocks_reach_outside_their_tensor_are_edges(tmp_path):
     longer ones only the first and the last row are edges."""
     reach, needless = map(int, host_program("norm_places", tmp_path)[3:])
     assert reach == 0 and needless == 0
+
+
+def test_plans_follow_the_epilogue_and_what_is_aligned():
+    """What an epilogue reads, and outputs off 16 bytes, cost it more and leave
+    other kernels the cheapest; the plan is told of both."""
+    PAIR, SINGLE, GUARDED = 1, 2, 4
+    assert hx.linear_plan("forward", 136, 5960, 8)[0] == SINGLE
+    assert hx.linear_plan("forward", 136, 5960, 8, plain=True)[0] == PAIR
+    assert hx.linear_plan("input_grad", 280, 8, 3416)[0] == SINGLE
+    assert hx.linear_plan("input_grad", 280, 8, 3416, plain=True)[0] == PAIR
+    operands = _ffi.LINEAR_ALIGNED_FIRST | _ffi.LINEAR_ALIGNED_SECOND
+    assert hx.linear_plan("weight_grad", 8, 4832, 144) == \
+        hx.linear_plan("weight_grad", 8, 4832, 144, plain=True) == \
+        hx.linear_plan("weight_grad", 8, 4832, 144,
+                       operands | _ffi.LINEAR_ALIGNED_REST)
+    assert hx.linear_plan("weight_grad", 8, 4832, 144)[0] == PAIR
+    assert hx.linear_plan("weight_grad", 8, 4832, 144, operands)[0] == SINGLE
+    for part in (_ffi.LINEAR_ALIGNED_FIRST, _ffi.LINEAR_ALIGNED_SECOND):
+        assert hx.linear_plan("forward", 256, 512, 512,
+                              part | _ffi.LINEAR_ALIGNED_REST)[0] == GUARDED
+    for op, empty in (("forward", (0, 8, 8)), ("forward", (8, 0, 8)),
+                      ("input_grad", (8, 8, 0)), ("weight_grad", (8, 8, 0))):
+        assert hx.linear_plan(op, *empty) == (0, 0, 0)
+    assert hx.linear_plan("weight_grad", 0, 8, 8)[0] == GUARDED
+    for bad in (dict(aligned=16), dict(flags=2), dict(flags=0x1000)):
+        with pytest.raises(_ffi.HexirError):
+            hx.linear_plan("forward", 8, 8, 8, **bad)
+    with pytest.raises(_ffi.HexirError):
+        hx.linear_plan("forward", 2 ** 31, 8, 8)       # as the call itself refuses
+    assert linear(flags=_ffi.LINEAR_PLAN_PLAIN) == BAD  # the plan's alone
