@@ -479,10 +479,11 @@ def _activation(act) -> int:
 
 
 def _counts(together: int) -> None:
-    """Refuses counts that the calls' 32-bit fields would cut off: `together`
-    is all of them or-ed."""
+    """Refuses counts that the calls' fields would cut off: `together` is all
+    of 32 bits or-ed, and of those of 64 bits their upper half (n >> 32)."""
     if together >> 32:
-        raise ValueError("a negative size or flag, or one of 2**32 or more")
+        raise ValueError("a negative count or flag, or one beyond its field of 32 "
+                         "bits (64 for rows and workspace_bytes)")
 
 
 def cuda_linear(ordinal: int, x: int, w: int, y: int, m: int, n: int, k: int,
@@ -508,7 +509,7 @@ def cuda_linear_output_grad(ordinal: int, dy: int, m: int, n: int,
     """dz = dy * activation'(preact) and dbias = the column sums of dz
     (hexir_cuda_linear_output_grad); dbias needs a workspace of
     grad_workspace_bytes(n, dtype)."""
-    _counts(m | n)
+    _counts(m | n | workspace_bytes >> 32)
     call = _ffi.LinearOutputGradCall(_dtype(dtype), _activation(activation), m, n,
                                      dy, preact, dz, dbias, workspace,
                                      workspace_bytes, lddy, ldp, lddz)
@@ -555,6 +556,7 @@ def linear_plan(op: str, m: int, n: int, k: int, aligned: int = True,
     start on 16-byte boundaries, or those of the tensors of
     _ffi.LINEAR_ALIGNED_*; plain: a call without residual and preact whose
     slope it takes."""
+    _counts(m | n | k | flags)
     if plain:
         flags |= _ffi.LINEAR_PLAN_PLAIN
     ops = ("forward", "input_grad", "weight_grad")
@@ -568,6 +570,7 @@ def linear_plan(op: str, m: int, n: int, k: int, aligned: int = True,
 def grad_workspace_bytes(cols: int, dtype: str = "bf16") -> int:
     """Workspace of the two calls that sum over rows
     (hexir_cuda_grad_workspace)."""
+    _counts(cols)
     return lib().hexir_cuda_grad_workspace(cols, _dtype(dtype))
 
 
@@ -577,7 +580,7 @@ def cuda_layer_norm(ordinal: int, x: int, y: int, rows: int, cols: int,
                     ldy: int = 0, stream: int = 0) -> None:
     """y = (x - mean) * rstd * gamma + beta along each row; mean and rstd
     (optional outputs, [rows]) are f32, f64 for f64 (hexir_cuda_layer_norm)."""
-    _counts(cols | (rows if rows < 0 else 0))
+    _counts(cols | rows >> 32)
     call = _ffi.LayerNormCall(_dtype(dtype), cols, rows, eps, x, gamma, beta, y,
                               mean, rstd, ldx, ldy)
     check(lib().hexir_cuda_layer_norm(ordinal, C.byref(call), stream or None),
@@ -593,7 +596,7 @@ def cuda_layer_norm_grad(ordinal: int, dy: int, x: int, mean: int, rstd: int,
     """Layer norm's gradient: dx (+ residual), dgamma and dbeta
     (hexir_cuda_layer_norm_grad); dgamma and dbeta need a workspace of
     grad_workspace_bytes(cols, dtype)."""
-    _counts(cols | (rows if rows < 0 else 0))
+    _counts(cols | rows >> 32 | workspace_bytes >> 32)
     call = _ffi.LayerNormGradCall(_dtype(dtype), cols, rows, dy, x, mean, rstd,
                                   gamma, residual, dx, dgamma, dbeta, workspace,
                                   workspace_bytes, lddy, ldx, ldr, lddx)

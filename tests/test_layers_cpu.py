@@ -251,3 +251,24 @@ def test_plans_follow_the_epilogue_and_what_is_aligned():
     with pytest.raises(_ffi.HexirError):
         hx.linear_plan("forward", 2 ** 31, 8, 8)       # as the call itself refuses
     assert linear(flags=_ffi.LINEAR_PLAN_PLAIN) == BAD  # the plan's alone
+
+
+def test_every_count_that_a_field_would_cut_off_is_refused():
+    """Plans and workspace sizes too, and 64-bit counts: a workspace of -1 bytes
+    would pass for one of 2**64 - 1."""
+    for bad in (1 << 32, (1 << 32) + 1, -1):
+        for call in (lambda: hx.linear_plan("forward", bad, 64, 64),
+                     lambda: hx.linear_plan("weight_grad", 64, 64, bad),
+                     lambda: hx.linear_plan("forward", 64, 64, 64, flags=bad),
+                     lambda: hx.grad_workspace_bytes(bad)):
+            with pytest.raises(ValueError):
+                call()
+    for bad in (1 << 64, (1 << 64) + 3, -1):
+        for call in (lambda: hx.cuda_layer_norm(0, P, P, bad, 8),
+                     lambda: hx.cuda_layer_norm_grad(0, P, P, P, P, P, bad, 8),
+                     lambda: hx.cuda_layer_norm_grad(0, P, P, P, P, P, 8, 8, dbeta=P,
+                                                     workspace=P, workspace_bytes=bad),
+                     lambda: hx.cuda_linear_output_grad(0, P, 8, 8, dbias=P, workspace=P,
+                                                        workspace_bytes=bad)):
+            with pytest.raises(ValueError):
+                call()
