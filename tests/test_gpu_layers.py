@@ -1094,3 +1094,53 @@ def test_the_plan_is_what_runs(op, m, n, k):
             plan = hx.linear_plan(op, m, n, k, aligned, plain=not reads)
             assert f"hexir_linear_16 {names[plan[0]]}:" in str(err.value), \
                 (aligned, reads, plan, str(err.value))
+
+
+@pytest.mark.parametrize("dtype", ["f64", "f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,cols", [(3, 7), (3000, 40), (2500, 256), (1500, 1000),
+                                       (1300, 1024), (700, 1025), (700, 3001),
+                                       (330, 4096), (330, 5000), (170, 8192),
+                                       (170, 16384), (5, 16385)])
+def test_norms_of_tensors_that_lie_differently(dtype, rows, cols):
+    """Every tensor has an alignment and a stride of its own, so that rows go
+    element by element in every type, at the lengths where the kernels change;
+    several rows a block; the gradient also in place of the residual."""
+    rng = np.random.default_rng(rows + cols)
+    wide = "f64" if dtype == "f64" else "f32"
+    x = inputs(rng, rows, cols, dtype, 1, 1, 2.0, 1.0)
+    y = Tensor(rows, cols, dtype, 0, 2)
+    dy = inputs(rng, rows, cols, dtype, 2, 3)
+    residual = inputs(rng, rows, cols, dtype, 5, 2)
+    dx = Tensor(rows, cols, dtype, 16, 0)
+    gamma = inputs(rng, 1, cols, dtype, shift=1, scale=0.2, mean=1.0)
+    beta = inputs(rng, 1, cols, dtype, shift=3, scale=0.2)
+    mean, rstd = Tensor(1, rows, wide, shift=1), Tensor(1, rows, wide)
+    dgamma, dbeta = Tensor(1, cols, dtype, shift=1), Tensor(1, cols, dtype, shift=2)
+    size = hx.grad_workspace_bytes(cols, dtype)
+    work = torch.full((size + 64,), 0xA5, device="cuda", dtype=torch.uint8)
+    hx.cuda_layer_norm(0, x.ptr, y.ptr, rows, cols, dtype, gamma=gamma.ptr,
+                       beta=beta.ptr, mean=mean.ptr, rstd=rstd.ptr, eps=1e-5, ldx=x.ld,
+                       ldy=y.ld, stream=stream())
+    sync()
+    want = ref.layer_norm(x.numpy(), gamma.numpy()[0], beta.numpy()[0], 1e-5, dtype)
+    for t, (w, bound), what in ((y, want[0], "y"), (mean, want[1], "mean"),
+                                (rstd, want[2], "rstd")):
+        t.check_frame()
+        got = t.numpy()
+        assert_within(got if what == "y" else got[0], w, bound, what)
+    want = ref.layer_norm_grad(dy.numpy(), x.numpy(), mean.numpy()[0], rstd.numpy()[0],
+                               gamma.numpy()[0], residual.numpy(), dtype)
+    for out in (dx, residual):
+        hx.cuda_layer_norm_grad(0, dy.ptr, x.ptr, mean.ptr, rstd.ptr, out.ptr, rows,
+                                cols, dtype, gamma=gamma.ptr, dgamma=dgamma.ptr,
+                                dbeta=dbeta.ptr, residual=residual.ptr,
+                                workspace=work.data_ptr(), workspace_bytes=size,
+                                lddy=dy.ld, ldx=x.ld, lddx=out.ld, ldr=residual.ld,
+                                stream=stream())
+        sync()
+        assert bool((work[size:] == 0xA5).all()), "a write behind the workspace"
+        for t, (w, bound), what in ((out, want[0], "dx"), (dgamma, want[1], "dgamma"),
+                                    (dbeta, want[2], "dbeta")):
+            t.check_frame()
+            got = t.numpy()
+            assert_within(got if what == "dx" else got[0], w, bound, what)
