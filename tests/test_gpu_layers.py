@@ -1144,3 +1144,44 @@ def test_norms_of_tensors_that_lie_differently(dtype, rows, cols):
             t.check_frame()
             got = t.numpy()
             assert_within(got if what == "dx" else got[0], w, bound, what)
+
+
+def run_fresh(body):
+    """`body` in a process of its own, whose device code is not loaded yet."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    head = ("import torch\nimport hexir_b200 as hx\n"
+            "from tests.test_gpu_layers import Block, feed_forward, sync, stream\n")
+    done = subprocess.run([sys.executable, "-c", head + body], cwd=root, timeout=300,
+                          capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_an_empty_call_is_enough_before_a_capture():
+    """In a new process: one empty call, then a step whose kernels have never run
+    is captured, behind copies (nodes that are no kernels), and replayed."""
+    run_fresh("""
+hx.cuda_linear(0, 0, 0, 0, 0, 8, 8)
+shapes = [(260, 256, 1000), (3, 130, 515), (40, 1024, 4096)]
+blocks = [(Block(*s), feed_forward(*s, seed=1), feed_forward(*s, seed=2)) for s in shapes]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    on = torch.cuda.current_stream().cuda_stream
+    for block, p, fresh in blocks:
+        for k in p:
+            p[k].copy_(fresh[k])
+        block.forward(p, on)
+        block.backward(p, on)
+graph.replay()
+sync()
+for (block, p, fresh), s in zip(blocks, shapes):
+    other = Block(*s)
+    other.forward(fresh, stream())
+    other.backward(fresh, stream())
+    sync()
+    for (name, a), b in zip(block.outputs().items(), other.outputs().values()):
+        assert torch.equal(a, b), (s, name)
+""")
