@@ -1185,3 +1185,33 @@ for (block, p, fresh), s in zip(blocks, shapes):
     for (name, a), b in zip(block.outputs().items(), other.outputs().values()):
         assert torch.equal(a, b), (s, name)
 """)
+
+
+@pytest.mark.parametrize("dtype,size", [("bf16", 120), ("f32", 120), ("f64", 1016)])
+@pytest.mark.parametrize("cols,pad,shift", [(64, 0, 0), (40, 0, 0), (41, 0, 3), (41, 3, 1),
+                                            (100, 0, 0)])
+def test_gradient_of_constant_rows_of_large_numbers(dtype, size, cols, pad, shift):
+    """x - mean is 0 and xhat with it, although mean * rstd is beyond the type's
+    range: threads without an element of the row must not bring it in.  Results
+    and bounds are those of x = mean = 0, whose xhat is as exact."""
+    wide, rows = "f64" if dtype == "f64" else "f32", 30
+    rng = np.random.default_rng(cols)
+    x = Tensor(rows, cols, dtype, pad, shift, np.full((rows, cols), 2.0 ** size))
+    x.view[::2] *= -1
+    dy = inputs(rng, rows, cols, dtype, pad, shift)
+    mean = Tensor(1, rows, wide, data=x.numpy()[:, 0])
+    rstd = Tensor(1, rows, wide, data=np.full(rows, 512.0))
+    dx = Tensor(rows, cols, dtype, pad, shift)
+    dgamma, dbeta = Tensor(1, cols, dtype), Tensor(1, cols, dtype)
+    work = torch.empty(hx.grad_workspace_bytes(cols, dtype), device="cuda",
+                       dtype=torch.uint8)
+    hx.cuda_layer_norm_grad(0, dy.ptr, x.ptr, mean.ptr, rstd.ptr, dx.ptr, rows, cols,
+                            dtype, dgamma=dgamma.ptr, dbeta=dbeta.ptr,
+                            workspace=work.data_ptr(), workspace_bytes=work.numel(),
+                            lddy=dy.ld, ldx=x.ld, lddx=dx.ld, stream=stream())
+    sync()
+    want = ref.layer_norm_grad(dy.numpy(), np.zeros((rows, cols)), np.zeros(rows),
+                               rstd.numpy()[0], None, None, dtype)
+    assert_within(dx.numpy(), *want[0], "dx")
+    assert_within(dgamma.numpy()[0], *want[1], "dgamma")
+    assert_within(dbeta.numpy()[0], *want[2], "dbeta")
