@@ -1215,3 +1215,65 @@ def test_gradient_of_constant_rows_of_large_numbers(dtype, size, cols, pad, shif
     assert_within(dx.numpy(), *want[0], "dx")
     assert_within(dgamma.numpy()[0], *want[1], "dgamma")
     assert_within(dbeta.numpy()[0], *want[2], "dbeta")
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (3, 1, 9), (5, 9, 1), (63, 1001, 77),
+                                   (129, 7, 513), (200, 249, 129), (300, 515, 67)])
+@pytest.mark.parametrize("dtype,extra", [("bf16", 0), ("f16", 8)])
+def test_odd_extents_on_16_byte_rows_in_every_kernel(m, n, k, dtype, extra):
+    """Rows of any length inside buffers whose rows start on 16-byte (and, by
+    `extra`, not on 32-byte) boundaries: what lies in the gaps is NaN."""
+    rng = np.random.default_rng(m + n + k)
+
+    def padded(rows, cols, data=None):
+        t = Tensor(rows, cols, dtype, -cols % 8 + extra,
+                   data=normal(rng, (rows, cols)) if data is None else data)
+        keep = t.view.clone()
+        t.flat.fill_(float("nan"))
+        t.view.copy_(keep)
+        return t
+    x, w, wt = padded(m, k), padded(k, n), padded(n, k)
+    xt, r, z0 = padded(k, m), padded(m, n), padded(m, n)
+    on = stream()
+    flags = [0, GUARDED | _ffi.LINEAR_SPLIT(2), SINGLE | _ffi.LINEAR_SPLIT(1),
+             SINGLE | _ffi.LINEAR_TILE(64) | _ffi.LINEAR_SPLIT(4),
+             PAIR | _ffi.LINEAR_TILE(128), PAIR | _ffi.LINEAR_TILE(256)]
+    for flag in flags + ([SKINNY, SKINNY | _ffi.LINEAR_SPLIT(4)] if m <= 64 else []):
+        y, z, dx, dw = (Tensor(m, n, dtype, -n % 8 + extra) for _ in range(4))
+        hx.cuda_linear(0, x.ptr, w.ptr, y.ptr, m, n, k, dtype, "gelu",
+                       bias=r.ptr, residual=r.ptr, preact=z.ptr, ldx=x.ld, ldw=w.ld,
+                       ldy=y.ld, ldr=r.ld, ldp=z.ld, flags=flag, stream=on)
+        if not flag & SKINNY:
+            hx.cuda_linear_input_grad(0, x.ptr, wt.ptr, dx.ptr, m, k, n, dtype, "swish",
+                                      preact=z0.ptr, residual=r.ptr, lddz=x.ld,
+                                      ldw=wt.ld, lddx=dx.ld, ldp=z0.ld, ldr=r.ld,
+                                      flags=flag, stream=on)
+            hx.cuda_linear_weight_grad(0, xt.ptr, w.ptr, dw.ptr, k, n, m, dtype,
+                                       ldx=xt.ld, lddz=w.ld, lddw=dw.ld, flags=flag,
+                                       stream=on)
+        sync()
+        for t in (y, z, dx, dw):
+            t.check_frame()
+        want = ref.linear(x.numpy(), w.numpy(), r.numpy()[0], "gelu", r.numpy(), dtype)
+        assert_within(y.numpy(), want[0], want[1], f"y {flag:#x}")
+        assert_within(z.numpy(), want[2], want[3], f"z {flag:#x}")
+        if not flag & SKINNY:
+            assert_within(dx.numpy(), *ref.product(
+                x.numpy(), wt.numpy().T, dtype, "swish", z0.numpy(), r.numpy()),
+                f"dx {flag:#x}")
+            assert_within(dw.numpy(), *ref.product(xt.numpy().T, w.numpy(), dtype),
+                          f"dw {flag:#x}")
+
+
+def test_layers_through_the_packages_own_buffers_and_streams():
+    """Without torch: the framework's device buffers, on the device's stream."""
+    rows, cols = 37, 64
+    rng = np.random.default_rng(5)
+    dev = hx.Device("cuda")
+    x = rng.standard_normal((rows, cols)).astype(np.float32)
+    bx, by = dev.buffer(x.nbytes), dev.buffer(x.nbytes)
+    bx.write(x)
+    hx.cuda_layer_norm(0, bx.ptr, by.ptr, rows, cols, "f32", eps=1e-5, stream=dev.stream)
+    hx.cuda_synchronize(0, dev.stream)
+    (want, bound), _, _ = ref.layer_norm(x.astype(np.float64), None, None, 1e-5, "f32")
+    assert_within(by.read((rows, cols), np.float32).astype(np.float64), want, bound, "y")
