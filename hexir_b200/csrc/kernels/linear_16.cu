@@ -647,10 +647,12 @@ struct Blocks {
   uint32_t apart;  // bit i: chunk i is to be taken element by element
 };
 
-// A load that stays where it is written.
+// A load that stays where it is written.  Not a non-coherent one: those want
+// memory that nothing writes during the kernel, which begins, up to its
+// griddep_wait, while the kernel before may still write the operands.
 __device__ __forceinline__ uint4 load_now(uintptr_t at) {
   uint4 w;
-  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];"
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
                : "l"(at)
                : "memory");

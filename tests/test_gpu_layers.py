@@ -1277,3 +1277,57 @@ def test_layers_through_the_packages_own_buffers_and_streams():
     hx.cuda_synchronize(0, dev.stream)
     (want, bound), _, _ = ref.layer_norm(x.astype(np.float64), None, None, 1e-5, "f32")
     assert_within(by.read((rows, cols), np.float32).astype(np.float64), want, bound, "y")
+
+
+@pytest.mark.parametrize("rows,cols", [(150, 131), (700, 259), (131, 1027)])
+def test_calls_back_to_back_read_what_the_call_before_wrote(rows, cols):
+    """A chain of calls that read each other's outputs, off 16 bytes and in
+    buffers that every round writes anew (so that an old line of a cache would
+    show), queued without a pause, against the same chain with a pause after each
+    call."""
+    rng = np.random.default_rng(rows)
+    start = normal(rng, (rows, cols))
+    w = inputs(rng, cols, cols, "bf16", 1, 1, scale=cols ** -0.5)
+
+    def chain(pause):
+        a, b = (Tensor(rows, cols, "bf16", 1, 1, start) for _ in range(2))
+        dw = Tensor(cols, cols, "bf16", 1, 1)
+        dbias = Tensor(1, cols, "bf16")
+        work = torch.empty(hx.grad_workspace_bytes(cols), device="cuda",
+                           dtype=torch.uint8)
+        on = stream()
+        seen = []
+        for _ in range(12):
+            for call in (
+                    lambda: hx.cuda_linear(0, a.ptr, w.ptr, b.ptr, rows, cols, cols,
+                                           residual=b.ptr, ldx=a.ld, ldw=w.ld, ldy=b.ld,
+                                           ldr=b.ld, stream=on),
+                    lambda: hx.cuda_layer_norm(0, b.ptr, a.ptr, rows, cols, "bf16",
+                                               ldx=b.ld, ldy=a.ld, stream=on),
+                    lambda: hx.cuda_linear_weight_grad(0, a.ptr, b.ptr, dw.ptr, rows,
+                                                       cols, cols, ldx=a.ld, lddz=b.ld,
+                                                       lddw=dw.ld, stream=on),
+                    lambda: hx.cuda_linear_input_grad(0, b.ptr, w.ptr, a.ptr, rows, cols,
+                                                      cols, residual=a.ptr, lddz=b.ld,
+                                                      ldw=w.ld, lddx=a.ld, ldr=a.ld,
+                                                      stream=on),
+                    lambda: hx.cuda_linear_output_grad(0, a.ptr, rows, cols, "bf16",
+                                                       "swish", preact=b.ptr, dz=a.ptr,
+                                                       dbias=dbias.ptr,
+                                                       workspace=work.data_ptr(),
+                                                       workspace_bytes=work.numel(),
+                                                       lddy=a.ld, ldp=b.ld, lddz=a.ld,
+                                                       stream=on),
+                    lambda: hx.cuda_layer_norm(0, a.ptr, a.ptr, rows, cols, "bf16",
+                                               ldx=a.ld, ldy=a.ld, stream=on)):
+                call()
+                if pause:
+                    sync()
+            seen.append([t.view.clone() for t in (a, b, dw, dbias)])
+        sync()
+        return seen
+    want = chain(True)
+    for _ in range(10):
+        for i, (got, expected) in enumerate(zip(chain(False), want)):
+            for name, g, e in zip(("a", "b", "dw", "dbias"), got, expected):
+                assert torch.equal(g, e), (i, name)
