@@ -75,7 +75,7 @@ __device__ __forceinline__ float sigmoid_near(float z) {
 // t in [1/6, 1], by reweighted least squares in extended precision) is within
 // 4.3e-8 of it.  Where t is below 1/6 (|z| > 14.1, without bound), e^(-z^2 / 2)
 // is below 2^-144, the last bits of f32's smallest numbers, or 0, and P, which
-// stays near 0.14, does not matter.  Above 0, Phi(z) = 1 - Phi(-z).
+// stays between 0.14 and 0.17, does not matter.  Above 0, Phi(z) = 1 - Phi(-z).
 __device__ __forceinline__ void normal_cdf(const Two<float> &z, Two<float> &phi,
                                            Two<float> &e) {
   const Two<float> t = {

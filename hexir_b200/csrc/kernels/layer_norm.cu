@@ -6,9 +6,9 @@
 // each pass reads its tensors once: forward x -> y, backward x, dy
 // (, residual) -> dx.  Both are bound by HBM; rows longer than a block holds
 // are read again from L2.  16384 x 4096, forward / gradient with its sums, and
-// the share of the measured copy bandwidth: bf16 45.0 / 75.2 us (0.91 / 0.82),
-// f32 91 / 134 (0.90 / 0.92), f64 186 / 264 (0.88 / 0.93).  The 16-bit gradient
-// is as much bound by its conversions (issue slots 57 % busy at two blocks an
+// the share of the measured copy bandwidth: bf16 45.1 / 75.1 us (0.91 / 0.82),
+// f32 85.6 / 134 (0.96 / 0.92), f64 190 / 261 (0.86 / 0.94).  The 16-bit gradient
+// is as much bound by its conversions (issue slots 59 % busy at two blocks an
 // SM; three, with their sums spilled, took 117 us).
 //
 // The gradients of gamma, beta and the bias are sums over rows: each block

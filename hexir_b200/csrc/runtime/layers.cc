@@ -557,7 +557,8 @@ ProductPlan plan_product(uint32_t op, uint32_t m, uint32_t n, uint32_t k,
   if (forced_split)
     p.split = forced_split;
   // One CTA per SM with a deep ring, or, where there are more and their
-  // epilogues need no slots, two whose main loops and epilogues overlap.
+  // epilogues need no slots, two whose main loops and epilogues overlap (the
+  // same shared memory for guarded loads, of which one fits by its registers).
   const uint64_t ctas = static_cast<uint64_t>(p.tiles_m) * p.tiles_n * p.split;
   const uint32_t epilogue =
       slots && p.variant != kSkinny
