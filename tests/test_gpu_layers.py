@@ -1282,7 +1282,7 @@ def test_layers_through_the_packages_own_buffers_and_streams():
 @pytest.mark.parametrize("rows,cols", [(150, 131), (700, 259), (131, 1027)])
 def test_calls_back_to_back_read_what_the_call_before_wrote(rows, cols):
     """A chain of calls that read each other's outputs, off 16 bytes and in
-    buffers that every round writes anew (so that an old line of a cache would
+    buffers that every pass writes anew (so that an old line of a cache would
     show), queued without a pause, against the same chain with a pause after each
     call."""
     rng = np.random.default_rng(rows)
